@@ -25,6 +25,14 @@ from .flash_gqa import (  # noqa: F401
     launch_flash_swa_forward_bf16_kernel,
     set_exchange_wait_limit,
 )
+from .kv8 import (  # noqa: F401
+    KV8Cache,
+    attention_weight_sums,
+    kv8_append,
+    kv8_cache,
+    kv8_decode,
+    kv8_evict,
+)
 from .sharded import (  # noqa: F401
     KVShardedDecoder,
     shard_batch,

@@ -16,6 +16,8 @@ E_DEVICE_TIMEOUT = -6
 KV_BSHD = 0
 KV_BHSD = 1
 WS_COUNTERS_ZERO = 0x100
+FMT_E4M3 = 0
+FMT_INT8 = 1
 
 _lib = None
 
@@ -50,6 +52,14 @@ _SIGNATURES = {
     "cllo_swa_prefill_fwd_bf16": (_i, [_vp, _vp, _vp, _f, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "cllo_mla_prefill_fwd_bf16": (_i, [_vp, _vp, _vp, _f, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "cllo_sgqa_prefill_fwd_bf16": (_i, [_vp, _vp, _vp, _vp, _i, _f, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "cllo_kv8_append_bf16": (_i, [_vp, ctypes.POINTER(_ll), _vp, ctypes.POINTER(_ll), _vp, _vp, _vp, _vp, _vp, _vp, _i, _i,
+                                  _i, _i, _i, _i, _i, _i, _vp]),
+    "cllo_kv8_decode_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "cllo_kv8_decode_bf16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _i,
+                                  _i, _vp]),
+    "cllo_attn_weight_sums_bf16": (_i, [_vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "cllo_kv8_evict": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i,
+                            _i, _i, _i, _vp]),
     "cllo_gqa_decode_bf16_noalloc": (_i, [_vp, _vp, _vp, _f, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "cllo_gqa_decode_bf16_compat": (_i, [_vp, _vp, _vp, _f, _vp, _vp, _i, _i, _i, _i, _i]),
 }

@@ -7,6 +7,10 @@
 #include "rope.cuh"
 #include "sgqa_prefill.cuh"
 #include "mla_prefill.cuh"
+#include "kv8_append.cuh"
+#include "kv8_decode.cuh"
+#include "kv8_evict.cuh"
+#include "weight_sums.cuh"
 
 #include <cstdio>
 #include <cstring>
@@ -363,6 +367,45 @@ int cllo_sgqa_prefill_fwd_bf16(const void* q, const void* k, const void* v, cons
                                int Hq, int Hkv, int D, void* stream) {
     return sgqa::launch(q, k, v, sparse_kv_indices, num_sparse_kv, scale, causal, o, lse, B, Sq, Skv, Hq, Hkv, D,
                         static_cast<cudaStream_t>(stream));
+}
+
+int cllo_kv8_append_bf16(const void* k_new, const long long k_strides[3], const void* v_new, const long long v_strides[3],
+                         const int* seq_lens, const int* new_lens, void* k_cache, void* v_cache, float* k_scale,
+                         float* v_scale, int B, int T, int capacity, int Hkv, int D, int kv_layout, int block_tokens,
+                         int format, void* stream) {
+    return kv8::append_launch(k_new, k_strides, v_new, v_strides, seq_lens, new_lens, k_cache, v_cache, k_scale, v_scale,
+                              B, T, capacity, Hkv, D, kv_layout, block_tokens, format, static_cast<cudaStream_t>(stream));
+}
+
+size_t cllo_kv8_decode_workspace_bytes(int B, int capacity, int Hq, int Hkv, int D, int with_weights, int num_workers) {
+    (void)num_workers;
+    return kv8::decode_workspace_bytes(B, capacity, Hq, Hkv, D, with_weights);
+}
+
+int cllo_kv8_decode_bf16(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                         const float* v_scale, const int* seq_lens, float scale, void* o, float* lse, float* weights,
+                         void* workspace, size_t workspace_bytes, int B, int capacity, int Hq, int Hkv, int D,
+                         int kv_layout, int block_tokens, int format, int num_workers, void* stream) {
+    return kv8::decode_launch(q, k_cache, v_cache, k_scale, v_scale, seq_lens, scale, o, lse, weights, workspace,
+                              workspace_bytes, B, capacity, Hq, Hkv, D, kv_layout & ~CLLO_WS_COUNTERS_ZERO, block_tokens,
+                              format, num_workers, static_cast<cudaStream_t>(stream));
+}
+
+int cllo_attn_weight_sums_bf16(const void* q, const void* k, const float* lse, const int* seq_lens, float scale, int causal,
+                               int q_start, int window, int accumulate, float* sums, int B, int Sq, int Skv, int Hq,
+                               int Hkv, int D, void* stream) {
+    return sums::launch(q, k, lse, seq_lens, scale, causal, q_start, window, accumulate, sums, B, Sq, Skv, Hq, Hkv, D,
+                        static_cast<cudaStream_t>(stream));
+}
+
+int cllo_kv8_evict(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                   const float* weights, const int* seq_lens, void* k_to, void* v_to, float* k_scale_to,
+                   float* v_scale_to, float* weights_to, int* new_lens, int* indices, int B, int capacity,
+                   int capacity_to, int Hkv, int D, int budget, int sink, int recent, int kv_layout, int block_tokens,
+                   int format, void* stream) {
+    return kv8::evict_launch(k_cache, v_cache, k_scale, v_scale, weights, seq_lens, k_to, v_to, k_scale_to, v_scale_to,
+                             weights_to, new_lens, indices, B, capacity, capacity_to, Hkv, D, budget, sink, recent,
+                             kv_layout, block_tokens, format, static_cast<cudaStream_t>(stream));
 }
 
 // Decode for callers that may not allocate device memory: the partials go to the fixed array above.

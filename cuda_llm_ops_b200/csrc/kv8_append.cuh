@@ -1,0 +1,169 @@
+// Append to the 8-bit KV cache: bf16 K/V rows -> codes and block scales.
+//
+// One thread block handles one (batch, kv head, cache block, K or V).  Of the cache block's rows some may be old (the
+// sequence ended inside it), some are new, the rest lie behind the sequence and are left alone:
+//     scale' = max(scale of the old rows, 2^e(amax of the new rows)),   code = rne(x / scale'),
+// and the old rows are re-rounded to scale' only if it grew.  The scale is that of format kv8_format.cuh: powers of two,
+// so x / scale' is a product and exact.
+//
+// Bound by memory: 2 B read and 1 B written per value.  The new rows are loaded once, 16 bytes per lane (half a warp per
+// row), and wait in registers for the block's amax.
+#pragma once
+
+#include "host_util.cuh"
+#include "kv8_format.cuh"
+
+namespace cllo {
+namespace kv8 {
+
+constexpr int kAppendThreads = 128;
+constexpr int kRowsPerPass = kAppendThreads / 16;  // half a warp per row
+
+struct AppendParams {
+    const __nv_bfloat16* src[2];  // K rows, V rows
+    RowStrides src_stride[2];
+    uint8_t* cache[2];
+    float* scale[2];  // [B, Hkv, n_blocks]
+    RowStrides stride;
+    const int* seq_lens;
+    const int* new_lens;  // nullable
+    int T, capacity, Hkv, n_blocks, blocks_touched;
+};
+
+template <int kFmt, int kBlock>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+    __shared__ float warp_amax[kAppendThreads / 32];
+    long long id = blockIdx.x;
+    const int which = blockIdx.y;
+    const int j = static_cast<int>(id % p.blocks_touched);
+    id /= p.blocks_touched;
+    const int h = static_cast<int>(id % p.Hkv), b = static_cast<int>(id / p.Hkv);
+    const int held = clamp_len(p.seq_lens[b], p.capacity);
+    int n = p.new_lens ? clamp_len(p.new_lens[b], p.T) : p.T;
+    if (n > p.capacity - held) n = p.capacity - held;
+    const int blk = held / kBlock + j;
+    const int row0 = blk * kBlock;  // first position of the cache block
+    if (n <= 0 || row0 >= held + n) return;
+
+    const int r_in = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
+    const __nv_bfloat16* src = p.src[which] + b * p.src_stride[which].batch + h * p.src_stride[which].head + c8;
+    uint8_t* dst = p.cache[which] + b * p.stride.batch + h * p.stride.head + c8;
+    float* scale = p.scale[which] + (static_cast<long long>(b) * p.Hkv + h) * p.n_blocks + blk;
+
+    constexpr int kPasses = kBlock / kRowsPerPass;
+    uint4 x[kPasses];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const int pos = row0 + i * kRowsPerPass + r_in;
+        x[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (pos >= held && pos < held + n)
+            x[i] = __ldg(reinterpret_cast<const uint4*>(src + (pos - held) * p.src_stride[which].token));
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            amax = fmaxf(amax, fmaxf(finite_abs(bf16_lo(w[e])), finite_abs(bf16_hi(w[e]))));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if ((threadIdx.x & 31) == 0) warp_amax[threadIdx.x >> 5] = amax;
+    const bool has_old = row0 < held;
+    const float old_scale = has_old ? *scale : 0.f;
+    __syncthreads();  // also: every thread has read the old scale before one of them writes the new one
+#pragma unroll
+    for (int i = 0; i < kAppendThreads / 32; ++i) amax = fmaxf(amax, warp_amax[i]);
+    const int e_new = scale_exp<kFmt>(amax);
+    float s = exp2_int(e_new), inv = exp2_int(-e_new);
+    if (has_old && old_scale >= s) {
+        s = old_scale;
+        inv = 1.f / old_scale;
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const int pos = row0 + i * kRowsPerPass + r_in;
+        uint2* at = reinterpret_cast<uint2*>(dst + pos * p.stride.token);
+        if (pos >= held && pos < held + n) {
+            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            uint2 c;
+            c.x = encode4<kFmt>(bf16_lo(w[0]) * inv, bf16_hi(w[0]) * inv, bf16_lo(w[1]) * inv, bf16_hi(w[1]) * inv);
+            c.y = encode4<kFmt>(bf16_lo(w[2]) * inv, bf16_hi(w[2]) * inv, bf16_lo(w[3]) * inv, bf16_hi(w[3]) * inv);
+            *at = c;
+        } else if (has_old && pos < held && s != old_scale) {
+            const uint2 c = *at;
+            const float ratio = old_scale * inv;
+            float v[8];
+            decode4<kFmt>(c.x, *reinterpret_cast<float(*)[4]>(v));
+            decode4<kFmt>(c.y, *reinterpret_cast<float(*)[4]>(v + 4));
+            uint2 d;
+            d.x = encode4<kFmt>(v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio);
+            d.y = encode4<kFmt>(v[4] * ratio, v[5] * ratio, v[6] * ratio, v[7] * ratio);
+            *at = d;
+        }
+    }
+    if (threadIdx.x == 0) *scale = s;
+}
+
+template <int kFmt>
+static void append_dispatch(const AppendParams& p, int block, dim3 grid, cudaStream_t st) {
+    switch (block) {
+        case 16: append_kernel<kFmt, 16><<<grid, kAppendThreads, 0, st>>>(p); break;
+        case 32: append_kernel<kFmt, 32><<<grid, kAppendThreads, 0, st>>>(p); break;
+        case 64: append_kernel<kFmt, 64><<<grid, kAppendThreads, 0, st>>>(p); break;
+        default: append_kernel<kFmt, 128><<<grid, kAppendThreads, 0, st>>>(p); break;
+    }
+}
+
+static int append_launch(const void* k_new, const long long* k_strides, const void* v_new, const long long* v_strides,
+                         const int* seq_lens, const int* new_lens, void* k_cache, void* v_cache, float* k_scale,
+                         float* v_scale, int B, int T, int capacity, int Hkv, int D, int kv_layout, int block, int format,
+                         cudaStream_t st) {
+    if (!k_new || !v_new || !k_strides || !v_strides || !seq_lens || !k_cache || !v_cache || !k_scale || !v_scale)
+        return CLLO_E_BAD_ARG;
+    if (B <= 0 || T <= 0 || capacity <= 0 || Hkv <= 0 || D <= 0) return CLLO_E_BAD_ARG;
+    if (kv_layout != CLLO_KV_BSHD && kv_layout != CLLO_KV_BHSD) return CLLO_E_BAD_ARG;
+    if (!valid_format(format) || !valid_block(block)) return CLLO_E_BAD_ARG;
+    if (D != kD || T > kMaxCapacity || capacity > kMaxCapacity) return CLLO_E_UNSUPPORTED;
+    if (!aligned_to(k_new, 16) || !aligned_to(v_new, 16) || !aligned_to(k_cache, 16) || !aligned_to(v_cache, 16) ||
+        !aligned_to(seq_lens, 4) || !aligned_to(new_lens, 4) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
+        return CLLO_E_BAD_ARG;
+    for (int i = 0; i < 3; ++i)
+        if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0) return CLLO_E_BAD_ARG;  // 16-byte loads of whole rows
+    DeviceInfo* di = nullptr;
+    int rc = current_device_info(&di);
+    if (rc != CLLO_OK) return rc;
+    if (di->cc_major != 10) return CLLO_E_UNSUPPORTED;
+    AppendParams p;
+    p.src[0] = static_cast<const __nv_bfloat16*>(k_new);
+    p.src[1] = static_cast<const __nv_bfloat16*>(v_new);
+    p.src_stride[0] = {k_strides[0], k_strides[1], k_strides[2]};
+    p.src_stride[1] = {v_strides[0], v_strides[1], v_strides[2]};
+    p.cache[0] = static_cast<uint8_t*>(k_cache);
+    p.cache[1] = static_cast<uint8_t*>(v_cache);
+    p.scale[0] = k_scale;
+    p.scale[1] = v_scale;
+    p.stride = cache_strides(kv_layout, capacity, Hkv);
+    p.seq_lens = seq_lens;
+    p.new_lens = new_lens;
+    p.T = T;
+    p.capacity = capacity;
+    p.Hkv = Hkv;
+    p.n_blocks = (capacity + block - 1) / block;
+    // T tokens starting anywhere inside a block reach this many blocks at most
+    const int touched = (T - 1 + block - 1) / block + 1;
+    p.blocks_touched = touched < p.n_blocks ? touched : p.n_blocks;
+    const long long blocks = static_cast<long long>(B) * Hkv * p.blocks_touched;
+    if (blocks > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
+    const dim3 grid(static_cast<unsigned>(blocks), 2);
+    if (format == CLLO_FMT_E4M3)
+        append_dispatch<CLLO_FMT_E4M3>(p, block, grid, st);
+    else
+        append_dispatch<CLLO_FMT_INT8>(p, block, grid, st);
+    CLLO_CUDA_TRY(cudaGetLastError());
+    return CLLO_OK;
+}
+
+}  // namespace kv8
+}  // namespace cllo

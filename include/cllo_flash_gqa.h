@@ -300,6 +300,75 @@ int cllo_swa_bwd_bf16(const void* q, const void* k, const void* v, const void* o
  */
 int cllo_rope_bf16(const void* input, void* output, int B, int S, int hidden, float base, void* stream);
 
+/*
+ * 8-bit KV cache (no upstream counterpart).  K and V are held as one byte per value -- e4m3 or a signed integer -- with
+ * one fp32 scale per (batch, kv head, block of block_tokens tokens) for K and one for V; a value is code * scale.
+ *   caches  [B,S,Hkv,D] or [B,Hkv,S,D] bytes by kv_layout, S = capacity in tokens, contiguous, 16-byte aligned
+ *   scales  [B,Hkv,ceil(capacity / block_tokens)] fp32;  block_tokens = 16, 32, 64 or 128
+ * The library writes power-of-two scales: the smallest 2^e, -60 <= e <= 60, with amax <= qmax * 2^e over the block's
+ * finite values (qmax = 448 or 127); infinities and what is beyond 2^60 * qmax saturate, a NaN is kept by e4m3 and becomes
+ * 0 as an integer.  The attention reads any positive scales within [2^-60, 2^60].
+ * seq_lens [B] int32 are lengths on the device, so a captured graph follows them; a length outside [0, capacity] is held
+ * to that range.  capacity <= 2^30.  D = 128.
+ */
+#define CLLO_FMT_E4M3 0
+#define CLLO_FMT_INT8 1
+
+/*
+ * Append: k_new / v_new bf16 rows of up to T tokens per sequence become positions [seq_lens[b], seq_lens[b] + n) of the
+ * cache, n = new_lens[b] (nullable: T for all), held to [0, T] and to the room that is left.  k_strides / v_strides are
+ * HOST arrays {batch, token, head} in elements (multiples of 8; rows of 128 values are contiguous), so that slices of a
+ * fused projection need no copy.  A block that holds old rows keeps its scale unless the new rows need a larger one, in
+ * which case the old rows are re-rounded to it; positions behind the new rows are not written.  seq_lens is not changed.
+ */
+int cllo_kv8_append_bf16(const void* k_new, const long long k_strides[3], const void* v_new, const long long v_strides[3],
+                         const int* seq_lens, const int* new_lens, void* k_cache, void* v_cache, float* k_scale,
+                         float* v_scale, int B, int T, int capacity, int Hkv, int D, int kv_layout, int block_tokens,
+                         int format, void* stream);
+
+/*
+ * Single-token decode over the cache: o[b,h] = softmax(scale * q[b,h] . K[b,:len]) V[b,:len], len = seq_lens[b];
+ * q, o [B,Hq,D] bf16, lse [B,Hq] fp32 (nullable).  A sequence of length 0 gives zeros and lse = -inf.
+ * weights (nullable, fp32 [B,Hkv,capacity]): the step's probabilities, summed over the query heads of each group, are
+ * ADDED to weights[b,h,0..len).
+ * workspace: cllo_kv8_decode_workspace_bytes(...) bytes, 256-byte aligned, contents arbitrary; calls that may overlap on
+ * the GPU need one each.  kv_layout may carry CLLO_WS_COUNTERS_ZERO as in cllo_gqa_decode_bf16.  num_workers: 0 = chosen
+ * by the library.
+ */
+size_t cllo_kv8_decode_workspace_bytes(int B, int capacity, int Hq, int Hkv, int D, int with_weights, int num_workers);
+int cllo_kv8_decode_bf16(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                         const float* v_scale, const int* seq_lens, float scale, void* o, float* lse, float* weights,
+                         void* workspace, size_t workspace_bytes, int B, int capacity, int Hq, int Hkv, int D,
+                         int kv_layout, int block_tokens, int format, int num_workers, void* stream);
+
+/*
+ * Weight sums of a prompt: sums[b,h,t] = sum over the heads g of the group and the counted query rows i of
+ * e^(scale * q[b,g,i] . k[b,h,t] - lse[b,g,i]); with causal != 0 only t <= q_start + i.  q [B,Hq,Sq,D], k [B,Hkv,Skv,D]
+ * bf16, lse [B,Hq,Sq] as the forward wrote it (rows with lse = -inf add nothing), sums fp32 [B,Hkv,Skv], added to when
+ * accumulate != 0.
+ * seq_lens (nullable) [B]: keys at t >= seq_lens[b] get 0, and with causal != 0 query rows at positions
+ * q_start + i >= seq_lens[b] (the padding of a batch) do not count.  window > 0: only the last `window` query
+ * positions before seq_lens[b] count -- the last rows of q where no lengths are given or the mask is not causal.
+ */
+int cllo_attn_weight_sums_bf16(const void* q, const void* k, const float* lse, const int* seq_lens, float scale, int causal,
+                               int q_start, int window, int accumulate, float* sums, int B, int Sq, int Skv, int Hq,
+                               int Hkv, int D, void* stream);
+
+/*
+ * Eviction by accumulated weight.  Per (batch, kv head) the cache's first `sink` and last `recent` tokens stay, and of the
+ * others the budget - sink - recent with the largest weights[b,h,t] (of equal weights the earliest; NaN counts as
+ * largest); a sequence within the budget stays whole.  What stays moves, in order, to the second cache (same layout, block
+ * size and format; capacity_to >= min(budget, capacity)), whose block scales are computed anew; weights_to (nullable,
+ * [B,Hkv,capacity_to]) receives the kept weights, indices [B,Hkv,budget] the kept positions (-1 behind them) and
+ * new_lens [B] = min(seq_lens, budget).  Rows behind new_lens are left as they were.  No tensor written to may overlap one
+ * that is read (CLLO_E_BAD_ARG).
+ */
+int cllo_kv8_evict(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                   const float* weights, const int* seq_lens, void* k_to, void* v_to, float* k_scale_to,
+                   float* v_scale_to, float* weights_to, int* new_lens, int* indices, int B, int capacity,
+                   int capacity_to, int Hkv, int D, int budget, int sink, int recent, int kv_layout, int block_tokens,
+                   int format, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
