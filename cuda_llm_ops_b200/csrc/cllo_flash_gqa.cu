@@ -378,8 +378,12 @@ int cllo_kv8_append_bf16(const void* k_new, const long long k_strides[3], const 
 }
 
 size_t cllo_kv8_decode_workspace_bytes(int B, int capacity, int Hq, int Hkv, int D, int with_weights, int num_workers) {
-    (void)num_workers;
-    return kv8::decode_workspace_bytes(B, capacity, Hq, Hkv, D, with_weights);
+    int sm = 256;  // no device visible: an upper bound for any current part
+    DeviceInfo* di = nullptr;
+    if (num_workers <= 0 && current_device_info(&di) == CLLO_OK && di->sm_count > 0) sm = di->sm_count;
+    kv8::DecodePlan plan;
+    if (kv8::make_decode_plan(B, capacity, Hq, Hkv, D, with_weights != 0, num_workers, sm, &plan) != CLLO_OK) return 0;
+    return plan.bytes;
 }
 
 int cllo_kv8_decode_bf16(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -387,7 +391,7 @@ int cllo_kv8_decode_bf16(const void* q, const void* k_cache, const void* v_cache
                          void* workspace, size_t workspace_bytes, int B, int capacity, int Hq, int Hkv, int D,
                          int kv_layout, int block_tokens, int format, int num_workers, void* stream) {
     return kv8::decode_launch(q, k_cache, v_cache, k_scale, v_scale, seq_lens, scale, o, lse, weights, workspace,
-                              workspace_bytes, B, capacity, Hq, Hkv, D, kv_layout & ~CLLO_WS_COUNTERS_ZERO, block_tokens,
+                              workspace_bytes, B, capacity, Hq, Hkv, D, kv_layout, block_tokens,
                               format, num_workers, static_cast<cudaStream_t>(stream));
 }
 

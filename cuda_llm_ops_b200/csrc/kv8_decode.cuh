@@ -2,130 +2,715 @@
 //
 //   s_t = scale * q . (kscale_blk(t) * k8_t),  o = sum_t softmax(s)_t * vscale_blk(t) * v8_t,  lse = log sum_t e^(s_t)
 //
-// over the sequence_lens[b] tokens that the cache holds of sequence b; with `weights`, the probabilities of the step are
+// over the seq_lens[b] tokens that the cache holds of sequence b; with `weights`, the probabilities of the step are
 // added to weights[b, kv head, t], summed over the query heads of the group in a fixed order.
 //
-// Plain form: one block per (sequence, query head), eight warps that take tokens in turn, 4 dims per lane, private online
-// softmax states merged at the end; the weights in a second kernel that forms the scores again.
+// Work decomposition, as in the bf16 decode kernel (gqa_decode.cuh): a unit is one (sequence, kv head, block of <= 16
+// query heads), cut into tiles of 64 tokens (at least one, so that an empty sequence writes its zeros); the tiles of all
+// units form one index space that W persistent blocks share evenly.  The lengths live on the device, so every block adds
+// them up for itself and finds its own range.  One producer warp streams the tiles by TMA (8 KB of K, 8 KB of V, 128-byte
+// swizzle, one box each) into a ring; eight consumer warps in two groups take stages alternately, 16 tokens per warp, with
+// a private online softmax state; states are merged through shared memory at the end of a unit, pieces of a cut unit
+// through the workspace by the last block to arrive.
+//
+// Arithmetic on codes.  The codes become f16, which holds every e4m3 and int8 value exactly, and feed mma.sync
+// m16n8k16 with fp32 accumulation; the scales never touch the codes:
+//   * a query row is brought to [2^14, 2^15) by a power of two before it becomes f16 (exact for every bf16 value within
+//     2^28 of the row's largest, and below 2^-39 of it otherwise), which is taken back in the factor of the scores;
+//   * the K scale is part of that factor: 16 tokens of a warp lie in one block of the cache (blocks are multiples of 16);
+//   * the V scale goes into the exponent: with lv = log2 vscale, p'_t = 2^(s_t + lv_t - m + 15), m = max(s_t + lv_t), so
+//     that O = sum p' v8 needs no scaling and l = sum p'_t / vscale_t.  p' is rounded to f16 for the product (2^-11
+//     relative down to 2^-29 of the largest one, nothing lost above 2^-39), l is summed in fp32 before rounding.
+//
+// Layout without transposes.  K: a lane reads 2 x 16 bytes of its token's row; dims may be permuted freely as long as Q
+// uses the same permutation, so each 4-byte word is one k-step of the B operand.  V: ldmatrix.trans on 16-bit pairs of
+// dims hands a lane {token a: d, d+1 | token b: d, d+1}; one byte permutation makes {a,b} pairs for dim d and for dim d + 1,
+// the B operands of an "even" and an "odd" n-block.  Tokens of an 8-row block are taken in the order 0,4,1,5,2,6,3,7,
+// which makes the 16-byte K reads free of bank conflicts under the TMA swizzle.
 #pragma once
 
+#include "gqa_decode.cuh"
 #include "host_util.cuh"
 #include "kv8_format.cuh"
 
 namespace cllo {
 namespace kv8 {
 
-constexpr int kDecodeWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+constexpr int kTok = 64;  // tokens per stage
+#ifndef CLLO_KV8_STAGES
+#define CLLO_KV8_STAGES 12
+#endif
+constexpr int kStages = CLLO_KV8_STAGES;
+constexpr int kGroups = 2;
+constexpr int kWarpsPerGroup = 4;
+constexpr int kConsumerWarps = kGroups * kWarpsPerGroup;
+constexpr int kDecodeThreads = (kConsumerWarps + 1) * 32;
+constexpr int kTileBytes = kTok * kD;         // K or V of one stage
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kRows = 16;
+constexpr int kPW = kD + 2;                   // {O[128], m (log2 units), l}
+constexpr int kSlotFloats = kRows * kPW;
+constexpr int kSmemStat = kStages * kStageBytes;
+constexpr int kSmemXchg = kSmemStat + kConsumerWarps * 4 * 32 * 4;
+constexpr int kSmemBar = kSmemXchg + kConsumerWarps * 16 * 32 * 4;
+constexpr int kDecodeSmemBytes = kSmemBar + 2 * kStages * 8 + 16 + 1024;
+constexpr float kPShift = 15.f;  // p' <= 2^15
+static_assert(kStages % kGroups == 0, "a stage buffer must always belong to the same consumer group");
+
+enum : int { SITE_KV8_FULL = 80, SITE_KV8_EMPTY = 81, SITE_KV8_DRAIN = 82 };
+
 struct DecodeParams {
     const __nv_bfloat16* q;
-    const uint8_t* k;
-    const uint8_t* v;
     const float* k_scale;
     const float* v_scale;
     const int* seq_lens;
     __nv_bfloat16* o;
-    float* lse;
-    float* weights;  // nullable
-    RowStrides stride;
+    float* lse;       // nullable
+    float* scores;    // nullable: [B, Hq, capacity] scaled scores in log2 units, for the weights
+    float* lse2;      // with scores: [B, Hq] log2 of the normaliser
+    float* slots;     // [W][2][16][kPW]
+    unsigned* counters;
     float scale_log2;
-    int Hq, Hkv, G, capacity, n_blocks, block_shift;
+    int B, Hq, Hkv, G, n_gblk, capacity, n_blocks, block_shift, kv_layout;
 };
 
-__device__ __forceinline__ float warp_sum(float x) {
+using decode::worker_lo;
+using decode::worker_of_tile;
+
+// tiles of a sequence; an empty one has one, so that its output is written
+__device__ __forceinline__ int tiles_of(int len) { return len <= 0 ? 1 : (len + kTok - 1) / kTok; }
+
+// sum over the warp's 32 lanes and inclusive prefix
+__device__ __forceinline__ long long warp_incl_sum(long long v, int lane) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    return x;
-}
-
-template <int kFmt>
-__device__ __forceinline__ float score_log2(const DecodeParams& p, const float (&q)[4], const uint8_t* k_row,
-                                            float k_scale, int lane) {
-    float x[4];
-    decode4<kFmt>(__ldg(reinterpret_cast<const uint32_t*>(k_row) + lane), x);
-    const float d = warp_sum(q[0] * x[0] + q[1] * x[1] + q[2] * x[2] + q[3] * x[3]);
-    return d * (k_scale * p.scale_log2);
-}
-
-__device__ __forceinline__ void load_q4(const __nv_bfloat16* q, int lane, float (&x)[4]) {
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(q) + lane);
-    x[0] = bf16_lo(w.x);
-    x[1] = bf16_hi(w.x);
-    x[2] = bf16_lo(w.y);
-    x[3] = bf16_hi(w.y);
-}
-
-template <int kFmt>
-__global__ void __launch_bounds__(kDecodeWarps * 32) decode_kernel(const DecodeParams p) {
-    __shared__ float sm[kDecodeWarps], sl[kDecodeWarps], so[kDecodeWarps][kD];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int hq = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq, h = hq / p.G;
-    const int len = clamp_len(p.seq_lens[b], p.capacity);
-    const long long base = b * p.stride.batch + h * p.stride.head;
-    const float* ks = p.k_scale + (static_cast<long long>(b) * p.Hkv + h) * p.n_blocks;
-    const float* vs = p.v_scale + (static_cast<long long>(b) * p.Hkv + h) * p.n_blocks;
-    float q[4];
-    load_q4(p.q + (static_cast<long long>(b) * p.Hq + hq) * kD, lane, q);
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int t = warp; t < len; t += kDecodeWarps) {
-        const float s = score_log2<kFmt>(p, q, p.k + base + t * p.stride.token, ks[t >> p.block_shift], lane);
-        const float mn = fmaxf(m, s);
-        const float ref = mn == -INFINITY ? 0.f : mn;  // a NaN score passes through the exponential
-        const float keep = fast_exp2(m - ref), e = fast_exp2(s - ref);
-        float x[4];
-        decode4<kFmt>(__ldg(reinterpret_cast<const uint32_t*>(p.v + base + t * p.stride.token) + lane), x);
-        const float w = e * vs[t >> p.block_shift];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = acc[i] * keep + w * x[i];
-        l = l * keep + e;
-        m = mn;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
     }
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) so[warp][lane * 4 + i] = acc[i];
-    __syncthreads();
-    if (threadIdx.x >= kD) return;
-    float mm = -INFINITY, ll = 0.f, o = 0.f;
-    for (int w = 0; w < kDecodeWarps; ++w) mm = fmaxf(mm, sm[w]);
-    for (int w = 0; w < kDecodeWarps; ++w) {
-        const float f = sl[w] == 0.f ? 0.f : fast_exp2(sm[w] - mm);
-        ll += f * sl[w];
-        o += f * so[w][threadIdx.x];
-    }
-    const long long row = static_cast<long long>(b) * p.Hq + hq;
-    p.o[row * kD + threadIdx.x] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
-    if (p.lse && threadIdx.x == 0) p.lse[row] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * kLn2;
+    return v;
 }
 
-// weights[b, h, t] += sum over the group's heads of e^(s_t - lse); one warp per token
-template <int kFmt>
-__global__ void __launch_bounds__(256) decode_weights_kernel(const DecodeParams p, int B) {
-    const int lane = threadIdx.x & 31;
-    const int b = blockIdx.y / p.Hkv, h = blockIdx.y % p.Hkv;
-    const int len = clamp_len(p.seq_lens[b], p.capacity);
-    const float* ks = p.k_scale + (static_cast<long long>(b) * p.Hkv + h) * p.n_blocks;
-    for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < len; t += gridDim.x * 8) {
-        float sum = 0.f;
-        for (int g = 0; g < p.G; ++g) {
-            const long long row = static_cast<long long>(b) * p.Hq + h * p.G + g;
-            float q[4];
-            load_q4(p.q + row * kD, lane, q);
-            const float s = score_log2<kFmt>(p, q, p.k + b * p.stride.batch + h * p.stride.head + t * p.stride.token,
-                                             ks[t >> p.block_shift], lane);
-            sum += fast_exp2(s - p.lse[row] * kLog2e);
+struct Share {
+    long long T, W, lo, hi;   // all tiles, blocks that take part, this block's range
+    int b;                    // the sequence that holds tile lo
+    long long seq_lo;         // index of that sequence's first tile
+};
+
+// Every warp of the block finds the block's share for itself: two passes over the lengths, the second from L1.
+__device__ __forceinline__ Share find_share(const DecodeParams& p, int lane) {
+    const int U = p.Hkv * p.n_gblk;
+    Share s;
+    long long sum = 0;
+    for (int i = lane; i < p.B; i += 32) sum += tiles_of(clamp_len(__ldg(p.seq_lens + i), p.capacity));
+    s.T = __shfl_sync(0xffffffffu, warp_incl_sum(sum, lane), 31) * U;
+    // no more blocks than tiles: every block of a cut unit then holds a piece of it, which the count of pieces relies on
+    s.W = gridDim.x < s.T ? gridDim.x : s.T;
+    s.lo = s.hi = 0;
+    if (blockIdx.x < s.W) {
+        s.lo = worker_lo(blockIdx.x, s.T, s.W);
+        s.hi = worker_lo(blockIdx.x + 1, s.T, s.W);
+    }
+    s.b = 0;
+    s.seq_lo = 0;
+    if (s.lo >= s.hi) return s;
+    long long before = 0;
+    for (int i0 = 0; i0 < p.B; i0 += 32) {
+        const int i = i0 + lane;
+        const long long n = i < p.B ? static_cast<long long>(tiles_of(clamp_len(__ldg(p.seq_lens + i), p.capacity))) * U : 0;
+        const long long end = before + warp_incl_sum(n, lane);
+        const unsigned holds = __ballot_sync(0xffffffffu, s.lo < end);
+        if (holds) {
+            const int at = __ffs(holds) - 1;
+            s.b = i0 + at;
+            s.seq_lo = __shfl_sync(0xffffffffu, end - n, at);
+            break;
         }
-        if (lane == 0) p.weights[(static_cast<long long>(b) * p.Hkv + h) * p.capacity + t] += sum;
+        before = __shfl_sync(0xffffffffu, end, 31);
+    }
+    return s;
+}
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 r;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
+    return r;
+}
+// {a: d, d+1 | b: d, d+1} -> f16 pairs {a,b} of dim d and of dim d + 1
+template <int kFmt>
+__device__ __forceinline__ void decode_token_pairs(uint32_t w, uint32_t& even, uint32_t& odd) {
+    decode4_f16<kFmt>(__byte_perm(w, 0u, 0x3120), even, odd);
+}
+
+// log-sum-exp merge of the pieces of one unit, 8 columns of one row per thread; pieces in worker order
+template <typename RowPtr>
+__device__ __forceinline__ void merge_pieces(int n, int c8, RowPtr row_ptr, float (&acc)[8], float& m_out, float& l_out) {
+    constexpr int kBatch = 4;
+    float mrun = -INFINITY, lrun = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += kBatch) {
+        float2 ml[kBatch], d[kBatch][4];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const float* row = row_ptr(i0 + i < n ? i0 + i : n - 1);
+            ml[i] = __ldcg(reinterpret_cast<const float2*>(row + kD));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[i][e] = __ldcg(reinterpret_cast<const float2*>(row + c8 + 2 * e));
+            if (i0 + i >= n) ml[i] = make_float2(-INFINITY, 0.f);
+        }
+        float mnew = mrun;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) mnew = fmaxf(mnew, ml[i].x);
+        const float keep = mrun == -INFINITY ? (lrun == 0.f ? 0.f : 1.f) : fast_exp2(mrun - mnew);
+        lrun *= keep;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] *= keep;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (ml[i].y == 0.f) continue;  // no token; a NaN passes
+            const float wgt = fast_exp2(ml[i].x - (mnew == -INFINITY ? 0.f : mnew));
+            lrun += wgt * ml[i].y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[2 * e] += wgt * d[i][e].x;
+                acc[2 * e + 1] += wgt * d[i][e].y;
+            }
+        }
+        mrun = mnew;
+    }
+    m_out = mrun;
+    l_out = lrun;
+}
+
+template <int kFmt, bool kScores>
+__global__ void __launch_bounds__(kDecodeThreads, 1)
+decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const DecodeParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
+    float* stat = reinterpret_cast<float*>(gen_base + kSmemStat);
+    float* xchg = reinterpret_cast<float*>(gen_base + kSmemXchg);
+    const uint32_t bar_base = base + kSmemBar;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + kSmemBar + 2 * kStages * 8);
+    volatile int* misc = abort_flag + 1;
+    auto full_bar = [&](int s) { return bar_base + s * 8; };
+    auto empty_bar = [&](int s) { return bar_base + (kStages + s) * 8; };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), kWarpsPerGroup);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    const Share share = find_share(p, lane);
+    __syncthreads();
+    const long long lo = share.lo, hi = share.hi;
+    if (lo >= hi) return;
+    const int U = p.Hkv * p.n_gblk;
+
+    if (warp == kConsumerWarps) {
+        // ------------------------------ producer ------------------------------
+        if (lane == 0) {
+            tma_prefetch_desc(&tm_k);
+            tma_prefetch_desc(&tm_v);
+            int b = share.b;
+            int n_t = tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
+            const long long in_seq = lo - share.seq_lo;
+            int unit = static_cast<int>(in_seq / n_t);
+            int tile = static_cast<int>(in_seq - static_cast<long long>(unit) * n_t);
+            int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
+            int slot = 0;
+            uint32_t phase = 0;
+            const bool bshd = p.kv_layout == CLLO_KV_BSHD;
+            const int n_tiles = static_cast<int>(hi - lo);
+#pragma unroll 1
+            for (int it = 0; it < n_tiles; ++it) {
+                mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag, SITE_KV8_EMPTY, slot);
+                const int s0 = tile * kTok;
+                const int c1 = bshd ? kvh : s0, c2 = bshd ? s0 : kvh;
+                const uint32_t dst = base + slot * kStageBytes;
+                mbar_arrive_expect_tx(full_bar(slot), kStageBytes);
+                tma_load_4d(dst, &tm_k, full_bar(slot), 0, c1, c2, b);
+                tma_load_4d(dst + kTileBytes, &tm_v, full_bar(slot), 0, c1, c2, b);
+                if (++slot == kStages) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+                if (++tile == n_t) {
+                    tile = 0;
+                    if (++gblk == p.n_gblk) {
+                        gblk = 0;
+                        if (++kvh == p.Hkv) {
+                            kvh = 0;
+                            if (++b < p.B) n_t = tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
+                        }
+                    }
+                }
+            }
+            if (*abort_flag) {
+                // a wait gave up somewhere: make sure no copy is still landing when the block retires
+                const long long n = hi - lo;
+                for (long long it = (n > kStages ? n - kStages : 0); it < n; ++it) {
+                    const int s = static_cast<int>(it % kStages);
+                    const long long t0 = clock64();
+                    while (!mbar_try_wait(full_bar(s), static_cast<uint32_t>(it / kStages) & 1u)) {
+                        if (clock64() - t0 > kWaitLimitCycles / 64) {
+                            record_timeout(SITE_KV8_DRAIN, s);
+                            break;
+                        }
+                    }
+                }
+            }
+        }
+        return;
+    }
+
+    // -------------------------------- consumers --------------------------------
+    const int g = lane >> 2, tig = lane & 3;
+    const int grp = warp / kWarpsPerGroup, sub = warp % kWarpsPerGroup;
+    // this lane's rows of a 16-token slice: K row of n-block nt is nt * 8 + tok_g; score columns are tokens
+    // nt * 8 + tig and nt * 8 + tig + 4
+    const int tok_g = (g >> 1) | ((g & 1) << 2);
+    // ldmatrix row pointers of V: lanes 0-7 rows of the first 8 tokens, 8-15 of the second, 16-31 the same of the next chunk
+    const int v_row_in = ((lane & 7) >> 1) | ((lane & 1) << 2);
+    const uint32_t v_row = static_cast<uint32_t>(sub * 16 + ((lane >> 3) & 1) * 8 + v_row_in);
+    const uint32_t k_row = static_cast<uint32_t>(sub * 16 + tok_g);
+
+    int b = share.b;
+    long long unit_lo;
+    int n_t, unit;  // unit within the sequence
+    int len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
+    n_t = tiles_of(len);
+    unit = static_cast<int>((lo - share.seq_lo) / n_t);
+    unit_lo = share.seq_lo + static_cast<long long>(unit) * n_t;
+    bool first_unit = true;
+
+#pragma unroll 1
+    while (unit_lo < hi) {
+        const long long unit_hi = unit_lo + n_t;
+        const long long seg_lo = lo > unit_lo ? lo : unit_lo;
+        const long long seg_hi = hi < unit_hi ? hi : unit_hi;
+        const int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
+        const int rows = (p.G - gblk * kRows) < kRows ? (p.G - gblk * kRows) : kRows;
+        const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(kvh) * p.G + gblk * kRows;
+        const float* ks = p.k_scale + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
+        const float* vs = p.v_scale + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
+
+        // Q fragments: k-step (j, w) takes dims 16 (tig + 4 j) + 4 w + {0,1} and + {2,3}
+        uint32_t qf[8][4];
+        float mul0, mul1;  // scale * log2(e) * 2^-shift of the two rows
+        {
+            uint2 raw[2][8];
+            float amax[2] = {0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const bool ok = g + 8 * r < rows;
+                const uint2* src = reinterpret_cast<const uint2*>(p.q + (head0 + g + 8 * r) * kD);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    raw[r][i] = ok ? __ldg(src + 4 * (tig + 4 * (i >> 2)) + (i & 3)) : make_uint2(0u, 0u);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    amax[r] = fmaxf(amax[r], fmaxf(fmaxf(finite_abs(bf16_lo(raw[r][i].x)), finite_abs(bf16_hi(raw[r][i].x))),
+                                                   fmaxf(finite_abs(bf16_lo(raw[r][i].y)), finite_abs(bf16_hi(raw[r][i].y)))));
+                amax[r] = fmaxf(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], 1));
+                amax[r] = fmaxf(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], 2));
+                int e = static_cast<int>(__float_as_uint(amax[r]) >> 23) - 127;
+                e = e < -100 ? -100 : e;  // rows below 2^-100 (zero among them): their scores vanish either way
+                const float f = exp2_int(14 - e);
+                (r ? mul1 : mul0) = p.scale_log2 * exp2_int(e - 14);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    qf[i][r] = pack_f16x2(bf16_lo(raw[r][i].x) * f, bf16_hi(raw[r][i].x) * f);
+                    qf[i][r + 2] = pack_f16x2(bf16_lo(raw[r][i].y) * f, bf16_hi(raw[r][i].y) * f);
+                }
+            }
+        }
+
+        float o[16][4];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+        const long long first = seg_lo + ((static_cast<long long>(grp) - (seg_lo - lo)) % kGroups + kGroups) % kGroups;
+        // this warp's block scales, one tile ahead of their use
+        auto block_of = [&](long long t) { return (static_cast<int>(t - unit_lo) * kTok + sub * 16) >> p.block_shift; };
+        float ks_next = 1.f, vs_next = 1.f;
+        if (first < seg_hi && block_of(first) < p.n_blocks) {
+            ks_next = __ldg(ks + block_of(first));
+            vs_next = __ldg(vs + block_of(first));
+        }
+#pragma unroll 1
+        for (long long t = first; t < seg_hi; t += kGroups) {
+            const int it = static_cast<int>(t - lo);
+            const int slot = it % kStages;
+            const float ksc = ks_next, vsc = vs_next;
+            if (t + kGroups < seg_hi && block_of(t + kGroups) < p.n_blocks) {
+                ks_next = __ldg(ks + block_of(t + kGroups));
+                vs_next = __ldg(vs + block_of(t + kGroups));
+            }
+            mbar_wait(full_bar(slot), static_cast<uint32_t>(it / kStages) & 1u, abort_flag, SITE_KV8_FULL, slot);
+            __syncwarp();
+            const uint32_t kb = base + slot * kStageBytes, vb = kb + kTileBytes;
+            const int tok0 = static_cast<int>(t - unit_lo) * kTok + sub * 16;
+            const int valid = len - tok0;  // of this warp's 16 tokens; the rest holds whatever the cache holds
+            if (valid > 0) {
+                // ---- scores: 16 heads x 16 tokens ----
+                float s[2][4];
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+                    const uint32_t row = k_row + nt * 8;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t chunk = static_cast<uint32_t>(tig + 4 * j) ^ (row & 7u);
+                        const uint4 w = lds128(kb + row * 128u + (chunk << 4));
+                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t b0, b1;
+                            decode4_f16<kFmt>(ww[i], b0, b1);
+                            mma_f16_16816(s[nt], qf[j * 4 + i], b0, b1);
+                        }
+                    }
+                }
+                // ---- online softmax, V scale in the exponent ----
+                const float f0 = mul0 * ksc, f1 = mul1 * ksc;
+                const float lv = __log2f(vsc), iv = __frcp_rn(vsc);
+                float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    s[nt][0] *= f0;
+                    s[nt][1] *= f0;
+                    s[nt][2] *= f1;
+                    s[nt][3] *= f1;
+                    if (valid < 16) {
+                        const int c = nt * 8 + tig;
+                        if (c >= valid) s[nt][0] = s[nt][2] = -INFINITY;
+                        if (c + 4 >= valid) s[nt][1] = s[nt][3] = -INFINITY;
+                    }
+                    mx0 = fmaxf(mx0, fmaxf(s[nt][0], s[nt][1]));
+                    mx1 = fmaxf(mx1, fmaxf(s[nt][2], s[nt][3]));
+                }
+                if (kScores) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        if (g + 8 * r < rows) {
+                            float* dst = p.scores + (head0 + g + 8 * r) * p.capacity + tok0 + tig;
+#pragma unroll
+                            for (int nt = 0; nt < 2; ++nt) {
+                                if (nt * 8 + tig < valid) dst[nt * 8] = s[nt][2 * r];
+                                if (nt * 8 + tig + 4 < valid) dst[nt * 8 + 4] = s[nt][2 * r + 1];
+                            }
+                        }
+                    }
+                }
+                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+                const float mn0 = fmaxf(m0, mx0 + lv), mn1 = fmaxf(m1, mx1 + lv);
+                if (__any_sync(0xffffffffu, (mn0 > m0) || (mn1 > m1))) {
+                    const float a0 = fast_exp2(m0 - mn0), a1 = fast_exp2(m1 - mn1);
+                    l0 *= a0;
+                    l1 *= a1;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        o[i][0] *= a0;
+                        o[i][1] *= a0;
+                        o[i][2] *= a1;
+                        o[i][3] *= a1;
+                    }
+                    m0 = mn0;
+                    m1 = mn1;
+                }
+                uint32_t pa[4];
+                {
+                    const float c0 = lv + kPShift - m0, c1 = lv + kPShift - m1;
+                    const float p00 = fast_exp2(s[0][0] + c0), p01 = fast_exp2(s[0][1] + c0);
+                    const float p02 = fast_exp2(s[0][2] + c1), p03 = fast_exp2(s[0][3] + c1);
+                    const float p10 = fast_exp2(s[1][0] + c0), p11 = fast_exp2(s[1][1] + c0);
+                    const float p12 = fast_exp2(s[1][2] + c1), p13 = fast_exp2(s[1][3] + c1);
+                    l0 += ((p00 + p01) + (p10 + p11)) * iv;
+                    l1 += ((p02 + p03) + (p12 + p13)) * iv;
+                    pa[0] = pack_f16x2(p00, p01);
+                    pa[1] = pack_f16x2(p02, p03);
+                    pa[2] = pack_f16x2(p10, p11);
+                    pa[3] = pack_f16x2(p12, p13);
+                }
+                // ---- O += P V ----
+                // bytes of tokens behind the sequence may be NaN codes, which a zero probability does not silence
+                uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;
+                if (valid < 16) {
+                    keep_lo = (tig < valid ? 0x0000ffffu : 0u) | (tig + 4 < valid ? 0xffff0000u : 0u);
+                    keep_hi = (tig + 8 < valid ? 0x0000ffffu : 0u) | (tig + 12 < valid ? 0xffff0000u : 0u);
+                }
+#pragma unroll
+                for (int cp = 0; cp < 4; ++cp) {
+                    const uint32_t chunk = (static_cast<uint32_t>(cp * 2 + (lane >> 4))) ^ (v_row & 7u);
+                    uint32_t w[4];
+                    ldmatrix_x4_trans(vb + v_row * 128u + (chunk << 4), w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t e0, e1, d0, d1;
+                        decode_token_pairs<kFmt>(w[2 * c] & keep_lo, e0, d0);
+                        decode_token_pairs<kFmt>(w[2 * c + 1] & keep_hi, e1, d1);
+                        mma_f16_16816(o[(cp * 2 + c) * 2], pa, e0, e1);
+                        mma_f16_16816(o[(cp * 2 + c) * 2 + 1], pa, d0, d1);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty_bar(slot));
+        }
+
+        // ---- merge the eight private states ----
+        stat[(warp * 4 + 0) * 32 + lane] = m0;
+        stat[(warp * 4 + 1) * 32 + lane] = m1;
+        stat[(warp * 4 + 2) * 32 + lane] = l0;
+        stat[(warp * 4 + 3) * 32 + lane] = l1;
+        named_bar_sync(1, kConsumerWarps * 32);
+        float ms0 = -INFINITY, ms1 = -INFINITY;
+#pragma unroll
+        for (int sw = 0; sw < kConsumerWarps; ++sw) {
+            ms0 = fmaxf(ms0, stat[(sw * 4 + 0) * 32 + lane]);
+            ms1 = fmaxf(ms1, stat[(sw * 4 + 1) * 32 + lane]);
+        }
+        // a state without tokens has l = 0; one whose scores are all NaN has m = -inf and l = NaN, which must survive
+        auto factor = [](float m, float l, float ms) {
+            return l == 0.f ? 0.f : fast_exp2(m - (ms == -INFINITY ? 0.f : ms));
+        };
+        float lt0 = 0.f, lt1 = 0.f;
+#pragma unroll
+        for (int sw = 0; sw < kConsumerWarps; ++sw) {
+            const float wl0 = stat[(sw * 4 + 2) * 32 + lane], wl1 = stat[(sw * 4 + 3) * 32 + lane];
+            lt0 += wl0 * factor(stat[(sw * 4 + 0) * 32 + lane], wl0, ms0);
+            lt1 += wl1 * factor(stat[(sw * 4 + 1) * 32 + lane], wl1, ms1);
+        }
+        lt0 += __shfl_xor_sync(0xffffffffu, lt0, 1);
+        lt0 += __shfl_xor_sync(0xffffffffu, lt0, 2);
+        lt1 += __shfl_xor_sync(0xffffffffu, lt1, 1);
+        lt1 += __shfl_xor_sync(0xffffffffu, lt1, 2);
+        // the four lanes of a row hold different columns: a lane's own l may be 0 where its row's is not
+        const float f0 = m0 == -INFINITY && l0 == 0.f ? 0.f : fast_exp2(m0 - (ms0 == -INFINITY ? 0.f : ms0));
+        const float f1 = m1 == -INFINITY && l1 == 0.f ? 0.f : fast_exp2(m1 - (ms1 == -INFINITY ? 0.f : ms1));
+        // four rounds over the 16-dim chunks 2r and 2r + 1: every warp posts 16 of its 64 (rescaled) values and sums, over the
+        // warps in fixed order, the two it owns: chunk 2r + (warp >> 2), row half (warp >> 1) & 1, dims 4 tig + 2 (warp & 1) + {0, 1}
+        float acc[4][2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int c = 2 * r + (i >> 3), half = (i >> 2) & 1, e = i & 3;
+                xchg[(warp * 16 + i) * 32 + lane] = o[2 * c + (e & 1)][half * 2 + (e >> 1)] * (half ? f1 : f0);
+            }
+            named_bar_sync(1, kConsumerWarps * 32);
+            float a = 0.f, c = 0.f;
+#pragma unroll
+            for (int sw = 0; sw < kConsumerWarps; ++sw) {
+                a += xchg[(sw * 16 + 2 * warp) * 32 + lane];
+                c += xchg[(sw * 16 + 2 * warp + 1) * 32 + lane];
+            }
+            acc[r][0] = a;
+            acc[r][1] = c;
+            named_bar_sync(1, kConsumerWarps * 32);
+        }
+
+        // ---- every warp writes its share ----
+        const bool whole = seg_lo == unit_lo && seg_hi == unit_hi;
+        {
+            const int half = (warp >> 1) & 1, row = g + 8 * half;
+            const float mrow = half ? ms1 : ms0, lrow = half ? lt1 : lt0;
+            const int col0 = (warp >> 2) * 16 + 4 * tig + 2 * (warp & 1);
+            if (row < rows) {
+                if (whole) {
+                    const float inv = lrow == 0.f ? 0.f : 1.f / lrow;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        *reinterpret_cast<uint32_t*>(p.o + (head0 + row) * kD + r * 32 + col0) =
+                            pack_bf16x2(acc[r][0] * inv, acc[r][1] * inv);
+                    if (tig == 0 && (warp & 5) == 0) {
+                        const float l2 = lrow == 0.f ? -INFINITY : mrow - kPShift + log2f(lrow);
+                        if (p.lse) p.lse[head0 + row] = l2 * kLn2;
+                        if (kScores) p.lse2[head0 + row] = l2;
+                    }
+                } else {
+                    float* dst = p.slots + (static_cast<long long>(blockIdx.x) * 2 + (first_unit ? 0 : 1)) * kSlotFloats + row * kPW;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        *reinterpret_cast<float2*>(dst + r * 32 + col0) = make_float2(acc[r][0], acc[r][1]);
+                    if (tig == 0 && (warp & 5) == 0) {
+                        dst[kD] = mrow;
+                        dst[kD + 1] = lrow;
+                    }
+                }
+            }
+        }
+
+        if (!whole) {
+            // this block's piece of the unit is in the workspace: count it in; the last one to arrive merges
+            const long long W = share.W;
+            const long long w_first = worker_of_tile(unit_lo, share.T, W), w_last = worker_of_tile(unit_hi - 1, share.T, W);
+            const int n_pieces = static_cast<int>(w_last - w_first) + 1;
+            unsigned* counter = p.counters + w_first;
+            named_bar_sync(1, kConsumerWarps * 32);
+            if (threadIdx.x == 0) {
+                __threadfence();
+                const bool last = atomicAdd(counter, 1u) == static_cast<unsigned>(n_pieces - 1);
+                __threadfence();
+                if (last) *counter = 0u;  // the counters are zero again when the kernel ends
+                misc[0] = last ? 1 : 0;
+            }
+            named_bar_sync(1, kConsumerWarps * 32);
+            if (misc[0] != 0) {
+                const int row = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
+                const int which_first = worker_lo(w_first, share.T, W) >= unit_lo ? 0 : 1;
+                if (row < rows) {
+                    float mg[8], mm, ll;
+                    merge_pieces(n_pieces, c8,
+                                 [&](int i) {
+                                     return p.slots + ((w_first + i) * 2 + (i == 0 ? which_first : 0)) * kSlotFloats + row * kPW;
+                                 },
+                                 mg, mm, ll);
+                    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+                    uint4 pk;
+                    pk.x = pack_bf16x2(mg[0] * inv, mg[1] * inv);
+                    pk.y = pack_bf16x2(mg[2] * inv, mg[3] * inv);
+                    pk.z = pack_bf16x2(mg[4] * inv, mg[5] * inv);
+                    pk.w = pack_bf16x2(mg[6] * inv, mg[7] * inv);
+                    *reinterpret_cast<uint4*>(p.o + (head0 + row) * kD + c8) = pk;
+                    if (c8 == 0) {
+                        const float l2 = ll == 0.f ? -INFINITY : mm - kPShift + log2f(ll);
+                        if (p.lse) p.lse[head0 + row] = l2 * kLn2;
+                        if (kScores) p.lse2[head0 + row] = l2;
+                    }
+                }
+            }
+        }
+
+        // next unit of this block's range
+        first_unit = false;
+        unit_lo = unit_hi;
+        if (++unit == U) {
+            unit = 0;
+            if (++b >= p.B) break;
+            len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
+            n_t = tiles_of(len);
+        }
     }
 }
 
-static size_t decode_workspace_bytes(int B, int capacity, int Hq, int Hkv, int D, int with_weights) {
-    if (B <= 0 || capacity <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D != kD) return 0;
-    return with_weights ? static_cast<size_t>(B) * Hq * sizeof(float) : 256;
+// weights[b, h, t] += sum over the group's heads, in order, of 2^(score - lse2); one thread per token
+constexpr int kWeightThreads = 256, kWeightTok = 1024;
+__global__ void __launch_bounds__(kWeightThreads) decode_weights_kernel(const DecodeParams p, float* weights, int n_chunks) {
+    const int chunk = blockIdx.x % n_chunks, row = blockIdx.x / n_chunks;  // row = (b, h)
+    const int b = row / p.Hkv, h = row - b * p.Hkv;
+    const int len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
+    const int t0 = chunk * kWeightTok;
+    if (t0 >= len) return;
+    constexpr int kPer = kWeightTok / kWeightThreads;
+    float sum[kPer] = {};
+    const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(h) * p.G;
+    for (int g = 0; g < p.G; ++g) {
+        const float l2 = __ldg(p.lse2 + head0 + g);
+        const float* src = p.scores + (head0 + g) * p.capacity;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int t = t0 + i * kWeightThreads + threadIdx.x;
+            if (t < len) sum[i] += fast_exp2(__ldcg(src + t) - l2);
+        }
+    }
+    float* dst = weights + static_cast<long long>(row) * p.capacity;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int t = t0 + i * kWeightThreads + threadIdx.x;
+        if (t < len) dst[t] += sum[i];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+// Workspace: arrival counters at the start (1024, as in the bf16 decode), partial slots, then -- with weights -- the
+// log2 normalisers and the scores of every (query head, token).
+struct DecodePlan {
+    int W, n_gblk;
+    size_t slot_offset, lse2_offset, score_offset, bytes;
+};
+
+static int make_decode_plan(int B, int capacity, int Hq, int Hkv, int D, bool with_weights, int num_workers, int sm_count,
+                            DecodePlan* plan) {
+    if (B <= 0 || capacity <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || num_workers < 0 || Hq % Hkv != 0) return CLLO_E_BAD_ARG;
+    if (D != kD || capacity > kMaxCapacity) return CLLO_E_UNSUPPORTED;
+    plan->n_gblk = (Hq / Hkv + kRows - 1) / kRows;
+    const long long units = static_cast<long long>(B) * Hkv * plan->n_gblk;
+    if (units * kRows > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
+    const long long most = units * ((capacity + kTok - 1) / kTok);  // tiles if every sequence filled the cache
+    long long W = num_workers > 0 ? num_workers : (static_cast<long long>(sm_count) * 173) / 200;
+    if (W > decode::kFixedCounters) W = decode::kFixedCounters;
+    if (W > most) W = most;
+    if (W < 1) W = 1;
+    if (most / W + 1 > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;  // a block's tile count is a 32-bit loop index
+    plan->W = static_cast<int>(W);
+    plan->slot_offset = decode::kSlotOffsetBytes;
+    plan->lse2_offset = plan->slot_offset + static_cast<size_t>(W) * 2 * kSlotFloats * sizeof(float);
+    const size_t rows = static_cast<size_t>(B) * Hq;
+    plan->score_offset = plan->lse2_offset + (with_weights ? (rows * sizeof(float) + 255) / 256 * 256 : 0);
+    plan->bytes = plan->score_offset + (with_weights ? rows * capacity * sizeof(float) : 0);
+    return CLLO_OK;
+}
+
+static int encode_cache_map(CUtensorMap* map, const void* base, int B, int capacity, int Hkv, int kv_layout) {
+    EncodeTiledFn fn;
+    int rc = get_encode_fn(&fn);
+    if (rc != CLLO_OK) return rc;
+    const bool bshd = kv_layout == CLLO_KV_BSHD;
+    const cuuint64_t S = static_cast<cuuint64_t>(capacity), H = static_cast<cuuint64_t>(Hkv);
+    cuuint64_t dims[4] = {kD, bshd ? H : S, bshd ? S : H, static_cast<cuuint64_t>(B)};
+    cuuint64_t strides[3] = {kD, bshd ? kD * H : kD * S, kD * H * S};
+    cuuint32_t box[4] = {kD, bshd ? 1u : kTok, bshd ? kTok : 1u, 1u};
+    cuuint32_t es[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, es,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        t_last_cuda_error = static_cast<int>(cudaErrorInvalidValue);
+        return CLLO_E_CUDA;
+    }
+    return CLLO_OK;
+}
+
+template <int kFmt, bool kScores>
+static int decode_launch_kernel(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const DecodeParams& p, int W,
+                                std::atomic<bool>* attr_set, cudaStream_t st) {
+    if (!*attr_set) {
+        CLLO_CUDA_TRY(cudaFuncSetAttribute(decode_kernel<kFmt, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           kDecodeSmemBytes));
+        *attr_set = true;
+    }
+    decode_kernel<kFmt, kScores><<<W, kDecodeThreads, kDecodeSmemBytes, st>>>(tm_k, tm_v, p);
+    CLLO_CUDA_TRY(cudaGetLastError());
+    return CLLO_OK;
 }
 
 static int decode_launch(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
@@ -133,46 +718,63 @@ static int decode_launch(const void* q, const void* k, const void* v, const floa
                          size_t workspace_bytes, int B, int capacity, int Hq, int Hkv, int D, int kv_layout, int block,
                          int format, int num_workers, cudaStream_t st) {
     if (!q || !k || !v || !k_scale || !v_scale || !seq_lens || !o) return CLLO_E_BAD_ARG;
-    if (B <= 0 || capacity <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv != 0) return CLLO_E_BAD_ARG;
+    const bool counters_zero = (kv_layout & CLLO_WS_COUNTERS_ZERO) != 0;
+    kv_layout &= ~CLLO_WS_COUNTERS_ZERO;
     if (kv_layout != CLLO_KV_BSHD && kv_layout != CLLO_KV_BHSD) return CLLO_E_BAD_ARG;
     if (!valid_format(format) || !valid_block(block)) return CLLO_E_BAD_ARG;
-    if (!isfinite(scale) || num_workers < 0) return CLLO_E_BAD_ARG;
-    if (D != kD || capacity > kMaxCapacity) return CLLO_E_UNSUPPORTED;
-    if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(o, 16)) return CLLO_E_BAD_ARG;
-    const size_t need = decode_workspace_bytes(B, capacity, Hq, Hkv, D, weights != nullptr);
-    if (!workspace || workspace_bytes < need || !aligned_to(workspace, 256)) return CLLO_E_WORKSPACE;
-    if (static_cast<long long>(B) * Hq > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
+    if (!isfinite(scale)) return CLLO_E_BAD_ARG;
+    if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(o, 16) || !aligned_to(k_scale, 4) ||
+        !aligned_to(v_scale, 4) || !aligned_to(seq_lens, 4) || !aligned_to(lse, 4) || !aligned_to(weights, 4))
+        return CLLO_E_BAD_ARG;
+    DecodePlan plan;
+    int rc = make_decode_plan(B, capacity, Hq, Hkv, D, weights != nullptr, num_workers, 1, &plan);  // arguments only
+    if (rc != CLLO_OK) return rc;
     DeviceInfo* di = nullptr;
-    int rc = current_device_info(&di);
+    rc = current_device_info(&di);
     if (rc != CLLO_OK) return rc;
     if (di->cc_major != 10) return CLLO_E_UNSUPPORTED;
+    rc = make_decode_plan(B, capacity, Hq, Hkv, D, weights != nullptr, num_workers, di->sm_count, &plan);
+    if (rc != CLLO_OK) return rc;
+    if (!workspace || workspace_bytes < plan.bytes || !aligned_to(workspace, 256)) return CLLO_E_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
     DecodeParams p;
     p.q = static_cast<const __nv_bfloat16*>(q);
-    p.k = static_cast<const uint8_t*>(k);
-    p.v = static_cast<const uint8_t*>(v);
     p.k_scale = k_scale;
     p.v_scale = v_scale;
     p.seq_lens = seq_lens;
     p.o = static_cast<__nv_bfloat16*>(o);
-    p.lse = lse ? lse : (weights ? static_cast<float*>(workspace) : nullptr);
-    p.weights = weights;
-    p.stride = cache_strides(kv_layout, capacity, Hkv);
+    p.lse = lse;
+    p.scores = weights ? reinterpret_cast<float*>(ws + plan.score_offset) : nullptr;
+    p.lse2 = reinterpret_cast<float*>(ws + plan.lse2_offset);
+    p.slots = reinterpret_cast<float*>(ws + plan.slot_offset);
+    p.counters = reinterpret_cast<unsigned*>(ws);
     p.scale_log2 = scale * kLog2e;
+    p.B = B;
     p.Hq = Hq;
     p.Hkv = Hkv;
     p.G = Hq / Hkv;
+    p.n_gblk = plan.n_gblk;
     p.capacity = capacity;
     p.n_blocks = (capacity + block - 1) / block;
     p.block_shift = block_shift_of(block);
-    const bool fp8 = format == CLLO_FMT_E4M3;
-    (fp8 ? decode_kernel<CLLO_FMT_E4M3> : decode_kernel<CLLO_FMT_INT8>)<<<B * Hq, kDecodeWarps * 32, 0, st>>>(p);
+    p.kv_layout = kv_layout;
+    CUtensorMap tm_k, tm_v;
+    if ((rc = encode_cache_map(&tm_k, k, B, capacity, Hkv, kv_layout)) != CLLO_OK) return rc;
+    if ((rc = encode_cache_map(&tm_v, v, B, capacity, Hkv, kv_layout)) != CLLO_OK) return rc;
+    if (!counters_zero && plan.W > 1) CLLO_CUDA_TRY(cudaMemsetAsync(ws, 0, plan.W * sizeof(unsigned), st));
+    std::atomic<bool>* attr = di->kv8_decode_attr_set;
+    if (format == CLLO_FMT_E4M3)
+        rc = weights ? decode_launch_kernel<CLLO_FMT_E4M3, true>(tm_k, tm_v, p, plan.W, attr + 0, st)
+                     : decode_launch_kernel<CLLO_FMT_E4M3, false>(tm_k, tm_v, p, plan.W, attr + 1, st);
+    else
+        rc = weights ? decode_launch_kernel<CLLO_FMT_INT8, true>(tm_k, tm_v, p, plan.W, attr + 2, st)
+                     : decode_launch_kernel<CLLO_FMT_INT8, false>(tm_k, tm_v, p, plan.W, attr + 3, st);
+    if (rc != CLLO_OK || !weights) return rc;
+    const int n_chunks = (capacity + kWeightTok - 1) / kWeightTok;
+    const long long blocks = static_cast<long long>(B) * Hkv * n_chunks;
+    if (blocks > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
+    decode_weights_kernel<<<static_cast<unsigned>(blocks), kWeightThreads, 0, st>>>(p, weights, n_chunks);
     CLLO_CUDA_TRY(cudaGetLastError());
-    if (weights) {
-        if (static_cast<long long>(B) * Hkv > 65535) return CLLO_E_UNSUPPORTED;
-        const int gx = (capacity + 7) / 8 < 512 ? (capacity + 7) / 8 : 512;
-        (fp8 ? decode_weights_kernel<CLLO_FMT_E4M3> : decode_weights_kernel<CLLO_FMT_INT8>)<<<dim3(gx, B * Hkv), 256, 0, st>>>(p, B);
-        CLLO_CUDA_TRY(cudaGetLastError());
-    }
     return CLLO_OK;
 }
 

@@ -61,7 +61,7 @@ def append(codes, scales, rows, held, n, block, dtype):
 
 
 def decode(q, cache, lens, scale):
-    """(out, lse, p, sum p|v|, largest scale * sum |q k|): p [B,Hq,S]."""
+    """(out, lse, p, sum p|v|, largest scale * sum |q k|, max_t (p vscale)_t * sum_t |v8|): p [B,Hq,S]."""
     k, v = values(cache)
     B, Hq, D = q.shape
     H = cache.num_kv_heads
@@ -75,8 +75,11 @@ def decode(q, cache, lens, scale):
     s = s.masked_fill(~seen[:, None, None], -math.inf)
     lse = torch.logsumexp(s, -1)
     p = torch.exp(s - torch.where(lse == -math.inf, torch.zeros_like(lse), lse)[..., None])
+    vs = cache.v_scale.double().repeat_interleave(cache.block_tokens, 2)[:, :, None, :S]
+    top = torch.where(seen[:, None, None], p * vs, torch.zeros_like(p)).amax(-1, keepdim=True)
+    codes = torch.where(seen[:, None, :, None], heads_first(cache.v, cache.kv_layout).double().abs(), torch.zeros_like(v))
     return ((p @ v).reshape(B, Hq, D), lse.reshape(B, Hq), p.reshape(B, Hq, S), (p @ v.abs()).reshape(B, Hq, D),
-            size.amax(-1).reshape(B, Hq))
+            size.amax(-1).reshape(B, Hq), (top * codes.sum(2)[:, :, None]).reshape(B, Hq, D))
 
 
 def weight_sums(q, k, lse, scale, causal, q_start=0, lens=None, window=None):
