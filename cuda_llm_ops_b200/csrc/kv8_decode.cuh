@@ -18,9 +18,11 @@
 //   * a query row is brought to [2^14, 2^15) by a power of two before it becomes f16 (exact for every bf16 value within
 //     2^28 of the row's largest, and below 2^-39 of it otherwise), which is taken back in the factor of the scores;
 //   * the K scale is part of that factor: 16 tokens of a warp lie in one block of the cache (blocks are multiples of 16);
-//   * the V scale goes into the exponent: with lv = log2 vscale, p'_t = 2^(s_t + lv_t - m + 15), m = max(s_t + lv_t), so
-//     that O = sum p' v8 needs no scaling and l = sum p'_t / vscale_t.  p' is rounded to f16 for the product (2^-11
-//     relative down to 2^-29 of the largest one, nothing lost above 2^-39), l is summed in fp32 before rounding.
+//   * the V scale goes into the exponent: with lv = log2 vscale, p'_t = 2^(s_t + lv_t - m + 11), m = max(s_t + lv_t), so
+//     that O = sum p' v8 needs no scaling and l = sum p'_t / vscale_t.  p' is rounded to f16 for the product (half a step:
+//     2^-11 relative, 2^-25 absolute below f16's normal range), l is summed in fp32 before rounding.  The reference m may
+//     lag behind the true maximum by 2^4 (kLazy), so the largest p' lies in [2^11, 2^15] and the absolute part is at most
+//     2^-36 of it.
 //
 // Layout without transposes.  K: a lane reads 2 x 16 bytes of its token's row; dims may be permuted freely as long as Q
 // uses the same permutation, so each 4-byte word is one k-step of the B operand.  V: ldmatrix.trans on 16-bit pairs of
@@ -44,10 +46,20 @@ constexpr int kTok = 64;  // tokens per stage
 #define CLLO_KV8_STAGES 12
 #endif
 constexpr int kStages = CLLO_KV8_STAGES;
-constexpr int kGroups = 2;
-constexpr int kWarpsPerGroup = 4;
+#ifndef CLLO_KV8_GROUPS
+#define CLLO_KV8_GROUPS 4
+#endif
+constexpr int kGroups = CLLO_KV8_GROUPS;
+constexpr int kWarpsPerGroup = 2;
+constexpr int kSubTok = kTok / kWarpsPerGroup;  // tokens per warp and stage: two halves of 16
 constexpr int kConsumerWarps = kGroups * kWarpsPerGroup;
-constexpr int kDecodeThreads = (kConsumerWarps + 1) * 32;
+// Two consumer warpgroups and one for the producer (its other warps only complete the warpgroup, which setmaxnreg needs):
+// the consumers hold a unit's Q and O fragments, 96 registers, and 32 tokens' codes and scores beside them.  The pool is
+// what the block was launched with; asking for more in total would never return.
+constexpr int kDecodeThreads = (kConsumerWarps + 4) * 32;
+constexpr int kLaunchRegs = 168, kConsumerRegs = 232, kProducerRegs = 40;
+static_assert(2 * kConsumerRegs + kProducerRegs <= 3 * kLaunchRegs, "setmaxnreg budget exceeds the block's register pool");
+static_assert(kConsumerWarps == 8 && kDecodeThreads == 384, "the register budget is for three warpgroups");
 constexpr int kTileBytes = kTok * kD;         // K or V of one stage
 constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kRows = 16;
@@ -56,8 +68,13 @@ constexpr int kSlotFloats = kRows * kPW;
 constexpr int kSmemStat = kStages * kStageBytes;
 constexpr int kSmemXchg = kSmemStat + kConsumerWarps * 4 * 32 * 4;
 constexpr int kSmemBar = kSmemXchg + kConsumerWarps * 16 * 32 * 4;
-constexpr int kDecodeSmemBytes = kSmemBar + 2 * kStages * 8 + 16 + 1024;
-constexpr float kPShift = 15.f;  // p' <= 2^15
+constexpr int kSmemScale = kSmemBar + 2 * kStages * 8;  // per stage: K and V scales of its four 16-token quarters
+constexpr int kQuarters = kTok / 16;
+constexpr int kSmemMisc = kSmemScale + kStages * 2 * kQuarters * 4;
+constexpr int kDecodeSmemBytes = kSmemMisc + 16 + 1024;
+constexpr float kLazy = 4.f;                 // a reference may lag behind the true maximum by this much (log2)
+constexpr float kPShift = 15.f - kLazy;      // p' <= 2^15
+constexpr float kMinFactor = 7.888609e-31f;  // 2^-100: a score is at most 2^31 times its factor, so this much is nothing
 static_assert(kStages % kGroups == 0, "a stage buffer must always belong to the same consumer group");
 
 enum : int { SITE_KV8_FULL = 80, SITE_KV8_EMPTY = 81, SITE_KV8_DRAIN = 82 };
@@ -134,9 +151,7 @@ __device__ __forceinline__ Share find_share(const DecodeParams& p, int lane) {
 }
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -150,10 +165,25 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
     return r;
 }
-// {a: d, d+1 | b: d, d+1} -> f16 pairs {a,b} of dim d and of dim d + 1
-template <int kFmt>
-__device__ __forceinline__ void decode_token_pairs(uint32_t w, uint32_t& even, uint32_t& odd) {
-    decode4_f16<kFmt>(__byte_perm(w, 0u, 0x3120), even, odd);
+__device__ __forceinline__ void lds64(uint32_t addr, float (&x)[2]) {
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(x[0]), "=f"(x[1]) : "r"(addr));
+}
+// 4-byte asynchronous copy, and an arrival on a barrier once this thread's earlier ones have landed
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float log2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // log-sum-exp merge of the pieces of one unit, 8 columns of one row per thread; pieces in worker order
@@ -207,7 +237,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     float* stat = reinterpret_cast<float*>(gen_base + kSmemStat);
     float* xchg = reinterpret_cast<float*>(gen_base + kSmemXchg);
     const uint32_t bar_base = base + kSmemBar;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + kSmemBar + 2 * kStages * 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + kSmemMisc);
     volatile int* misc = abort_flag + 1;
     auto full_bar = [&](int s) { return bar_base + s * 8; };
     auto empty_bar = [&](int s) { return bar_base + (kStages + s) * 8; };
@@ -215,7 +245,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(full_bar(s), 1);
+            mbar_init(full_bar(s), 1 + 2 * kQuarters);  // the tile copy and the eight scale copies
             mbar_init(empty_bar(s), kWarpsPerGroup);
         }
         *abort_flag = 0;
@@ -227,11 +257,17 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     if (lo >= hi) return;
     const int U = p.Hkv * p.n_gblk;
 
-    if (warp == kConsumerWarps) {
+    if (warp >= kConsumerWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+        if (warp > kConsumerWarps) return;
         // ------------------------------ producer ------------------------------
-        if (lane == 0) {
-            tma_prefetch_desc(&tm_k);
-            tma_prefetch_desc(&tm_v);
+        // Lane 0 issues the tile copies; lanes 0-7 copy one block scale each (a quarter's K or V scale) into the stage, and
+        // their arrivals are part of the stage's full barrier.
+        if (lane < 2 * kQuarters) {
+            if (lane == 0) {
+                tma_prefetch_desc(&tm_k);
+                tma_prefetch_desc(&tm_v);
+            }
             int b = share.b;
             int n_t = tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
             const long long in_seq = lo - share.seq_lo;
@@ -242,15 +278,25 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
             uint32_t phase = 0;
             const bool bshd = p.kv_layout == CLLO_KV_BSHD;
             const int n_tiles = static_cast<int>(hi - lo);
+            const float* scales = lane < kQuarters ? p.k_scale : p.v_scale;
+            const float* row = scales + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
+            const int quarter = lane % kQuarters;
+            const uint32_t scale_dst = base + kSmemScale + lane * 4;
 #pragma unroll 1
             for (int it = 0; it < n_tiles; ++it) {
                 mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag, SITE_KV8_EMPTY, slot);
                 const int s0 = tile * kTok;
-                const int c1 = bshd ? kvh : s0, c2 = bshd ? s0 : kvh;
-                const uint32_t dst = base + slot * kStageBytes;
-                mbar_arrive_expect_tx(full_bar(slot), kStageBytes);
-                tma_load_4d(dst, &tm_k, full_bar(slot), 0, c1, c2, b);
-                tma_load_4d(dst + kTileBytes, &tm_v, full_bar(slot), 0, c1, c2, b);
+                int blk = (s0 + quarter * 16) >> p.block_shift;
+                blk = blk < p.n_blocks ? blk : p.n_blocks - 1;  // a quarter behind the cache: any scale, nobody uses it
+                cp_async_4(scale_dst + slot * (2 * kQuarters * 4), row + blk);
+                cp_async_arrive(full_bar(slot));
+                if (lane == 0) {
+                    const int c1 = bshd ? kvh : s0, c2 = bshd ? s0 : kvh;
+                    const uint32_t dst = base + slot * kStageBytes;
+                    mbar_arrive_expect_tx(full_bar(slot), kStageBytes);
+                    tma_load_4d(dst, &tm_k, full_bar(slot), 0, c1, c2, b);
+                    tma_load_4d(dst + kTileBytes, &tm_v, full_bar(slot), 0, c1, c2, b);
+                }
                 if (++slot == kStages) {
                     slot = 0;
                     phase ^= 1u;
@@ -263,6 +309,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                             kvh = 0;
                             if (++b < p.B) n_t = tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
                         }
+                        row = scales + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
                     }
                 }
             }
@@ -285,6 +332,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     }
 
     // -------------------------------- consumers --------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
     const int g = lane >> 2, tig = lane & 3;
     const int grp = warp / kWarpsPerGroup, sub = warp % kWarpsPerGroup;
     // this lane's rows of a 16-token slice: K row of n-block nt is nt * 8 + tok_g; score columns are tokens
@@ -292,8 +340,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     const int tok_g = (g >> 1) | ((g & 1) << 2);
     // ldmatrix row pointers of V: lanes 0-7 rows of the first 8 tokens, 8-15 of the second, 16-31 the same of the next chunk
     const int v_row_in = ((lane & 7) >> 1) | ((lane & 1) << 2);
-    const uint32_t v_row = static_cast<uint32_t>(sub * 16 + ((lane >> 3) & 1) * 8 + v_row_in);
-    const uint32_t k_row = static_cast<uint32_t>(sub * 16 + tok_g);
+    const uint32_t v_row = static_cast<uint32_t>(sub * kSubTok + ((lane >> 3) & 1) * 8 + v_row_in);
+    const uint32_t k_row = static_cast<uint32_t>(sub * kSubTok + tok_g);
 
     int b = share.b;
     long long unit_lo;
@@ -303,6 +351,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     unit = static_cast<int>((lo - share.seq_lo) / n_t);
     unit_lo = share.seq_lo + static_cast<long long>(unit) * n_t;
     bool first_unit = true;
+    int slot = grp;  // the next stage of this group; its stages are taken in order across units
+    uint32_t phase = 0;
 
 #pragma unroll 1
     while (unit_lo < hi) {
@@ -312,9 +362,6 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         const int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
         const int rows = (p.G - gblk * kRows) < kRows ? (p.G - gblk * kRows) : kRows;
         const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(kvh) * p.G + gblk * kRows;
-        const float* ks = p.k_scale + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
-        const float* vs = p.v_scale + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
-
         // Q fragments: k-step (j, w) takes dims 16 (tig + 4 j) + 4 w + {0,1} and + {2,3}
         uint32_t qf[8][4];
         float mul0, mul1;  // scale * log2(e) * 2^-shift of the two rows
@@ -337,8 +384,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                 amax[r] = fmaxf(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], 2));
                 int e = static_cast<int>(__float_as_uint(amax[r]) >> 23) - 127;
                 e = e < -100 ? -100 : e;  // rows below 2^-100 (zero among them): their scores vanish either way
-                const float f = exp2_int(14 - e);
-                (r ? mul1 : mul0) = p.scale_log2 * exp2_int(e - 14);
+                const float f = copysignf(exp2_int(14 - e), p.scale_log2);  // the sign of the scale goes with the query
+                (r ? mul1 : mul0) = fabsf(p.scale_log2) * exp2_int(e - 14);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     qf[i][r] = pack_f16x2(bf16_lo(raw[r][i].x) * f, bf16_hi(raw[r][i].x) * f);
@@ -352,65 +399,77 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-        const long long first = seg_lo + ((static_cast<long long>(grp) - (seg_lo - lo)) % kGroups + kGroups) % kGroups;
-        // this warp's block scales, one tile ahead of their use
-        auto block_of = [&](long long t) { return (static_cast<int>(t - unit_lo) * kTok + sub * 16) >> p.block_shift; };
-        float ks_next = 1.f, vs_next = 1.f;
-        if (first < seg_hi && block_of(first) < p.n_blocks) {
-            ks_next = __ldg(ks + block_of(first));
-            vs_next = __ldg(vs + block_of(first));
-        }
+        // tiles of this group in the segment: local index (t - lo) congruent to grp modulo kGroups
+        const int skip = static_cast<int>((static_cast<long long>(grp) - (seg_lo - lo)) & (kGroups - 1));
+        int tile = static_cast<int>(seg_lo - unit_lo) + skip;  // index within the unit
+        const int tile_end = static_cast<int>(seg_hi - unit_lo);
 #pragma unroll 1
-        for (long long t = first; t < seg_hi; t += kGroups) {
-            const int it = static_cast<int>(t - lo);
-            const int slot = it % kStages;
-            const float ksc = ks_next, vsc = vs_next;
-            if (t + kGroups < seg_hi && block_of(t + kGroups) < p.n_blocks) {
-                ks_next = __ldg(ks + block_of(t + kGroups));
-                vs_next = __ldg(vs + block_of(t + kGroups));
-            }
-            mbar_wait(full_bar(slot), static_cast<uint32_t>(it / kStages) & 1u, abort_flag, SITE_KV8_FULL, slot);
+        for (; tile < tile_end; tile += kGroups) {
+            mbar_wait(full_bar(slot), phase, abort_flag, SITE_KV8_FULL, slot);
             __syncwarp();
             const uint32_t kb = base + slot * kStageBytes, vb = kb + kTileBytes;
-            const int tok0 = static_cast<int>(t - unit_lo) * kTok + sub * 16;
-            const int valid = len - tok0;  // of this warp's 16 tokens; the rest holds whatever the cache holds
+            const int tok0 = tile * kTok + sub * kSubTok;
+            const int valid = len - tok0;  // of this warp's 32 tokens; the rest holds whatever the cache holds
             if (valid > 0) {
-                // ---- scores: 16 heads x 16 tokens ----
-                float s[2][4];
+                float ksc[2], vsc[2];  // of this warp's two halves
+                lds64(base + kSmemScale + slot * (2 * kQuarters * 4) + sub * 8, ksc);
+                lds64(base + kSmemScale + slot * (2 * kQuarters * 4) + kQuarters * 4 + sub * 8, vsc);
+                // ---- scores: 16 heads x 2 x 16 tokens; two accumulators per n-block make independent chains ----
+                float s[2][2][4];
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-                    const uint32_t row = k_row + nt * 8;
+                for (int u = 0; u < 2; ++u) {
+                    uint4 kw[2][2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt)
+                            kw[nt][j] = lds128(kb + (k_row + u * 16 + nt * 8) * 128u +
+                                               ((static_cast<uint32_t>(tig + 4 * j) ^ (k_row & 7u)) << 4));
+                    float s2[2][4];
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[u][nt][e] = s2[nt][e] = 0.f;
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const uint32_t chunk = static_cast<uint32_t>(tig + 4 * j) ^ (row & 7u);
-                        const uint4 w = lds128(kb + row * 128u + (chunk << 4));
-                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            uint32_t b0, b1;
-                            decode4_f16<kFmt>(ww[i], b0, b1);
-                            mma_f16_16816(s[nt], qf[j * 4 + i], b0, b1);
+#pragma unroll
+                            for (int nt = 0; nt < 2; ++nt) {
+                                const uint32_t ww[4] = {kw[nt][j].x, kw[nt][j].y, kw[nt][j].z, kw[nt][j].w};
+                                uint32_t b0, b1;
+                                decode4_f16<kFmt>(ww[i], b0, b1);
+                                mma_f16_16816((i & 1) ? s2[nt] : s[u][nt], qf[j * 4 + i], b0, b1);
+                            }
                         }
                     }
-                }
-                // ---- online softmax, V scale in the exponent ----
-                const float f0 = mul0 * ksc, f1 = mul1 * ksc;
-                const float lv = __log2f(vsc), iv = __frcp_rn(vsc);
-                float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    s[nt][0] *= f0;
-                    s[nt][1] *= f0;
-                    s[nt][2] *= f1;
-                    s[nt][3] *= f1;
-                    if (valid < 16) {
-                        const int c = nt * 8 + tig;
-                        if (c >= valid) s[nt][0] = s[nt][2] = -INFINITY;
-                        if (c + 4 >= valid) s[nt][1] = s[nt][3] = -INFINITY;
-                    }
-                    mx0 = fmaxf(mx0, fmaxf(s[nt][0], s[nt][1]));
-                    mx1 = fmaxf(mx1, fmaxf(s[nt][2], s[nt][3]));
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[u][nt][e] += s2[nt][e];
+                }
+                if (valid < kSubTok) {
+                    // tokens behind the sequence have no score, a half without tokens no scales that anybody wrote
+                    if (valid <= 16) ksc[1] = vsc[1] = 1.f;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt) {
+                            const int c = u * 16 + nt * 8 + tig;
+                            if (c >= valid) s[u][nt][0] = s[u][nt][2] = -INFINITY;
+                            if (c + 4 >= valid) s[u][nt][1] = s[u][nt][3] = -INFINITY;
+                        }
+                }
+                // ---- online softmax on the raw scores: y = s * f, V scale in the exponent ----
+                float f0[2], f1[2], lv[2];
+                float mn0 = -INFINITY, mn1 = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    f0[u] = fmaxf(mul0 * ksc[u], kMinFactor);
+                    f1[u] = fmaxf(mul1 * ksc[u], kMinFactor);
+                    lv[u] = log2_approx(vsc[u]);
+                    mn0 = fmaxf(mn0, fmaf(fmaxf(fmaxf(s[u][0][0], s[u][0][1]), fmaxf(s[u][1][0], s[u][1][1])), f0[u], lv[u]));
+                    mn1 = fmaxf(mn1, fmaf(fmaxf(fmaxf(s[u][0][2], s[u][0][3]), fmaxf(s[u][1][2], s[u][1][3])), f1[u], lv[u]));
                 }
                 if (kScores) {
 #pragma unroll
@@ -418,20 +477,25 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                         if (g + 8 * r < rows) {
                             float* dst = p.scores + (head0 + g + 8 * r) * p.capacity + tok0 + tig;
 #pragma unroll
-                            for (int nt = 0; nt < 2; ++nt) {
-                                if (nt * 8 + tig < valid) dst[nt * 8] = s[nt][2 * r];
-                                if (nt * 8 + tig + 4 < valid) dst[nt * 8 + 4] = s[nt][2 * r + 1];
-                            }
+                            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                                for (int nt = 0; nt < 2; ++nt) {
+                                    const int c = u * 16 + nt * 8;
+                                    const float f = r ? f1[u] : f0[u];
+                                    if (c + tig < valid) dst[c] = s[u][nt][2 * r] * f;
+                                    if (c + tig + 4 < valid) dst[c + 4] = s[u][nt][2 * r + 1] * f;
+                                }
                         }
                     }
                 }
-                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-                const float mn0 = fmaxf(m0, mx0 + lv), mn1 = fmaxf(m1, mx1 + lv);
-                if (__any_sync(0xffffffffu, (mn0 > m0) || (mn1 > m1))) {
-                    const float a0 = fast_exp2(m0 - mn0), a1 = fast_exp2(m1 - mn1);
+                // the reference is raised only when a p' would pass 2^15
+                if (__any_sync(0xffffffffu, (mn0 > m0 + kLazy) || (mn1 > m1 + kLazy))) {
+                    mn0 = fmaxf(mn0, __shfl_xor_sync(0xffffffffu, mn0, 1));
+                    mn1 = fmaxf(mn1, __shfl_xor_sync(0xffffffffu, mn1, 1));
+                    mn0 = fmaxf(mn0, __shfl_xor_sync(0xffffffffu, mn0, 2));
+                    mn1 = fmaxf(mn1, __shfl_xor_sync(0xffffffffu, mn1, 2));
+                    const float r0 = fmaxf(m0, mn0), r1 = fmaxf(m1, mn1);
+                    const float a0 = fast_exp2(m0 - r0), a1 = fast_exp2(m1 - r1);
                     l0 *= a0;
                     l1 *= a1;
 #pragma unroll
@@ -441,47 +505,54 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                         o[i][2] *= a1;
                         o[i][3] *= a1;
                     }
-                    m0 = mn0;
-                    m1 = mn1;
+                    m0 = r0;
+                    m1 = r1;
                 }
-                uint32_t pa[4];
-                {
-                    const float c0 = lv + kPShift - m0, c1 = lv + kPShift - m1;
-                    const float p00 = fast_exp2(s[0][0] + c0), p01 = fast_exp2(s[0][1] + c0);
-                    const float p02 = fast_exp2(s[0][2] + c1), p03 = fast_exp2(s[0][3] + c1);
-                    const float p10 = fast_exp2(s[1][0] + c0), p11 = fast_exp2(s[1][1] + c0);
-                    const float p12 = fast_exp2(s[1][2] + c1), p13 = fast_exp2(s[1][3] + c1);
-                    l0 += ((p00 + p01) + (p10 + p11)) * iv;
-                    l1 += ((p02 + p03) + (p12 + p13)) * iv;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t vw[4][4];
+#pragma unroll
+                    for (int cp = 0; cp < 4; ++cp)
+                        ldmatrix_x4_trans(vb + (v_row + u * 16) * 128u + ((static_cast<uint32_t>(cp * 2 + (lane >> 4)) ^ (v_row & 7u)) << 4),
+                                          vw[cp][0], vw[cp][1], vw[cp][2], vw[cp][3]);
+                    const float iv = rcp_approx(vsc[u]);
+                    const float c0 = lv[u] + kPShift - m0, c1 = lv[u] + kPShift - m1;
+                    const float p00 = fast_exp2(fmaf(s[u][0][0], f0[u], c0)), p01 = fast_exp2(fmaf(s[u][0][1], f0[u], c0));
+                    const float p02 = fast_exp2(fmaf(s[u][0][2], f1[u], c1)), p03 = fast_exp2(fmaf(s[u][0][3], f1[u], c1));
+                    const float p10 = fast_exp2(fmaf(s[u][1][0], f0[u], c0)), p11 = fast_exp2(fmaf(s[u][1][1], f0[u], c0));
+                    const float p12 = fast_exp2(fmaf(s[u][1][2], f1[u], c1)), p13 = fast_exp2(fmaf(s[u][1][3], f1[u], c1));
+                    l0 = fmaf((p00 + p01) + (p10 + p11), iv, l0);
+                    l1 = fmaf((p02 + p03) + (p12 + p13), iv, l1);
+                    uint32_t pa[4];
                     pa[0] = pack_f16x2(p00, p01);
                     pa[1] = pack_f16x2(p02, p03);
                     pa[2] = pack_f16x2(p10, p11);
                     pa[3] = pack_f16x2(p12, p13);
-                }
-                // ---- O += P V ----
-                // bytes of tokens behind the sequence may be NaN codes, which a zero probability does not silence
-                uint32_t keep_lo = 0xffffffffu, keep_hi = 0xffffffffu;
-                if (valid < 16) {
-                    keep_lo = (tig < valid ? 0x0000ffffu : 0u) | (tig + 4 < valid ? 0xffff0000u : 0u);
-                    keep_hi = (tig + 8 < valid ? 0x0000ffffu : 0u) | (tig + 12 < valid ? 0xffff0000u : 0u);
-                }
+                    // ---- O += P V: {a: d, d+1 | b: d, d+1} -> {a.d, b.d, a.d+1, b.d+1} -> f16 pairs ----
+                    uint32_t sel_lo = 0x3120u, sel_hi = 0x3120u;
+                    if (valid < kSubTok) {
+                        // values of tokens behind the sequence may be NaN codes, which a zero probability does not
+                        // silence: zero bytes in their place
+                        const int c = u * 16 + tig;
+                        sel_lo = (c < valid ? 0x0100u : 0x0404u) | (c + 4 < valid ? 0x3020u : 0x4040u);
+                        sel_hi = (c + 8 < valid ? 0x0100u : 0x0404u) | (c + 12 < valid ? 0x3020u : 0x4040u);
+                    }
 #pragma unroll
-                for (int cp = 0; cp < 4; ++cp) {
-                    const uint32_t chunk = (static_cast<uint32_t>(cp * 2 + (lane >> 4))) ^ (v_row & 7u);
-                    uint32_t w[4];
-                    ldmatrix_x4_trans(vb + v_row * 128u + (chunk << 4), w[0], w[1], w[2], w[3]);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
+                    for (int c = 0; c < 8; ++c) {
                         uint32_t e0, e1, d0, d1;
-                        decode_token_pairs<kFmt>(w[2 * c] & keep_lo, e0, d0);
-                        decode_token_pairs<kFmt>(w[2 * c + 1] & keep_hi, e1, d1);
-                        mma_f16_16816(o[(cp * 2 + c) * 2], pa, e0, e1);
-                        mma_f16_16816(o[(cp * 2 + c) * 2 + 1], pa, d0, d1);
+                        decode4_f16<kFmt>(__byte_perm(vw[c >> 1][2 * (c & 1)], 0u, sel_lo), e0, d0);
+                        decode4_f16<kFmt>(__byte_perm(vw[c >> 1][2 * (c & 1) + 1], 0u, sel_hi), e1, d1);
+                        mma_f16_16816(o[c * 2], pa, e0, e1);
+                        mma_f16_16816(o[c * 2 + 1], pa, d0, d1);
                     }
                 }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty_bar(slot));
+            if ((slot += kGroups) >= kStages) {
+                slot -= kStages;
+                phase ^= 1u;
+            }
         }
 
         // ---- merge the eight private states ----
@@ -691,7 +762,7 @@ static int encode_cache_map(CUtensorMap* map, const void* base, int B, int capac
     cuuint32_t box[4] = {kD, bshd ? 1u : kTok, bshd ? kTok : 1u, 1u};
     cuuint32_t es[4] = {1, 1, 1, 1};
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, es,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         t_last_cuda_error = static_cast<int>(cudaErrorInvalidValue);
@@ -704,6 +775,10 @@ template <int kFmt, bool kScores>
 static int decode_launch_kernel(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const DecodeParams& p, int W,
                                 std::atomic<bool>* attr_set, cudaStream_t st) {
     if (!*attr_set) {
+        // refuse to launch, rather than wait inside setmaxnreg, should the compiler have given the kernel a smaller pool
+        cudaFuncAttributes fa;
+        CLLO_CUDA_TRY(cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(decode_kernel<kFmt, kScores>)));
+        if (fa.numRegs < kLaunchRegs) return CLLO_E_UNSUPPORTED;
         CLLO_CUDA_TRY(cudaFuncSetAttribute(decode_kernel<kFmt, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            kDecodeSmemBytes));
         *attr_set = true;

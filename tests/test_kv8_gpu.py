@@ -154,12 +154,12 @@ def test_append_of_special_values(dtype):
 def _check_decode(cache, q, lens, scale, out, lse=None, added=None):
     """Bounds, per value.  Scores: fp32 sums of 128 products, off by at most 128 * 2^-24 of the sum of magnitudes, plus
     2^-19 for rounding and the exponential.  out: half a bf16 step (2^-8 relative), the probabilities' rounding to f16
-    (2^-11) and the normaliser's error, relative to sum p|v|.  The probabilities times their V scales are brought to at
-    most 2^15 before they become f16, whose steps are 2^-24 at least: half of that, 2^-40 of the largest, times |v8| is
-    what any token can be off by where that is more than 2^-11 of its own."""
+    (2^-11) and the normaliser's error, relative to sum p|v|.  The probabilities times their V scales are brought to
+    [2^11, 2^15] (the largest one) before they become f16, whose steps are 2^-24 at least: half of that, 2^-36 of the
+    largest, times |v8| is what any token can be off by where that is more than 2^-11 of its own."""
     want, want_lse, p, mag, size, floor = ref.decode(q, cache, lens, scale)
     ds = size * (128 * 2.0 ** -24) + 2.0 ** -19
-    tol = want.abs() * 2.0 ** -8 + mag * (2.0 ** -11 + 2 * ds[..., None] + 2.0 ** -16) + 2.0 ** -40 * floor + 1e-30
+    tol = want.abs() * 2.0 ** -8 + mag * (2.0 ** -11 + 2 * ds[..., None] + 2.0 ** -16) + 2.0 ** -36 * floor + 1e-30
     worst = ((out.double() - want).abs() / tol).max().item()
     assert worst <= 1, worst
     if lse is not None:
