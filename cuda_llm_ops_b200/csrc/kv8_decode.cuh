@@ -8,10 +8,11 @@
 // Work decomposition, as in the bf16 decode kernel (gqa_decode.cuh): a unit is one (sequence, kv head, block of <= 16
 // query heads), cut into tiles of 64 tokens (at least one, so that an empty sequence writes its zeros); the tiles of all
 // units form one index space that W persistent blocks share evenly.  The lengths live on the device, so every block adds
-// them up for itself and finds its own range.  One producer warp streams the tiles by TMA (8 KB of K, 8 KB of V, 128-byte
-// swizzle, one box each) into a ring; eight consumer warps in two groups take stages alternately, 16 tokens per warp, with
-// a private online softmax state; states are merged through shared memory at the end of a unit, pieces of a cut unit
-// through the workspace by the last block to arrive.
+// them up for itself and finds its own range.  Four producer warps stream the tiles by TMA (8 KB of K, 8 KB of V, 128-byte
+// swizzle, one box each) into a ring of eight stages; eight consumer warps in four groups take the tiles in turn, 32 tokens
+// per warp, with a private online softmax state; states are merged through shared memory at the end of a unit, pieces of
+// a cut unit through the workspace by the last block to arrive.  All SMs take part: at 8 stages (128 KB) the bytes in
+// flight stay below what slows the memory system (12 stages: 5 % slower on 148 SMs), and it is the arithmetic that bounds.
 //
 // Arithmetic on codes.  The codes become f16, which holds every e4m3 and int8 value exactly, and feed mma.sync
 // m16n8k16 with fp32 accumulation; the scales never touch the codes:
@@ -42,42 +43,47 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 constexpr int kTok = 64;  // tokens per stage
-#ifndef CLLO_KV8_STAGES
-#define CLLO_KV8_STAGES 12
-#endif
-constexpr int kStages = CLLO_KV8_STAGES;
-#ifndef CLLO_KV8_GROUPS
-#define CLLO_KV8_GROUPS 4
-#endif
-constexpr int kGroups = CLLO_KV8_GROUPS;
+constexpr int kStages = 8;
+constexpr int kGroups = 4;
 constexpr int kWarpsPerGroup = 2;
-constexpr int kSubTok = kTok / kWarpsPerGroup;  // tokens per warp and stage: two halves of 16
+constexpr int kSubTok = kTok / kWarpsPerGroup;  // tokens per warp and stage
+constexpr int kParts = kSubTok / 16;            // 16 tokens each: one k-step of P V
 constexpr int kConsumerWarps = kGroups * kWarpsPerGroup;
-// Two consumer warpgroups and one for the producer (its other warps only complete the warpgroup, which setmaxnreg needs):
-// the consumers hold a unit's Q and O fragments, 96 registers, and 32 tokens' codes and scores beside them.  The pool is
-// what the block was launched with; asking for more in total would never return.
+// Two consumer warpgroups and one of producers.  The consumers hold a unit's Q and O fragments, 96 registers, and the codes
+// and scores of their tokens beside them; at the 168 registers that 384 threads get they would spill.  The pool is what
+// the block was launched with; asking for more in total would never return.
 constexpr int kDecodeThreads = (kConsumerWarps + 4) * 32;
 constexpr int kLaunchRegs = 168, kConsumerRegs = 232, kProducerRegs = 40;
 static_assert(2 * kConsumerRegs + kProducerRegs <= 3 * kLaunchRegs, "setmaxnreg budget exceeds the block's register pool");
 static_assert(kConsumerWarps == 8 && kDecodeThreads == 384, "the register budget is for three warpgroups");
-constexpr int kTileBytes = kTok * kD;         // K or V of one stage
+constexpr int kTileBytes = kTok * kD;           // K or V of one stage
 constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kRows = 16;
 constexpr int kPW = kD + 2;                   // {O[128], m (log2 units), l}
 constexpr int kSlotFloats = kRows * kPW;
-constexpr int kSmemStat = kStages * kStageBytes;
-constexpr int kSmemXchg = kSmemStat + kConsumerWarps * 4 * 32 * 4;
-constexpr int kSmemBar = kSmemXchg + kConsumerWarps * 16 * 32 * 4;
-constexpr int kSmemScale = kSmemBar + 2 * kStages * 8;  // per stage: K and V scales of its four 16-token quarters
 constexpr int kQuarters = kTok / 16;
+constexpr int kQPitch = kD * 2 + 16;          // a query row in shared memory; the padding spreads the rows over the banks
+constexpr int kQBytes = kRows * kQPitch;      // two of them: the next unit's rows arrive while this one's are in use
+// shared memory: ring | exchange of the eight states | their (m, l) | Q x 2 | barriers | block scales per stage | misc
+constexpr int kSmemXchg = kStages * kStageBytes;
+constexpr int kSmemStat = kSmemXchg + kConsumerWarps * 16 * 32 * 4;
+constexpr int kSmemQ = kSmemStat + kConsumerWarps * 4 * 32 * 4;
+constexpr int kSmemBar = kSmemQ + 2 * kQBytes;
+constexpr int kNumBars = 2 * kStages + 4;
+constexpr int kSmemScale = kSmemBar + kNumBars * 8;
 constexpr int kSmemMisc = kSmemScale + kStages * 2 * kQuarters * 4;
 constexpr int kDecodeSmemBytes = kSmemMisc + 16 + 1024;
+static_assert(kDecodeSmemBytes <= 227 * 1024, "shared memory of a block");
+// What a unit costs beyond its tiles (its query rows, the merge of the eight states, the output), in tiles.  The shares of
+// the blocks are cut in these units, so that a block that gets many short sequences is not the last one to finish: 17
+// sequences of 0 to 16384 tokens, 8 kv heads: 81 us at 0, 61 at 4, 55 at 6, 49 at 12, 53 at 16; no effect on full batches.
+constexpr int kUnitCost = 10;
 constexpr float kLazy = 4.f;                 // a reference may lag behind the true maximum by this much (log2)
 constexpr float kPShift = 15.f - kLazy;      // p' <= 2^15
 constexpr float kMinFactor = 7.888609e-31f;  // 2^-100: a score is at most 2^31 times its factor, so this much is nothing
 static_assert(kStages % kGroups == 0, "a stage buffer must always belong to the same consumer group");
 
-enum : int { SITE_KV8_FULL = 80, SITE_KV8_EMPTY = 81, SITE_KV8_DRAIN = 82 };
+enum : int { SITE_KV8_FULL = 80, SITE_KV8_EMPTY = 81, SITE_KV8_DRAIN = 82, SITE_KV8_Q_FULL = 83, SITE_KV8_Q_EMPTY = 84 };
 
 struct DecodeParams {
     const __nv_bfloat16* q;
@@ -97,8 +103,9 @@ struct DecodeParams {
 using decode::worker_lo;
 using decode::worker_of_tile;
 
-// tiles of a sequence; an empty one has one, so that its output is written
-__device__ __forceinline__ int tiles_of(int len) { return len <= 0 ? 1 : (len + kTok - 1) / kTok; }
+// cells of a unit in the index space that the blocks share: kUnitCost without a tile, then one per tile; an empty
+// sequence has one tile, so that its output is written
+__device__ __forceinline__ int cells_of(int len) { return kUnitCost + (len <= 0 ? 1 : (len + kTok - 1) / kTok); }
 
 // sum over the warp's 32 lanes and inclusive prefix
 __device__ __forceinline__ long long warp_incl_sum(long long v, int lane) {
@@ -111,9 +118,9 @@ __device__ __forceinline__ long long warp_incl_sum(long long v, int lane) {
 }
 
 struct Share {
-    long long T, W, lo, hi;   // all tiles, blocks that take part, this block's range
-    int b;                    // the sequence that holds tile lo
-    long long seq_lo;         // index of that sequence's first tile
+    long long T, W, lo, hi;   // all cells, blocks that take part, this block's range
+    int b;                    // the sequence that holds cell lo
+    long long seq_lo;         // index of that sequence's first cell
 };
 
 // Every warp of the block finds the block's share for itself: two passes over the lengths, the second from L1.
@@ -121,9 +128,10 @@ __device__ __forceinline__ Share find_share(const DecodeParams& p, int lane) {
     const int U = p.Hkv * p.n_gblk;
     Share s;
     long long sum = 0;
-    for (int i = lane; i < p.B; i += 32) sum += tiles_of(clamp_len(__ldg(p.seq_lens + i), p.capacity));
+    for (int i = lane; i < p.B; i += 32) sum += cells_of(clamp_len(__ldg(p.seq_lens + i), p.capacity));
     s.T = __shfl_sync(0xffffffffu, warp_incl_sum(sum, lane), 31) * U;
-    // no more blocks than tiles: every block of a cut unit then holds a piece of it, which the count of pieces relies on
+    // no more blocks than cells: every block between the first and the last tile of a unit then holds some of its tiles,
+    // which the count of pieces relies on
     s.W = gridDim.x < s.T ? gridDim.x : s.T;
     s.lo = s.hi = 0;
     if (blockIdx.x < s.W) {
@@ -136,7 +144,7 @@ __device__ __forceinline__ Share find_share(const DecodeParams& p, int lane) {
     long long before = 0;
     for (int i0 = 0; i0 < p.B; i0 += 32) {
         const int i = i0 + lane;
-        const long long n = i < p.B ? static_cast<long long>(tiles_of(clamp_len(__ldg(p.seq_lens + i), p.capacity))) * U : 0;
+        const long long n = i < p.B ? static_cast<long long>(cells_of(clamp_len(__ldg(p.seq_lens + i), p.capacity))) * U : 0;
         const long long end = before + warp_incl_sum(n, lane);
         const unsigned holds = __ballot_sync(0xffffffffu, s.lo < end);
         if (holds) {
@@ -165,8 +173,10 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
     return r;
 }
-__device__ __forceinline__ void lds64(uint32_t addr, float (&x)[2]) {
-    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(x[0]), "=f"(x[1]) : "r"(addr));
+__device__ __forceinline__ float lds32(uint32_t addr) {
+    float x;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr));
+    return x;
 }
 // 4-byte asynchronous copy, and an arrival on a barrier once this thread's earlier ones have landed
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
@@ -174,6 +184,16 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
 }
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint2 lds64u(uint32_t addr) {
+    uint2 r;
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(addr));
+    return r;
+}
+// untiled asynchronous copy, 16-byte aligned, size a multiple of 16
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 __device__ __forceinline__ float log2_approx(float x) {
     float y;
@@ -241,12 +261,18 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     volatile int* misc = abort_flag + 1;
     auto full_bar = [&](int s) { return bar_base + s * 8; };
     auto empty_bar = [&](int s) { return bar_base + (kStages + s) * 8; };
+    auto q_full_bar = [&](int s) { return bar_base + (2 * kStages + s) * 8; };
+    auto q_empty_bar = [&](int s) { return bar_base + (2 * kStages + 2 + s) * 8; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full_bar(s), 1 + 2 * kQuarters);  // the tile copy and the eight scale copies
             mbar_init(empty_bar(s), kWarpsPerGroup);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(q_full_bar(s), 1);
+            mbar_init(q_empty_bar(s), kConsumerWarps);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -259,73 +285,96 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
     if (warp >= kConsumerWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-        if (warp > kConsumerWarps) return;
-        // ------------------------------ producer ------------------------------
-        // Lane 0 issues the tile copies; lanes 0-7 copy one block scale each (a quarter's K or V scale) into the stage, and
-        // their arrivals are part of the stage's full barrier.
+        // ------------------------------ producers ------------------------------
+        // One warp per consumer group, each with the group's own three stages: a wait, two tile copies and the scale copies
+        // take the issuing thread about as long as a block at full bandwidth has for two tiles, so one producer for all
+        // groups was what bounded the kernel.  Lane 0 copies the tiles, lanes 0-7 one block scale each (a quarter's K or V
+        // scale); their arrivals are part of the stage's full barrier.  The first producer also brings the query rows.
+        const int grp = warp - kConsumerWarps;
         if (lane < 2 * kQuarters) {
             if (lane == 0) {
                 tma_prefetch_desc(&tm_k);
                 tma_prefetch_desc(&tm_v);
             }
             int b = share.b;
-            int n_t = tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
-            const long long in_seq = lo - share.seq_lo;
-            int unit = static_cast<int>(in_seq / n_t);
-            int tile = static_cast<int>(in_seq - static_cast<long long>(unit) * n_t);
+            int n_cells = cells_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
+            const long long pos = lo - share.seq_lo;
+            int unit = static_cast<int>(pos / n_cells);
+            int cell = static_cast<int>(pos - static_cast<long long>(unit) * n_cells);  // of the unit, next to look at
             int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
-            int slot = 0;
-            uint32_t phase = 0;
+            int slot = grp, q_slot = 0;
+            uint32_t phase = 0, q_phase = 0;
+            int turn = 0;  // the group whose turn the next tile is
             const bool bshd = p.kv_layout == CLLO_KV_BSHD;
-            const int n_tiles = static_cast<int>(hi - lo);
             const float* scales = lane < kQuarters ? p.k_scale : p.v_scale;
-            const float* row = scales + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
             const int quarter = lane % kQuarters;
             const uint32_t scale_dst = base + kSmemScale + lane * 4;
+            long long left = hi - lo;  // cells of this block's range still ahead
 #pragma unroll 1
-            for (int it = 0; it < n_tiles; ++it) {
-                mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag, SITE_KV8_EMPTY, slot);
-                const int s0 = tile * kTok;
-                int blk = (s0 + quarter * 16) >> p.block_shift;
-                blk = blk < p.n_blocks ? blk : p.n_blocks - 1;  // a quarter behind the cache: any scale, nobody uses it
-                cp_async_4(scale_dst + slot * (2 * kQuarters * 4), row + blk);
-                cp_async_arrive(full_bar(slot));
-                if (lane == 0) {
-                    const int c1 = bshd ? kvh : s0, c2 = bshd ? s0 : kvh;
-                    const uint32_t dst = base + slot * kStageBytes;
-                    mbar_arrive_expect_tx(full_bar(slot), kStageBytes);
-                    tma_load_4d(dst, &tm_k, full_bar(slot), 0, c1, c2, b);
-                    tma_load_4d(dst + kTileBytes, &tm_v, full_bar(slot), 0, c1, c2, b);
-                }
-                if (++slot == kStages) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
-                if (++tile == n_t) {
-                    tile = 0;
-                    if (++gblk == p.n_gblk) {
-                        gblk = 0;
-                        if (++kvh == p.Hkv) {
-                            kvh = 0;
-                            if (++b < p.B) n_t = tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
+            while (left > 0) {
+                const int here = static_cast<int>(left < n_cells - cell ? left : n_cells - cell);  // of this unit
+                int tile = cell - kUnitCost;
+                const int tile_end = tile + here;
+                if (tile < 0) tile = 0;
+                if (tile < tile_end) {
+                    const int n_here = tile_end - tile;
+                    if (grp == 0 && lane == 0) {
+                        const int rows = (p.G - gblk * kRows) < kRows ? (p.G - gblk * kRows) : kRows;
+                        const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(kvh) * p.G + gblk * kRows;
+                        mbar_wait(q_empty_bar(q_slot), q_phase ^ 1u, abort_flag, SITE_KV8_Q_EMPTY, q_slot);
+                        mbar_arrive_expect_tx(q_full_bar(q_slot), rows * kD * 2);
+                        for (int r = 0; r < rows; ++r)
+                            bulk_load(base + kSmemQ + q_slot * kQBytes + r * kQPitch, p.q + (head0 + r) * kD, kD * 2, q_full_bar(q_slot));
+                    }
+                    if ((q_slot ^= 1) == 0) q_phase ^= 1u;
+                    const float* row = scales + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
+#pragma unroll 1
+                    for (tile += (grp - turn + kGroups) % kGroups; tile < tile_end; tile += kGroups) {
+                        mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag, SITE_KV8_EMPTY, slot);
+                        const int s0 = tile * kTok;
+                        int blk = (s0 + quarter * 16) >> p.block_shift;
+                        blk = blk < p.n_blocks ? blk : p.n_blocks - 1;  // a quarter behind the cache: any scale, nobody uses it
+                        cp_async_4(scale_dst + slot * (2 * kQuarters * 4), row + blk);
+                        cp_async_arrive(full_bar(slot));
+                        if (lane == 0) {
+                            const int c1 = bshd ? kvh : s0, c2 = bshd ? s0 : kvh;
+                            const uint32_t dst = base + slot * kStageBytes;
+                            mbar_arrive_expect_tx(full_bar(slot), kStageBytes);
+                            tma_load_4d(dst, &tm_k, full_bar(slot), 0, c1, c2, b);
+                            tma_load_4d(dst + kTileBytes, &tm_v, full_bar(slot), 0, c1, c2, b);
                         }
-                        row = scales + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
+                        if ((slot += kGroups) >= kStages) {
+                            slot -= kStages;
+                            phase ^= 1u;
+                        }
+                    }
+                    turn = (turn + n_here) % kGroups;
+                }
+                left -= here;
+                cell = 0;
+                if (++gblk == p.n_gblk) {
+                    gblk = 0;
+                    if (++kvh == p.Hkv) {
+                        kvh = 0;
+                        if (++b < p.B) n_cells = cells_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
                     }
                 }
             }
-            if (*abort_flag) {
-                // a wait gave up somewhere: make sure no copy is still landing when the block retires
-                const long long n = hi - lo;
-                for (long long it = (n > kStages ? n - kStages : 0); it < n; ++it) {
-                    const int s = static_cast<int>(it % kStages);
-                    const long long t0 = clock64();
-                    while (!mbar_try_wait(full_bar(s), static_cast<uint32_t>(it / kStages) & 1u)) {
+            if (lane == 0 && *abort_flag) {
+                // a wait gave up somewhere: make sure no copy of this warp is still landing when the block retires.  A stage
+                // that was filled n times is in phase n - 1; (slot, phase) say how often each one was.
+                const long long t0 = clock64();
+                auto drain = [&](uint32_t bar, uint32_t parity) {
+                    while (!mbar_try_wait(bar, parity)) {
                         if (clock64() - t0 > kWaitLimitCycles / 64) {
-                            record_timeout(SITE_KV8_DRAIN, s);
+                            record_timeout(SITE_KV8_DRAIN, grp);
                             break;
                         }
                     }
-                }
+                };
+                for (int st = grp; st < kStages; st += kGroups) drain(full_bar(st), st < slot ? phase : phase ^ 1u);
+                if (grp == 0)
+                    for (int st = 0; st < 2; ++st) drain(q_full_bar(st), st < q_slot ? q_phase : q_phase ^ 1u);
             }
         }
         return;
@@ -344,80 +393,88 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     const uint32_t k_row = static_cast<uint32_t>(sub * kSubTok + tok_g);
 
     int b = share.b;
-    long long unit_lo;
-    int n_t, unit;  // unit within the sequence
     int len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
-    n_t = tiles_of(len);
-    unit = static_cast<int>((lo - share.seq_lo) / n_t);
-    unit_lo = share.seq_lo + static_cast<long long>(unit) * n_t;
+    int n_cells = cells_of(len);
+    int unit = static_cast<int>((lo - share.seq_lo) / n_cells);  // within the sequence
+    long long unit_lo = share.seq_lo + static_cast<long long>(unit) * n_cells;
     bool first_unit = true;
-    int slot = grp;  // the next stage of this group; its stages are taken in order across units
+    int turn = 0;    // the group whose turn the next tile is
+    int slot = grp;  // the next stage of this warp's group
     uint32_t phase = 0;
+    int q_slot = 0;
+    uint32_t q_phase = 0;
 
 #pragma unroll 1
     while (unit_lo < hi) {
-        const long long unit_hi = unit_lo + n_t;
-        const long long seg_lo = lo > unit_lo ? lo : unit_lo;
-        const long long seg_hi = hi < unit_hi ? hi : unit_hi;
+        const int n_t = n_cells - kUnitCost;
+        // this block's tiles of the unit
+        int tile = lo > unit_lo + kUnitCost ? static_cast<int>(lo - unit_lo) - kUnitCost : 0;
+        const int tile_end = hi < unit_lo + n_cells ? static_cast<int>(hi - unit_lo) - kUnitCost : n_t;
+        const bool whole = tile == 0 && tile_end == n_t;
+        if (tile < tile_end) {
         const int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
         const int rows = (p.G - gblk * kRows) < kRows ? (p.G - gblk * kRows) : kRows;
         const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(kvh) * p.G + gblk * kRows;
+
         // Q fragments: k-step (j, w) takes dims 16 (tig + 4 j) + 4 w + {0,1} and + {2,3}
         uint32_t qf[8][4];
-        float mul0, mul1;  // scale * log2(e) * 2^-shift of the two rows
-        {
-            uint2 raw[2][8];
-            float amax[2] = {0.f, 0.f};
+        float mul0, mul1;  // |scale| * log2(e) * 2^-shift of the two rows
+        mbar_wait(q_full_bar(q_slot), q_phase, abort_flag, SITE_KV8_Q_FULL, q_slot);
+        __syncwarp();
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const bool ok = g + 8 * r < rows;
-                const uint2* src = reinterpret_cast<const uint2*>(p.q + (head0 + g + 8 * r) * kD);
+        for (int r = 0; r < 2; ++r) {
+            uint2 raw[8];
+            float amax = 0.f;
+            const bool ok = g + 8 * r < rows;
+            const uint32_t src = base + kSmemQ + q_slot * kQBytes + (g + 8 * r) * kQPitch + tig * 32;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    raw[r][i] = ok ? __ldg(src + 4 * (tig + 4 * (i >> 2)) + (i & 3)) : make_uint2(0u, 0u);
-                }
+            for (int i = 0; i < 8; ++i) raw[i] = ok ? lds64u(src + (i >> 2) * 128 + (i & 3) * 8) : make_uint2(0u, 0u);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    amax[r] = fmaxf(amax[r], fmaxf(fmaxf(finite_abs(bf16_lo(raw[r][i].x)), finite_abs(bf16_hi(raw[r][i].x))),
-                                                   fmaxf(finite_abs(bf16_lo(raw[r][i].y)), finite_abs(bf16_hi(raw[r][i].y)))));
-                amax[r] = fmaxf(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], 1));
-                amax[r] = fmaxf(amax[r], __shfl_xor_sync(0xffffffffu, amax[r], 2));
-                int e = static_cast<int>(__float_as_uint(amax[r]) >> 23) - 127;
-                e = e < -100 ? -100 : e;  // rows below 2^-100 (zero among them): their scores vanish either way
-                const float f = copysignf(exp2_int(14 - e), p.scale_log2);  // the sign of the scale goes with the query
-                (r ? mul1 : mul0) = fabsf(p.scale_log2) * exp2_int(e - 14);
+            for (int i = 0; i < 8; ++i)
+                amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(bf16_lo(raw[i].x)), finite_abs(bf16_hi(raw[i].x))),
+                                         fmaxf(finite_abs(bf16_lo(raw[i].y)), finite_abs(bf16_hi(raw[i].y)))));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+            e = e < -100 ? -100 : e;  // rows below 2^-100 (zero among them): their scores vanish either way
+            const float f = copysignf(exp2_int(14 - e), p.scale_log2);  // the sign of the scale goes with the query
+            (r ? mul1 : mul0) = fabsf(p.scale_log2) * exp2_int(e - 14);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    qf[i][r] = pack_f16x2(bf16_lo(raw[r][i].x) * f, bf16_hi(raw[r][i].x) * f);
-                    qf[i][r + 2] = pack_f16x2(bf16_lo(raw[r][i].y) * f, bf16_hi(raw[r][i].y) * f);
-                }
+            for (int i = 0; i < 8; ++i) {
+                qf[i][r] = pack_f16x2(bf16_lo(raw[i].x) * f, bf16_hi(raw[i].x) * f);
+                qf[i][r + 2] = pack_f16x2(bf16_lo(raw[i].y) * f, bf16_hi(raw[i].y) * f);
             }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_empty_bar(q_slot));
+        if ((q_slot ^= 1) == 0) q_phase ^= 1u;
 
         float o[16][4];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-        // tiles of this group in the segment: local index (t - lo) congruent to grp modulo kGroups
-        const int skip = static_cast<int>((static_cast<long long>(grp) - (seg_lo - lo)) & (kGroups - 1));
-        int tile = static_cast<int>(seg_lo - unit_lo) + skip;  // index within the unit
-        const int tile_end = static_cast<int>(seg_hi - unit_lo);
+        // the groups take the block's tiles in turn, across units, so that a stage always belongs to the same group
+        const int n_here = tile_end - tile;
 #pragma unroll 1
-        for (; tile < tile_end; tile += kGroups) {
+        for (tile += (grp - turn + kGroups) % kGroups; tile < tile_end; tile += kGroups) {
             mbar_wait(full_bar(slot), phase, abort_flag, SITE_KV8_FULL, slot);
             __syncwarp();
             const uint32_t kb = base + slot * kStageBytes, vb = kb + kTileBytes;
             const int tok0 = tile * kTok + sub * kSubTok;
-            const int valid = len - tok0;  // of this warp's 32 tokens; the rest holds whatever the cache holds
+            const int valid = len - tok0;  // of this warp's tokens; the rest holds whatever the cache holds
             if (valid > 0) {
-                float ksc[2], vsc[2];  // of this warp's two halves
-                lds64(base + kSmemScale + slot * (2 * kQuarters * 4) + sub * 8, ksc);
-                lds64(base + kSmemScale + slot * (2 * kQuarters * 4) + kQuarters * 4 + sub * 8, vsc);
-                // ---- scores: 16 heads x 2 x 16 tokens; two accumulators per n-block make independent chains ----
-                float s[2][2][4];
+                float ksc[kParts], vsc[kParts];  // of this warp's 16-token parts
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < kParts; ++u) {
+                    const uint32_t at = base + kSmemScale + slot * (2 * kQuarters * 4) + (sub * kParts + u) * 4;
+                    ksc[u] = lds32(at);
+                    vsc[u] = lds32(at + kQuarters * 4);
+                }
+                // ---- scores: 16 heads x 16 tokens a part; two accumulators per n-block make independent chains ----
+                float s[kParts][2][4];
+#pragma unroll
+                for (int u = 0; u < kParts; ++u) {
                     uint4 kw[2][2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
@@ -450,9 +507,9 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                 }
                 if (valid < kSubTok) {
                     // tokens behind the sequence have no score, a half without tokens no scales that anybody wrote
-                    if (valid <= 16) ksc[1] = vsc[1] = 1.f;
+                    if (kParts > 1 && valid <= 16) ksc[kParts - 1] = vsc[kParts - 1] = 1.f;
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
+                    for (int u = 0; u < kParts; ++u)
 #pragma unroll
                         for (int nt = 0; nt < 2; ++nt) {
                             const int c = u * 16 + nt * 8 + tig;
@@ -461,10 +518,10 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                         }
                 }
                 // ---- online softmax on the raw scores: y = s * f, V scale in the exponent ----
-                float f0[2], f1[2], lv[2];
+                float f0[kParts], f1[kParts], lv[kParts];
                 float mn0 = -INFINITY, mn1 = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < kParts; ++u) {
                     f0[u] = fmaxf(mul0 * ksc[u], kMinFactor);
                     f1[u] = fmaxf(mul1 * ksc[u], kMinFactor);
                     lv[u] = log2_approx(vsc[u]);
@@ -477,7 +534,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                         if (g + 8 * r < rows) {
                             float* dst = p.scores + (head0 + g + 8 * r) * p.capacity + tok0 + tig;
 #pragma unroll
-                            for (int u = 0; u < 2; ++u)
+                            for (int u = 0; u < kParts; ++u)
 #pragma unroll
                                 for (int nt = 0; nt < 2; ++nt) {
                                     const int c = u * 16 + nt * 8;
@@ -509,7 +566,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     m1 = r1;
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < kParts; ++u) {
                     uint32_t vw[4][4];
 #pragma unroll
                     for (int cp = 0; cp < 4; ++cp)
@@ -554,94 +611,82 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                 phase ^= 1u;
             }
         }
+        turn = (turn + n_here) % kGroups;
 
-        // ---- merge the eight private states ----
-        stat[(warp * 4 + 0) * 32 + lane] = m0;
-        stat[(warp * 4 + 1) * 32 + lane] = m1;
-        stat[(warp * 4 + 2) * 32 + lane] = l0;
-        stat[(warp * 4 + 3) * 32 + lane] = l1;
-        named_bar_sync(1, kConsumerWarps * 32);
-        float ms0 = -INFINITY, ms1 = -INFINITY;
+        // ---- merge the private states: every warp posts its (m, l) and, two 16-dim chunks at a time, its O; a warp
+        // sums two values per lane and round over the warps, in fixed order and with each one's factor: chunk 2 rd + (warp >> 2), row
+        // half (warp >> 1) & 1, and of the 32 lanes' quads the half that (warp & 1) says ----
+        *reinterpret_cast<float4*>(stat + (warp * 32 + lane) * 4) = make_float4(m0, m1, l0, l1);
+        float4* post = reinterpret_cast<float4*>(xchg);
+        const int half = (warp >> 1) & 1, my_chunk = warp >> 2;
+        float f[kConsumerWarps], ms = -INFINITY, lt = 0.f, acc[4][2];
 #pragma unroll
-        for (int sw = 0; sw < kConsumerWarps; ++sw) {
-            ms0 = fmaxf(ms0, stat[(sw * 4 + 0) * 32 + lane]);
-            ms1 = fmaxf(ms1, stat[(sw * 4 + 1) * 32 + lane]);
-        }
-        // a state without tokens has l = 0; one whose scores are all NaN has m = -inf and l = NaN, which must survive
-        auto factor = [](float m, float l, float ms) {
-            return l == 0.f ? 0.f : fast_exp2(m - (ms == -INFINITY ? 0.f : ms));
-        };
-        float lt0 = 0.f, lt1 = 0.f;
+        for (int rd = 0; rd < 4; ++rd) {
 #pragma unroll
-        for (int sw = 0; sw < kConsumerWarps; ++sw) {
-            const float wl0 = stat[(sw * 4 + 2) * 32 + lane], wl1 = stat[(sw * 4 + 3) * 32 + lane];
-            lt0 += wl0 * factor(stat[(sw * 4 + 0) * 32 + lane], wl0, ms0);
-            lt1 += wl1 * factor(stat[(sw * 4 + 1) * 32 + lane], wl1, ms1);
-        }
-        lt0 += __shfl_xor_sync(0xffffffffu, lt0, 1);
-        lt0 += __shfl_xor_sync(0xffffffffu, lt0, 2);
-        lt1 += __shfl_xor_sync(0xffffffffu, lt1, 1);
-        lt1 += __shfl_xor_sync(0xffffffffu, lt1, 2);
-        // the four lanes of a row hold different columns: a lane's own l may be 0 where its row's is not
-        const float f0 = m0 == -INFINITY && l0 == 0.f ? 0.f : fast_exp2(m0 - (ms0 == -INFINITY ? 0.f : ms0));
-        const float f1 = m1 == -INFINITY && l1 == 0.f ? 0.f : fast_exp2(m1 - (ms1 == -INFINITY ? 0.f : ms1));
-        // four rounds over the 16-dim chunks 2r and 2r + 1: every warp posts 16 of its 64 (rescaled) values and sums, over the
-        // warps in fixed order, the two it owns: chunk 2r + (warp >> 2), row half (warp >> 1) & 1, dims 4 tig + 2 (warp & 1) + {0, 1}
-        float acc[4][2];
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int c = 2 * r + (i >> 3), half = (i >> 2) & 1, e = i & 3;
-                xchg[(warp * 16 + i) * 32 + lane] = o[2 * c + (e & 1)][half * 2 + (e >> 1)] * (half ? f1 : f0);
-            }
+                for (int r = 0; r < 2; ++r) {  // dims 16 (2 rd + c) + 4 tig + {0..3} of row g + 8 r
+                    const int b0 = 2 * (2 * rd + c);
+                    post[((warp * 2 + c) * 2 + r) * 32 + lane] =
+                        make_float4(o[b0][2 * r], o[b0 + 1][2 * r], o[b0][2 * r + 1], o[b0 + 1][2 * r + 1]);
+                }
             named_bar_sync(1, kConsumerWarps * 32);
-            float a = 0.f, c = 0.f;
+            if (rd == 0) {
+#pragma unroll
+                for (int sw = 0; sw < kConsumerWarps; ++sw) ms = fmaxf(ms, stat[(sw * 32 + lane) * 4 + half]);
+#pragma unroll
+                for (int sw = 0; sw < kConsumerWarps; ++sw) {
+                    // a state without tokens has m = -inf and l = 0; one whose scores are all NaN has m = -inf and l = NaN,
+                    // and its NaN must survive
+                    const float m = stat[(sw * 32 + lane) * 4 + half], l = stat[(sw * 32 + lane) * 4 + 2 + half];
+                    f[sw] = m == -INFINITY && l == 0.f ? 0.f : fast_exp2(m - (ms == -INFINITY ? 0.f : ms));
+                    lt += l * f[sw];
+                }
+                lt += __shfl_xor_sync(0xffffffffu, lt, 1);
+                lt += __shfl_xor_sync(0xffffffffu, lt, 2);
+            }
+            float a0 = 0.f, a1 = 0.f;
 #pragma unroll
             for (int sw = 0; sw < kConsumerWarps; ++sw) {
-                a += xchg[(sw * 16 + 2 * warp) * 32 + lane];
-                c += xchg[(sw * 16 + 2 * warp + 1) * 32 + lane];
+                const float2 x = *reinterpret_cast<const float2*>(
+                    reinterpret_cast<const float*>(&post[((sw * 2 + my_chunk) * 2 + half) * 32 + lane]) + 2 * (warp & 1));
+                a0 += x.x * f[sw];
+                a1 += x.y * f[sw];
             }
-            acc[r][0] = a;
-            acc[r][1] = c;
+            acc[rd][0] = a0;
+            acc[rd][1] = a1;
             named_bar_sync(1, kConsumerWarps * 32);
         }
 
-        // ---- every warp writes its share ----
-        const bool whole = seg_lo == unit_lo && seg_hi == unit_hi;
-        {
-            const int half = (warp >> 1) & 1, row = g + 8 * half;
-            const float mrow = half ? ms1 : ms0, lrow = half ? lt1 : lt0;
-            const int col0 = (warp >> 2) * 16 + 4 * tig + 2 * (warp & 1);
-            if (row < rows) {
-                if (whole) {
-                    const float inv = lrow == 0.f ? 0.f : 1.f / lrow;
+        // ---- every warp writes its share: dims 32 rd + 16 (warp >> 2) + 4 tig + 2 (warp & 1) + {0, 1} of row g + 8 half ----
+        const int col0 = my_chunk * 16 + 4 * tig + 2 * (warp & 1), row = g + 8 * half;
+        if (row < rows) {
+            const bool head_of_row = tig == 0 && (warp & 5) == 0;
+            if (whole) {
+                const float inv = lt == 0.f ? 0.f : 1.f / lt;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        *reinterpret_cast<uint32_t*>(p.o + (head0 + row) * kD + r * 32 + col0) =
-                            pack_bf16x2(acc[r][0] * inv, acc[r][1] * inv);
-                    if (tig == 0 && (warp & 5) == 0) {
-                        const float l2 = lrow == 0.f ? -INFINITY : mrow - kPShift + log2f(lrow);
-                        if (p.lse) p.lse[head0 + row] = l2 * kLn2;
-                        if (kScores) p.lse2[head0 + row] = l2;
-                    }
-                } else {
-                    float* dst = p.slots + (static_cast<long long>(blockIdx.x) * 2 + (first_unit ? 0 : 1)) * kSlotFloats + row * kPW;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        *reinterpret_cast<float2*>(dst + r * 32 + col0) = make_float2(acc[r][0], acc[r][1]);
-                    if (tig == 0 && (warp & 5) == 0) {
-                        dst[kD] = mrow;
-                        dst[kD + 1] = lrow;
-                    }
+                for (int rd = 0; rd < 4; ++rd)
+                    *reinterpret_cast<uint32_t*>(p.o + (head0 + row) * kD + rd * 32 + col0) =
+                        pack_bf16x2(acc[rd][0] * inv, acc[rd][1] * inv);
+                if (head_of_row) {
+                    const float l2 = lt == 0.f ? -INFINITY : ms - kPShift + log2f(lt);
+                    if (p.lse) p.lse[head0 + row] = l2 * kLn2;
+                    if (kScores) p.lse2[head0 + row] = l2;
                 }
+            } else {
+                float* dst = p.slots + (static_cast<long long>(blockIdx.x) * 2 + (first_unit ? 0 : 1)) * kSlotFloats + row * kPW;
+#pragma unroll
+                for (int rd = 0; rd < 4; ++rd)
+                    *reinterpret_cast<float2*>(dst + rd * 32 + col0) = make_float2(acc[rd][0], acc[rd][1]);
+                if (head_of_row) *reinterpret_cast<float2*>(dst + kD) = make_float2(ms, lt);
             }
         }
 
         if (!whole) {
             // this block's piece of the unit is in the workspace: count it in; the last one to arrive merges
             const long long W = share.W;
-            const long long w_first = worker_of_tile(unit_lo, share.T, W), w_last = worker_of_tile(unit_hi - 1, share.T, W);
+            const long long w_first = worker_of_tile(unit_lo + kUnitCost, share.T, W);
+            const long long w_last = worker_of_tile(unit_lo + n_cells - 1, share.T, W);
             const int n_pieces = static_cast<int>(w_last - w_first) + 1;
             unsigned* counter = p.counters + w_first;
             named_bar_sync(1, kConsumerWarps * 32);
@@ -654,13 +699,13 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
             }
             named_bar_sync(1, kConsumerWarps * 32);
             if (misc[0] != 0) {
-                const int row = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
+                const int mrow = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
                 const int which_first = worker_lo(w_first, share.T, W) >= unit_lo ? 0 : 1;
-                if (row < rows) {
+                if (mrow < rows) {
                     float mg[8], mm, ll;
                     merge_pieces(n_pieces, c8,
                                  [&](int i) {
-                                     return p.slots + ((w_first + i) * 2 + (i == 0 ? which_first : 0)) * kSlotFloats + row * kPW;
+                                     return p.slots + ((w_first + i) * 2 + (i == 0 ? which_first : 0)) * kSlotFloats + mrow * kPW;
                                  },
                                  mg, mm, ll);
                     const float inv = ll == 0.f ? 0.f : 1.f / ll;
@@ -669,24 +714,25 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     pk.y = pack_bf16x2(mg[2] * inv, mg[3] * inv);
                     pk.z = pack_bf16x2(mg[4] * inv, mg[5] * inv);
                     pk.w = pack_bf16x2(mg[6] * inv, mg[7] * inv);
-                    *reinterpret_cast<uint4*>(p.o + (head0 + row) * kD + c8) = pk;
+                    *reinterpret_cast<uint4*>(p.o + (head0 + mrow) * kD + c8) = pk;
                     if (c8 == 0) {
                         const float l2 = ll == 0.f ? -INFINITY : mm - kPShift + log2f(ll);
-                        if (p.lse) p.lse[head0 + row] = l2 * kLn2;
-                        if (kScores) p.lse2[head0 + row] = l2;
+                        if (p.lse) p.lse[head0 + mrow] = l2 * kLn2;
+                        if (kScores) p.lse2[head0 + mrow] = l2;
                     }
                 }
             }
         }
 
+        }
         // next unit of this block's range
         first_unit = false;
-        unit_lo = unit_hi;
+        unit_lo += n_cells;
         if (++unit == U) {
             unit = 0;
             if (++b >= p.B) break;
             len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
-            n_t = tiles_of(len);
+            n_cells = cells_of(len);
         }
     }
 }
@@ -737,7 +783,7 @@ static int make_decode_plan(int B, int capacity, int Hq, int Hkv, int D, bool wi
     const long long units = static_cast<long long>(B) * Hkv * plan->n_gblk;
     if (units * kRows > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
     const long long most = units * ((capacity + kTok - 1) / kTok);  // tiles if every sequence filled the cache
-    long long W = num_workers > 0 ? num_workers : (static_cast<long long>(sm_count) * 173) / 200;
+    long long W = num_workers > 0 ? num_workers : sm_count;
     if (W > decode::kFixedCounters) W = decode::kFixedCounters;
     if (W > most) W = most;
     if (W < 1) W = 1;
