@@ -18,6 +18,7 @@ KV_BHSD = 1
 WS_COUNTERS_ZERO = 0x100
 FMT_E4M3 = 0
 FMT_INT8 = 1
+SUMS_ACCUMULATE = 1
 
 _lib = None
 
@@ -57,7 +58,8 @@ _SIGNATURES = {
     "cllo_kv8_decode_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "cllo_kv8_decode_bf16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i, _i, _i,
                                   _i, _vp]),
-    "cllo_attn_weight_sums_bf16": (_i, [_vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _vp]),
+    "cllo_attn_weight_sums_workspace_bytes": (_sz, []),
+    "cllo_attn_weight_sums_bf16": (_i, [_vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _vp, _vp, _sz, _i, _i, _i, _i, _i, _i, _vp]),
     "cllo_kv8_evict": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i,
                             _i, _i, _i, _vp]),
     "cllo_gqa_decode_bf16_noalloc": (_i, [_vp, _vp, _vp, _f, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),

@@ -395,11 +395,17 @@ int cllo_kv8_decode_bf16(const void* q, const void* k_cache, const void* v_cache
                               format, num_workers, static_cast<cudaStream_t>(stream));
 }
 
+size_t cllo_attn_weight_sums_workspace_bytes(void) {
+    DeviceInfo* di = nullptr;
+    if (current_device_info(&di) == CLLO_OK && di->sm_count > 0) return sums::workspace_bytes(di->sm_count);
+    return sums::workspace_bytes(256);  // no device visible: an upper bound for any current part
+}
+
 int cllo_attn_weight_sums_bf16(const void* q, const void* k, const float* lse, const int* seq_lens, float scale, int causal,
-                               int q_start, int window, int accumulate, float* sums, int B, int Sq, int Skv, int Hq,
-                               int Hkv, int D, void* stream) {
-    return sums::launch(q, k, lse, seq_lens, scale, causal, q_start, window, accumulate, sums, B, Sq, Skv, Hq, Hkv, D,
-                        static_cast<cudaStream_t>(stream));
+                               int q_start, int window, int flags, float* sums, void* workspace, size_t workspace_bytes,
+                               int B, int Sq, int Skv, int Hq, int Hkv, int D, void* stream) {
+    return sums::launch(q, k, lse, seq_lens, scale, causal, q_start, window, flags, sums, workspace, workspace_bytes, B, Sq,
+                        Skv, Hq, Hkv, D, static_cast<cudaStream_t>(stream));
 }
 
 int cllo_kv8_evict(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,

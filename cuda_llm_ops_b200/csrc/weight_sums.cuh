@@ -1,4 +1,4 @@
-// Attention weight sums of a prompt: how much weight its queries gave to every key.
+// Attention weight sums of a prompt (tcgen05, tensor memory, TMA): how much weight its queries gave to every key.
 //
 //   sums[b, h, t] (+)= sum over the query heads g of kv head h and the counted queries i of
 //                      e^(scale * q[b,g,i] . k[b,h,t] - lse[b,g,i])            (t <= q_start + i when causal)
@@ -8,124 +8,574 @@
 // q_start + i, is a query of the same sequence and counts when that position is < len.  A window > 0 counts only the last
 // `window` of them: positions >= len - window, or the last rows of q where there are no positions to go by.
 //
-// Plain form: a block of 256 threads owns 64 keys and walks over 64-query tiles in shared memory, 4 x 4 products a thread.
+// The product is formed transposed, S^T = K Q^T: keys are the 128 rows of the accumulator and queries its columns, so a
+// thread that reads its tensor-memory lane holds one key, and the sum over queries is a sum over its own registers -- no
+// reduction across threads, no second product.  Per element that leaves one fused multiply-add (scale and lse), one
+// exponential and one addition.
+//
+// Work decomposition.  A unit is (sequence, kv head, 256 keys): two key tiles that share every query tile.  Its steps are
+// the (head of the group, 128 queries) pairs that the mask lets it see; under a causal mask the first keys have the
+// most.  The steps of all units (plus kUnitCost cells each for what a unit costs by itself) form one index space that the
+// persistent blocks share evenly; the lengths live on the device, so every block works out its share for itself, in closed
+// form per sequence.  A unit cut between blocks leaves one fp32 partial per key and block; the last block to arrive adds
+// them up in block order.
+//
+// Warps: 0-3 key tile 0, 4-7 key tile 1 (one key per thread), 8 TMA producer, 9 MMA issuer, 10 lse loader, 11 idle.
+// Tensor memory: two 128-column accumulators per key tile.  Shared memory: K 2 x 64 KB (the next unit's keys arrive during
+// this one's steps), Q 2 x 32 KB, lse 4 x 512 B.
 #pragma once
 
-#include "host_util.cuh"
+#include "gqa_prefill.cuh"
 #include "kv8_format.cuh"
 
 namespace cllo {
 namespace sums {
 
 constexpr int kD = 128;
-constexpr int kTile = 64;
-constexpr int kPitch = kD + 4;
+constexpr int kKeys = 128, kTiles = 2, kPair = kKeys * kTiles;  // keys per tile and unit
+constexpr int kQ = 128;                                          // queries per step
+constexpr int kThreads = 384;
+constexpr int kUnitCost = 2;
+constexpr int kSlabBytes = 128 * 128;         // [128 rows][64 dims] bf16, one swizzled slab
+constexpr int kTileBytes = 2 * kSlabBytes;
+constexpr int kKStageBytes = kTiles * kTileBytes;
+constexpr int kKStages = 2, kQStages = 2, kLseStages = 4;
+constexpr int kSmemK = 0;
+constexpr int kSmemQ = kKStages * kKStageBytes;
+constexpr int kSmemLse = kSmemQ + kQStages * kTileBytes;
+constexpr int kSmemBar = kSmemLse + kLseStages * kQ * 4;
+constexpr int kNumBars = 2 * kKStages + 2 * kQStages + 2 * kLseStages + 4 * kTiles + 1;
+constexpr int kSmemMisc = kSmemBar + kNumBars * 8;
+constexpr int kSmemBytes = kSmemMisc + 32 + 1024;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kSmemBytes = 2 * kTile * kPitch * 4 + kTile * 4;
+constexpr int kEpiThreads = kTiles * 128;
+
+enum : int {
+    SITE_SUMS_K = 90, SITE_SUMS_Q = 91, SITE_SUMS_LSE = 92, SITE_SUMS_D = 93, SITE_SUMS_DRAIN = 94,
+};
 
 struct Params {
-    const __nv_bfloat16* q;
-    const __nv_bfloat16* k;
     const float* lse;
     const int* seq_lens;  // nullable
     float* out;
+    float* slots;         // [W][2][kPair]
+    unsigned* counters;
     float scale_log2;
-    int Sq, Skv, Hq, Hkv, G, q_start, window, causal, accumulate;
+    int B, Sq, Skv, Hq, Hkv, G, q_start, window, causal, accumulate, n_pairs;
 };
 
-__device__ __forceinline__ void load_tile(float* dst, const __nv_bfloat16* src, int rows) {
-    for (int i = threadIdx.x; i < kTile * (kD / 2); i += blockDim.x) {
-        const int r = i / (kD / 2), c = i % (kD / 2);
-        const uint32_t w = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + static_cast<long long>(r) * kD) + c) : 0u;
-        dst[r * kPitch + 2 * c] = kv8::bf16_lo(w);
-        dst[r * kPitch + 2 * c + 1] = kv8::bf16_hi(w);
+using decode::worker_lo;
+using decode::worker_of_tile;
+
+// The part of a sequence's work that does not depend on the kv head: which queries count, and how many steps a pair of key
+// tiles takes per head.
+struct Seq {
+    int len;           // keys that take part
+    int i_lo, i_hi;    // counted query rows
+    int np;            // pairs that hold keys; of these
+    int p1, n0, m;     // pairs p < p1 see n0 query tiles per head, later ones max(0, m - 2 p)
+    long long cells;   // of all pairs of one kv head
+
+    __device__ __forceinline__ int tiles(int p) const {
+        if (p < p1) return n0;
+        return p < np && m > 2 * p ? m - 2 * p : 0;
+    }
+    // cells of the pairs before p
+    __device__ __forceinline__ long long before(const Params& prm, int p) const {
+        const int a = p < p1 ? p : p1;
+        long long n = static_cast<long long>(n0) * a;
+        // pairs [p1, e) have m - 2 p > 0 tiles
+        int e = (m + 1) / 2;
+        if (e > np) e = np;
+        if (e > p) e = p;
+        if (e > p1) n += static_cast<long long>(m) * (e - p1) - (static_cast<long long>(e) * (e - 1) - static_cast<long long>(p1) * (p1 - 1));
+        return static_cast<long long>(kUnitCost) * p + prm.G * n;
+    }
+};
+
+__device__ __forceinline__ Seq describe(const Params& p, int b) {
+    Seq s;
+    s.len = p.seq_lens ? kv8::clamp_len(__ldg(p.seq_lens + b), p.Skv) : p.Skv;
+    const bool positions = p.causal && p.seq_lens;
+    const long long end = positions ? static_cast<long long>(s.len) - p.q_start : p.Sq;
+    const long long start = p.window > 0 ? end - p.window : 0;
+    s.i_hi = static_cast<int>(end < 0 ? 0 : (end > p.Sq ? p.Sq : end));
+    s.i_lo = static_cast<int>(start < 0 ? 0 : (start > p.Sq ? p.Sq : start));
+    s.np = (s.len + kPair - 1) / kPair;
+    if (s.i_lo >= s.i_hi || s.len == 0) {
+        s.p1 = s.n0 = s.m = 0;
+    } else if (p.causal) {
+        s.n0 = (s.i_hi - s.i_lo + kQ - 1) / kQ;
+        // no query before position t sees key t: later pairs start at their own first key
+        s.p1 = (s.i_lo + p.q_start) / kPair + 1;
+        s.m = (s.i_hi + p.q_start + kQ - 1) / kQ;
+        if (s.p1 > s.np) s.p1 = s.np;
+    } else {
+        s.n0 = (s.i_hi - s.i_lo + kQ - 1) / kQ;
+        s.p1 = s.np;
+        s.m = 0;
+    }
+    s.cells = s.before(p, p.n_pairs);
+    return s;
+}
+
+// Walks over the units of a block's share.  Every role of the block walks for itself.
+struct Walk {
+    long long T, W, lo, hi;
+    long long unit_lo;  // first cell of the current unit
+    int b, kvh, p;
+    Seq seq;
+    // of the current unit
+    int n, steps;       // query tiles per head, steps in all
+    int s_lo, s_hi;     // this block's steps
+    bool first;         // the block's first unit
+
+    __device__ __forceinline__ void enter(const Params& prm) {
+        n = seq.tiles(p);
+        steps = prm.G * n;
+        const long long base = unit_lo + kUnitCost;
+        s_lo = lo > base ? static_cast<int>(lo - base) : 0;
+        s_hi = hi < base + steps ? static_cast<int>(hi - base) : steps;
+    }
+    __device__ __forceinline__ bool done() const { return unit_lo >= hi; }
+    __device__ __forceinline__ bool active() const { return s_lo < s_hi; }
+    __device__ __forceinline__ void next(const Params& prm) {
+        first = false;
+        unit_lo += kUnitCost + steps;
+        if (++p == prm.n_pairs) {
+            p = 0;
+            if (++kvh == prm.Hkv) {
+                kvh = 0;
+                if (++b == prm.B) {
+                    unit_lo = hi;
+                    return;
+                }
+                seq = describe(prm, b);
+            }
+        }
+        if (unit_lo < hi) enter(prm);
+    }
+    // first query row of the unit's tile j, and the number of its columns that count
+    __device__ __forceinline__ int row0(const Params& prm, int j) const {
+        const int own = prm.causal ? p * kPair - prm.q_start : 0;
+        return (own > seq.i_lo ? own : seq.i_lo) + j * kQ;
+    }
+    // whether key tile t of the unit has anything to do with the query tile at row i0
+    __device__ __forceinline__ bool sees(const Params& prm, int t, int i0) const {
+        const int key0 = p * kPair + t * kKeys;
+        return key0 < seq.len && !(prm.causal && prm.q_start + i0 + kQ - 1 < key0);
+    }
+};
+
+__device__ __forceinline__ Walk start_walk(const Params& p, int lane) {
+    Walk w;
+    long long sum = 0;
+    for (int i = lane; i < p.B; i += 32) sum += describe(p, i).cells;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    w.T = sum * p.Hkv;
+    w.W = gridDim.x < w.T ? gridDim.x : w.T;
+    w.lo = w.hi = w.unit_lo = 0;
+    w.b = w.kvh = w.p = 0;
+    w.first = true;
+    if (blockIdx.x >= w.W) return w;
+    w.lo = worker_lo(blockIdx.x, w.T, w.W);
+    w.hi = worker_lo(blockIdx.x + 1, w.T, w.W);
+    long long seq_lo = 0;
+    for (int i0 = 0; i0 < p.B; i0 += 32) {
+        const int i = i0 + lane;
+        const long long n = i < p.B ? describe(p, i).cells * p.Hkv : 0;
+        long long end = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += u;
+        }
+        end += seq_lo;
+        const unsigned holds = __ballot_sync(0xffffffffu, w.lo < end);
+        if (holds) {
+            const int at = __ffs(holds) - 1;
+            w.b = i0 + at;
+            seq_lo = __shfl_sync(0xffffffffu, end - n, at);
+            break;
+        }
+        seq_lo = __shfl_sync(0xffffffffu, end, 31);
+    }
+    w.seq = describe(p, w.b);
+    w.kvh = static_cast<int>((w.lo - seq_lo) / w.seq.cells);
+    const long long head_lo = seq_lo + w.kvh * w.seq.cells;
+    const long long off = w.lo - head_lo;
+    int a = 0, z = p.n_pairs;  // the last pair whose first cell is <= off
+    while (z - a > 1) {
+        const int mid = a + (z - a) / 2;
+        if (w.seq.before(p, mid) <= off)
+            a = mid;
+        else
+            z = mid;
+    }
+    w.p = a;
+    w.unit_lo = head_lo + w.seq.before(p, a);
+    w.enter(p);
+    return w;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const Params p) {
+    using namespace prefill;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
+    float* lse_buf = reinterpret_cast<float*>(gen_base + sums::kSmemLse);
+    const uint32_t bar0 = base + sums::kSmemBar;
+    auto k_full = [&](int s) { return bar0 + 8 * s; };
+    auto k_empty = [&](int s) { return bar0 + 8 * (kKStages + s); };
+    auto q_full = [&](int s) { return bar0 + 8 * (2 * kKStages + s); };
+    auto q_empty = [&](int s) { return bar0 + 8 * (2 * kKStages + kQStages + s); };
+    constexpr int kLseBar = 2 * kKStages + 2 * kQStages;
+    auto lse_full = [&](int s) { return bar0 + 8 * (kLseBar + s); };
+    auto lse_empty = [&](int s) { return bar0 + 8 * (kLseBar + kLseStages + s); };
+    constexpr int kDBar = kLseBar + 2 * kLseStages;
+    auto d_full = [&](int t, int s) { return bar0 + 8 * (kDBar + t * 2 + s); };
+    auto d_empty = [&](int t, int s) { return bar0 + 8 * (kDBar + 2 * sums::kTiles + t * 2 + s); };
+    const uint32_t drain_bar = bar0 + 8 * (sums::kNumBars - 1);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen_base + sums::kSmemMisc);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + sums::kSmemMisc + 8);
+    volatile int* misc = abort_flag + 1;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kKStages; ++s) {
+            mbar_init(k_full(s), 1);
+            mbar_init(k_empty(s), 1);
+        }
+        for (int s = 0; s < kQStages; ++s) {
+            mbar_init(q_full(s), 1);
+            mbar_init(q_empty(s), 1);
+        }
+        for (int s = 0; s < kLseStages; ++s) {
+            mbar_init(lse_full(s), 32);
+            mbar_init(lse_empty(s), kEpiThreads / 32);
+        }
+        for (int t = 0; t < sums::kTiles; ++t)
+            for (int s = 0; s < 2; ++s) {
+                mbar_init(d_full(t, s), 1);
+                mbar_init(d_empty(t, s), 4);
+            }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_relinquish();
+    }
+    Walk w = start_walk(p, lane);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 8) {
+        // ------------------------------- TMA producer -------------------------------
+        if (lane == 0) {
+            tma_prefetch_desc(&tm_q);
+            tma_prefetch_desc(&tm_k);
+            int ks = 0, qs = 0, n_k = 0, n_q = 0;
+            uint32_t kp = 0, qp = 0;
+            for (; !w.done(); w.next(p)) {
+                if (!w.active()) continue;
+                mbar_wait(k_empty(ks), kp ^ 1u, abort_flag, SITE_SUMS_K, ks);
+                const int n_tiles = w.p * kPair + kKeys < w.seq.len ? 2 : 1;  // a second tile without keys is not loaded
+                mbar_arrive_expect_tx(k_full(ks), n_tiles * sums::kTileBytes);
+                for (int t = 0; t < n_tiles; ++t)
+                    for (int d = 0; d < 2; ++d)
+                        tma_load_4d(base + sums::kSmemK + ks * kKStageBytes + t * sums::kTileBytes + d * kSlabBytes, &tm_k, k_full(ks),
+                                    d * 64, w.p * kPair + t * kKeys, w.kvh, w.b);
+                if (++ks == kKStages) {
+                    ks = 0;
+                    kp ^= 1u;
+                }
+                ++n_k;
+                int g = w.s_lo / w.n, j = w.s_lo - g * w.n;
+                for (int s = w.s_lo; s < w.s_hi; ++s) {
+                    mbar_wait(q_empty(qs), qp ^ 1u, abort_flag, SITE_SUMS_Q, qs);
+                    mbar_arrive_expect_tx(q_full(qs), sums::kTileBytes);
+                    for (int d = 0; d < 2; ++d)
+                        tma_load_4d(base + sums::kSmemQ + qs * sums::kTileBytes + d * kSlabBytes, &tm_q, q_full(qs), d * 64,
+                                    w.row0(p, j), w.kvh * p.G + g, w.b);
+                    if (++qs == kQStages) {
+                        qs = 0;
+                        qp ^= 1u;
+                    }
+                    ++n_q;
+                    if (++j == w.n) {
+                        j = 0;
+                        ++g;
+                    }
+                }
+            }
+            if (*abort_flag) {
+                // a wait gave up somewhere: let the copies already issued land before the block retires
+                const long long t0 = clock64();
+                auto drain = [&](uint32_t bar, uint32_t parity) {
+                    while (!mbar_try_wait(bar, parity) && clock64() - t0 < kWaitLimitCycles / 64) {
+                    }
+                };
+                for (int s = 0; s < kKStages; ++s) drain(k_full(s), s < ks ? kp : kp ^ 1u);
+                for (int s = 0; s < kQStages; ++s) drain(q_full(s), s < qs ? qp : qp ^ 1u);
+            }
+        }
+    } else if (warp == 9) {
+        // -------------------------------- MMA issuer --------------------------------
+        // the whole warp runs the loop and the leader lane's predicate guards the MMAs (see tc_mma_ss_lo_if)
+        const uint32_t leader = lane == 0 ? 1u : 0u;
+        const uint32_t hi = smem_desc_hi(1024);
+        int ks = 0, qs = 0, ds[sums::kTiles] = {0, 0};
+        uint32_t kp = 0, qp = 0, dp[sums::kTiles] = {0, 0};
+        for (; !w.done(); w.next(p)) {
+            if (!w.active()) continue;
+            if (lane == 0) mbar_wait(k_full(ks), kp, abort_flag, SITE_SUMS_K, ks);
+            __syncwarp();
+            int j = w.s_lo % w.n;
+            for (int s = w.s_lo; s < w.s_hi; ++s) {
+                if (lane == 0) mbar_wait(q_full(qs), qp, abort_flag, SITE_SUMS_Q, qs);
+                const int i0 = w.row0(p, j);
+#pragma unroll
+                for (int t = 0; t < sums::kTiles; ++t) {
+                    if (!w.sees(p, t, i0)) continue;
+                    if (lane == 0) mbar_wait(d_empty(t, ds[t]), dp[t] ^ 1u, abort_flag, SITE_SUMS_D, t);
+                    __syncwarp();
+                    tc_fence_after();
+                    const uint32_t a = smem_desc_lo(base + sums::kSmemK + ks * kKStageBytes + t * sums::kTileBytes, 16);
+                    const uint32_t bq = smem_desc_lo(base + sums::kSmemQ + qs * sums::kTileBytes, 16);
+                    const uint32_t d = tmem_base + (t * 2 + ds[t]) * kQ;
+                    tc_mma_ss_lo_if<false>(leader, d, a, bq, hi, kIdescQK);
+#pragma unroll
+                    for (int k = 1; k < 8; ++k) {
+                        const uint32_t off = ((k >> 2) * kSlabBytes + (k & 3) * 32) >> 4;
+                        tc_mma_ss_lo_if<true>(leader, d, a + off, bq + off, hi, kIdescQK);
+                    }
+                    tc_commit_if(leader, d_full(t, ds[t]));
+                    if ((ds[t] ^= 1) == 0) dp[t] ^= 1u;
+                }
+                tc_commit_if(leader, q_empty(qs));
+                if (++qs == kQStages) {
+                    qs = 0;
+                    qp ^= 1u;
+                }
+                if (++j == w.n) j = 0;
+            }
+            tc_commit_if(leader, k_empty(ks));
+            if (++ks == kKStages) {
+                ks = 0;
+                kp ^= 1u;
+            }
+        }
+        __syncwarp();
+        if (lane == 0) {
+            // everything issued must have retired before tensor memory is released
+            tc_commit(drain_bar);
+            mbar_wait(drain_bar, 0, abort_flag, SITE_SUMS_DRAIN, 0);
+            if (*abort_flag) {
+                const long long t0 = clock64();
+                while (!mbar_try_wait(drain_bar, 0) && clock64() - t0 < kWaitLimitCycles / 64) {
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 10) {
+        // -------------------------------- lse loader --------------------------------
+        // -lse * log2(e) of the step's 128 queries; -inf (no contribution) for rows that saw no key
+        int ls = 0;
+        uint32_t lp = 0;
+        for (; !w.done(); w.next(p)) {
+            if (!w.active()) continue;
+            int g = w.s_lo / w.n, j = w.s_lo - g * w.n;
+            for (int s = w.s_lo; s < w.s_hi; ++s) {
+                const int i0 = w.row0(p, j);
+                const float* src = p.lse + (static_cast<long long>(w.b) * p.Hq + w.kvh * p.G + g) * p.Sq;
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = i0 + e * 32 + lane;
+                    x[e] = i < w.seq.i_hi ? __ldg(src + i) : -INFINITY;
+                    x[e] = x[e] == -INFINITY ? -INFINITY : -x[e] * sums::kLog2e;
+                }
+                mbar_wait(lse_empty(ls), lp ^ 1u, abort_flag, SITE_SUMS_LSE, ls);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) lse_buf[ls * kQ + e * 32 + lane] = x[e];
+                mbar_arrive(lse_full(ls));
+                if (++ls == kLseStages) {
+                    ls = 0;
+                    lp ^= 1u;
+                }
+                if (++j == w.n) {
+                    j = 0;
+                    ++g;
+                }
+            }
+        }
+    } else if (warp < 8) {
+        // ------------------------- exponentials and sums (one key per thread) -------------------------
+        const int t = warp >> 2;
+        const int key_in_pair = threadIdx.x;  // 0..255
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        int ls = 0, dsl = 0;
+        uint32_t lp = 0, dph = 0;
+        for (; !w.done(); w.next(p)) {
+            const int key = w.p * kPair + key_in_pair;
+            float* out = p.out + (static_cast<long long>(w.b) * p.Hkv + w.kvh) * p.Skv + key;
+            if (!w.active()) {
+                // a unit without steps: whoever holds its first cell clears its sums
+                if (w.steps == 0 && w.unit_lo >= w.lo && key < p.Skv && !p.accumulate) *out = 0.f;
+                continue;
+            }
+            float total = 0.f;
+            int j = w.s_lo % w.n;
+            for (int s = w.s_lo; s < w.s_hi; ++s) {
+                const int i0 = w.row0(p, j);
+                if (++j == w.n) j = 0;
+                mbar_wait(lse_full(ls), lp, abort_flag, SITE_SUMS_LSE, ls);
+                if (w.sees(p, t, i0)) {
+                    mbar_wait(d_full(t, dsl), dph, abort_flag, SITE_SUMS_D, t);
+                    __syncwarp();
+                    tc_fence_after();
+                    const int n_cols = w.seq.i_hi - i0 < kQ ? w.seq.i_hi - i0 : kQ;
+                    const int key0 = w.p * kPair + t * kKeys;
+                    // columns [c_lo, n_cols) of this key's row count
+                    const int c_lo = p.causal ? key - p.q_start - i0 : 0;
+                    const bool need_mask = n_cols < kQ || (p.causal && p.q_start + i0 < key0 + kKeys - 1);
+                    const uint64_t c2 = pk2(p.scale_log2, p.scale_log2);
+                    uint64_t sum2 = pk2(0.f, 0.f), sum3 = sum2;
+#pragma unroll 1
+                    for (int c = 0; c < n_cols; c += 32) {
+                        float x[32];
+                        tmem_ld32_wait(tmem_base + lane_base + (t * 2 + dsl) * kQ + c, x);
+                        const float4* nl = reinterpret_cast<const float4*>(lse_buf + ls * kQ + c);
+                        if (need_mask) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 l4 = nl[e >> 2];
+                                const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+                                for (int f = 0; f < 4; ++f) {
+                                    const int col = c + e + f;
+                                    x[e + f] = col >= c_lo && col < n_cols && l[f] != -INFINITY
+                                                   ? fast_exp2(fmaf(x[e + f], p.scale_log2, l[f])) : 0.f;
+                                }
+                                sum2 = add2(sum2, pk2(x[e], x[e + 1]));
+                                sum3 = add2(sum3, pk2(x[e + 2], x[e + 3]));
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 l4 = nl[e >> 2];
+                                float y0, y1, y2, y3;
+                                upk2(fma2(pk2(x[e], x[e + 1]), c2, pk2(l4.x, l4.y)), y0, y1);
+                                upk2(fma2(pk2(x[e + 2], x[e + 3]), c2, pk2(l4.z, l4.w)), y2, y3);
+                                sum2 = add2(sum2, pk2(fast_exp2(y0), fast_exp2(y1)));
+                                sum3 = add2(sum3, pk2(fast_exp2(y2), fast_exp2(y3)));
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(d_empty(t, dsl));
+                    if ((dsl ^= 1) == 0) dph ^= 1u;
+                    float a0, a1;
+                    upk2(add2(sum2, sum3), a0, a1);
+                    total += a0 + a1;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(lse_empty(ls));
+                if (++ls == kLseStages) {
+                    ls = 0;
+                    lp ^= 1u;
+                }
+            }
+            if (key >= w.seq.len) total = 0.f;  // whatever lies behind the sequence
+            if (w.s_lo == 0 && w.s_hi == w.steps) {
+                if (key < p.Skv) *out = p.accumulate ? *out + total : total;
+                continue;
+            }
+            // this block's part of the unit goes to the workspace; the last block to arrive adds the parts up
+            p.slots[(static_cast<long long>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * kPair + key_in_pair] = total;
+            const long long w_first = worker_of_tile(w.unit_lo + kUnitCost, w.T, w.W);
+            const long long w_last = worker_of_tile(w.unit_lo + kUnitCost + w.steps - 1, w.T, w.W);
+            const int n_pieces = static_cast<int>(w_last - w_first) + 1;
+            named_bar_sync(1, kEpiThreads);
+            if (threadIdx.x == 0) {
+                unsigned* counter = p.counters + w_first;
+                __threadfence();
+                const bool last = atomicAdd(counter, 1u) == static_cast<unsigned>(n_pieces - 1);
+                __threadfence();
+                if (last) *counter = 0u;  // the counters are zero again when the kernel ends
+                *misc = last ? 1 : 0;
+            }
+            named_bar_sync(1, kEpiThreads);
+            if (*misc != 0) {
+                const int which_first = worker_lo(w_first, w.T, w.W) >= w.unit_lo ? 0 : 1;
+                float sum = 0.f;
+                for (int i = 0; i < n_pieces; ++i)
+                    sum += __ldcg(p.slots + ((w_first + i) * 2 + (i == 0 ? which_first : 0)) * kPair + key_in_pair);
+                if (key < p.Skv) *out = p.accumulate ? *out + sum : sum;
+            }
+        }
+        tc_fence_before();
+    }
+
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
     }
 }
 
-__global__ void __launch_bounds__(256) weight_sums_kernel(const Params p) {
-    extern __shared__ float sm[];
-    float* sk = sm;
-    float* sq = sm + kTile * kPitch;
-    float* sl = sq + kTile * kPitch;
-    const int h = blockIdx.y % p.Hkv, b = blockIdx.y / p.Hkv;
-    const int t0 = blockIdx.x * kTile;
-    int len = p.seq_lens ? kv8::clamp_len(p.seq_lens[b], p.Skv) : p.Skv;
-    // counted queries: rows [i_lo, i_hi)
-    long long i_hi = p.causal && p.seq_lens ? static_cast<long long>(len) - p.q_start : p.Sq;
-    long long i_lo = p.window > 0 ? i_hi - p.window : 0;
-    if (i_hi > p.Sq) i_hi = p.Sq;
-    if (i_lo < 0) i_lo = 0;
-    if (p.causal && i_lo < t0 - p.q_start) i_lo = t0 - p.q_start;
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;  // keys ty*4.., queries tx*4..
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    if (t0 < len && i_lo < i_hi) {
-        load_tile(sk, p.k + ((static_cast<long long>(b) * p.Hkv + h) * p.Skv + t0) * kD, p.Skv - t0);
-        for (int g = 0; g < p.G; ++g) {
-            const long long head = static_cast<long long>(b) * p.Hq + h * p.G + g;
-            for (int i0 = static_cast<int>(i_lo); i0 < i_hi; i0 += kTile) {
-                __syncthreads();
-                load_tile(sq, p.q + (head * p.Sq + i0) * kD, static_cast<int>(i_hi) - i0);
-                if (threadIdx.x < kTile)
-                    sl[threadIdx.x] = i0 + static_cast<int>(threadIdx.x) < i_hi ? p.lse[head * p.Sq + i0 + threadIdx.x] * kLog2e : INFINITY;
-                __syncthreads();
-                float acc[4][4] = {};
-                for (int d = 0; d < kD; ++d) {
-                    float a[4], c[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        a[e] = sk[(ty * 4 + e) * kPitch + d];
-                        c[e] = sq[(tx * 4 + e) * kPitch + d];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int f = 0; f < 4; ++f) acc[e][f] += a[e] * c[f];
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) {
-                        const int i = i0 + tx * 4 + f;
-                        const bool counts = i < i_hi && sl[tx * 4 + f] != -INFINITY &&
-                                            (!p.causal || t0 + ty * 4 + e <= p.q_start + i);
-                        if (counts) sum[e] += fast_exp2(acc[e][f] * p.scale_log2 - sl[tx * 4 + f]);
-                    }
-            }
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        for (int o = 8; o; o >>= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
-        const int t = t0 + ty * 4 + e;
-        if (tx == 0 && t < p.Skv) {
-            float* out = p.out + (static_cast<long long>(b) * p.Hkv + h) * p.Skv + t;
-            const float add = t < len ? sum[e] : 0.f;
-            *out = p.accumulate ? *out + add : add;
-        }
-    }
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+static int encode_map(CUtensorMap* map, const void* basep, int B, int H, int S) {
+    const uint64_t row = static_cast<uint64_t>(kD) * 2;
+    const uint64_t dims[4] = {static_cast<uint64_t>(kD), static_cast<uint64_t>(S), static_cast<uint64_t>(H),
+                              static_cast<uint64_t>(B)};
+    const uint64_t strides[3] = {row, row * S, row * S * H};
+    const uint32_t box[4] = {64, 128, 1, 1};
+    return encode_bf16_4d(map, basep, dims, strides, box);
+}
+
+static int blocks_for(int sm_count) {
+    return sm_count < decode::kFixedCounters ? sm_count : decode::kFixedCounters;
+}
+static size_t workspace_bytes(int sm_count) {
+    return decode::kSlotOffsetBytes + static_cast<size_t>(blocks_for(sm_count)) * 2 * kPair * sizeof(float);
 }
 
 static int launch(const void* q, const void* k, const float* lse, const int* seq_lens, float scale, int causal, int q_start,
-                  int window, int accumulate, float* out, int B, int Sq, int Skv, int Hq, int Hkv, int D, cudaStream_t st) {
+                  int window, int flags, float* out, void* workspace, size_t ws_bytes, int B, int Sq, int Skv, int Hq,
+                  int Hkv, int D, cudaStream_t st) {
     if (!q || !k || !lse || !out) return CLLO_E_BAD_ARG;
     if (B <= 0 || Sq <= 0 || Skv <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq % Hkv != 0) return CLLO_E_BAD_ARG;
-    if (q_start < 0 || window < 0 || !isfinite(scale)) return CLLO_E_BAD_ARG;
+    if (q_start < 0 || window < 0 || !isfinite(scale) || (flags & ~(CLLO_SUMS_ACCUMULATE | CLLO_WS_COUNTERS_ZERO)))
+        return CLLO_E_BAD_ARG;
     if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(lse, 4) || !aligned_to(out, 4) || !aligned_to(seq_lens, 4))
         return CLLO_E_BAD_ARG;
-    if (D != kD) return CLLO_E_UNSUPPORTED;
-    if (static_cast<long long>(B) * Hkv > 65535 || Sq > (1 << 30) || Skv > (1 << 30) || q_start > (1 << 30))
-        return CLLO_E_UNSUPPORTED;
+    const int most = 1 << 30;
+    if (D != kD || Sq > most || Skv > most || q_start > most / 2) return CLLO_E_UNSUPPORTED;
+    const long long tiles = static_cast<long long>(Hq / Hkv) * ((Sq + kQ - 1) / kQ);
+    if (tiles > most) return CLLO_E_UNSUPPORTED;  // a unit's steps are counted in 32 bits
     DeviceInfo* di = nullptr;
     int rc = current_device_info(&di);
     if (rc != CLLO_OK) return rc;
     if (di->cc_major != 10) return CLLO_E_UNSUPPORTED;
+    if (!workspace || ws_bytes < workspace_bytes(di->sm_count) || !aligned_to(workspace, 256)) return CLLO_E_WORKSPACE;
     Params p;
-    p.q = static_cast<const __nv_bfloat16*>(q);
-    p.k = static_cast<const __nv_bfloat16*>(k);
     p.lse = lse;
     p.seq_lens = seq_lens;
     p.out = out;
+    p.counters = static_cast<unsigned*>(workspace);
+    p.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + decode::kSlotOffsetBytes);
     p.scale_log2 = scale * kLog2e;
+    p.B = B;
     p.Sq = Sq;
     p.Skv = Skv;
     p.Hq = Hq;
@@ -134,12 +584,18 @@ static int launch(const void* q, const void* k, const float* lse, const int* seq
     p.q_start = q_start;
     p.window = window;
     p.causal = causal ? 1 : 0;
-    p.accumulate = accumulate ? 1 : 0;
+    p.accumulate = flags & CLLO_SUMS_ACCUMULATE ? 1 : 0;
+    p.n_pairs = (Skv + kPair - 1) / kPair;
+    CUtensorMap tm_q, tm_k;
+    if ((rc = encode_map(&tm_q, q, B, Hq, Sq)) != CLLO_OK) return rc;
+    if ((rc = encode_map(&tm_k, k, B, Hkv, Skv)) != CLLO_OK) return rc;
     if (!di->sums_attr_set) {
         CLLO_CUDA_TRY(cudaFuncSetAttribute(weight_sums_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
         di->sums_attr_set = true;
     }
-    weight_sums_kernel<<<dim3((Skv + kTile - 1) / kTile, B * Hkv), 256, kSmemBytes, st>>>(p);
+    const int blocks = blocks_for(di->sm_count);
+    if (!(flags & CLLO_WS_COUNTERS_ZERO)) CLLO_CUDA_TRY(cudaMemsetAsync(workspace, 0, blocks * sizeof(unsigned), st));
+    weight_sums_kernel<<<blocks, kThreads, kSmemBytes, st>>>(tm_q, tm_k, p);
     CLLO_CUDA_TRY(cudaGetLastError());
     return CLLO_OK;
 }

@@ -146,16 +146,16 @@ _workspaces = {}
 _workspaces_lock = threading.Lock()
 
 
-def _decode_workspace(device, nbytes):
+def _workspace(kind, device, nbytes):
     """(scratch, flag): scratch whose arrival counters are zero, and the flag that vouches for it.
 
-    Eager calls share one tensor per (device, stream): calls on one stream do not overlap, and the kernel leaves the
+    Eager calls of one kind share one tensor per (device, stream): calls on one stream do not overlap, and the kernel leaves the
     counters zero.  A call that is being captured gets a tensor of its own from the graph's pool, and the call clears the
     counters at every replay: two graphs may be replayed at the same time.
     """
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device), 0
-    key = (device.index, _stream_ptr())
+    key = (kind, device.index, _stream_ptr())
     with _workspaces_lock:
         ws = _workspaces.get(key)
         if ws is None or ws.numel() < nbytes:
@@ -197,7 +197,7 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
         nbytes = _decode_workspace_bytes(device, B, cache.capacity, Hq, H, weights is not None, num_workers)
         flag = 0
         if workspace is None:
-            workspace, flag = _decode_workspace(device, nbytes)
+            workspace, flag = _workspace("decode", device, nbytes)
         rc = lib.cllo_kv8_decode_bf16(
             q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
             seq_lens.data_ptr(), scale, out.data_ptr(), None if lse is None else lse.data_ptr(),
@@ -224,7 +224,7 @@ def _decode_workspace_bytes(device, B, capacity, Hq, Hkv, with_weights, num_work
 
 
 def attention_weight_sums(q, k, lse, scale=None, causal=True, q_start=0, seq_lens=None, window=None, out=None,
-                          accumulate=False):
+                          accumulate=False, workspace=None):
     """How much weight a prompt's queries gave to every key: fp32 [B,Hkv,Skv].
 
     ``out[b,h,t] = sum over the group's heads g and the query rows i of exp(scale * q[b,g,i] . k[b,h,t] - lse[b,g,i])``
@@ -263,11 +263,16 @@ def attention_weight_sums(q, k, lse, scale=None, causal=True, q_start=0, seq_len
         _check_fp32("out", out, (B, H, Skv), device)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
+    lib = _lib.load()
     with torch.cuda.device(device):
-        rc = _lib.load().cllo_attn_weight_sums_bf16(
+        flags = _lib.SUMS_ACCUMULATE if accumulate else 0
+        if workspace is None:
+            workspace, zero = _workspace("sums", device, int(lib.cllo_attn_weight_sums_workspace_bytes()))
+            flags |= zero
+        rc = lib.cllo_attn_weight_sums_bf16(
             q.data_ptr(), k.data_ptr(), lse.data_ptr(), None if seq_lens is None else seq_lens.data_ptr(), scale,
-            1 if causal else 0, q_start, window or 0, 1 if accumulate else 0, out.data_ptr(), B, Sq, Skv, Hq, H, D,
-            _stream_ptr())
+            1 if causal else 0, q_start, window or 0, flags, out.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), B, Sq, Skv, Hq, H, D, _stream_ptr())
     _lib.check(rc, "cllo_attn_weight_sums_bf16")
     return out
 

@@ -344,15 +344,20 @@ int cllo_kv8_decode_bf16(const void* q, const void* k_cache, const void* v_cache
 /*
  * Weight sums of a prompt: sums[b,h,t] = sum over the heads g of the group and the counted query rows i of
  * e^(scale * q[b,g,i] . k[b,h,t] - lse[b,g,i]); with causal != 0 only t <= q_start + i.  q [B,Hq,Sq,D], k [B,Hkv,Skv,D]
- * bf16, lse [B,Hq,Sq] as the forward wrote it (rows with lse = -inf add nothing), sums fp32 [B,Hkv,Skv], added to when
- * accumulate != 0.
+ * bf16, lse [B,Hq,Sq] as the forward wrote it (rows with lse = -inf add nothing), sums fp32 [B,Hkv,Skv].
+ * flags: CLLO_SUMS_ACCUMULATE adds to sums instead of overwriting it; CLLO_WS_COUNTERS_ZERO as in cllo_gqa_decode_bf16.
+ * workspace: cllo_attn_weight_sums_workspace_bytes() bytes, 256-byte aligned, contents arbitrary: arrival counters and
+ * one partial sum per key and block where a key's queries are shared between blocks (added up in a fixed order, no
+ * atomics on values).  Calls that may overlap on the GPU need one each.
  * seq_lens (nullable) [B]: keys at t >= seq_lens[b] get 0, and with causal != 0 query rows at positions
  * q_start + i >= seq_lens[b] (the padding of a batch) do not count.  window > 0: only the last `window` query
  * positions before seq_lens[b] count -- the last rows of q where no lengths are given or the mask is not causal.
  */
+#define CLLO_SUMS_ACCUMULATE 1
+size_t cllo_attn_weight_sums_workspace_bytes(void);
 int cllo_attn_weight_sums_bf16(const void* q, const void* k, const float* lse, const int* seq_lens, float scale, int causal,
-                               int q_start, int window, int accumulate, float* sums, int B, int Sq, int Skv, int Hq,
-                               int Hkv, int D, void* stream);
+                               int q_start, int window, int flags, float* sums, void* workspace, size_t workspace_bytes,
+                               int B, int Sq, int Skv, int Hq, int Hkv, int D, void* stream);
 
 /*
  * Eviction by accumulated weight.  Per (batch, kv head) the cache's first `sink` and last `recent` tokens stay, and of the

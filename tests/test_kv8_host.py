@@ -89,10 +89,11 @@ def test_c_interface_refusals(built_library):
     assert lib.cllo_kv8_decode_workspace_bytes(1, 64, 3, 2, 128, 0, 0) == 0
     assert lib.cllo_kv8_decode_workspace_bytes(1, 64, 2, 2, 64, 0, 0) == 0
 
-    def sums(q=x, lse=x, scale=1.0, q_start=0, window=0, B=1, Sq=8, Skv=8, Hq=2, H=1, Dh=128):
-        return lib.cllo_attn_weight_sums_bf16(q, x, lse, None, scale, 1, q_start, window, 0, x, B, Sq, Skv, Hq, H, Dh, None)
+    def sums(q=x, lse=x, scale=1.0, q_start=0, window=0, flags=0, B=1, Sq=8, Skv=8, Hq=2, H=1, Dh=128):
+        return lib.cllo_attn_weight_sums_bf16(q, x, lse, None, scale, 1, q_start, window, flags, x, x, 1 << 30, B, Sq, Skv, Hq, H, Dh,
+                                              None)
     for bad in (dict(q=None), dict(q=x + 4), dict(lse=None), dict(scale=float("nan")), dict(q_start=-1), dict(window=-1),
-                dict(Sq=0), dict(Skv=0), dict(Hq=3, H=2)):
+                dict(flags=2), dict(Sq=0), dict(Skv=0), dict(Hq=3, H=2)):
         assert sums(**bad) == _lib.E_BAD_ARG, bad
     for bad in (dict(Dh=64), dict(Sq=(1 << 30) + 1)):
         assert sums(**bad) == _lib.E_UNSUPPORTED, bad
