@@ -97,6 +97,38 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// The same bounded wait for a warp that has nothing else to do and usually waits long (a producer, an MMA issuer beside
+// busy arithmetic warps): the look carries a time hint, so that the hardware puts the thread to sleep until the phase
+// completes or the hint runs out, instead of having it take issue slots from the warps beside it.
+__device__ __forceinline__ bool mbar_try_wait_for(uint32_t bar, uint32_t parity, uint32_t ns) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(ns)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ void mbar_wait_idle(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site,
+                                               int aux) {
+    constexpr uint32_t kHintNs = 20000;
+    if (mbar_try_wait_for(bar, parity, kHintNs)) return;
+    if (*abort_flag) return;
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (true) {
+        if (mbar_try_wait_for(bar, parity, kHintNs)) return;
+        if (*abort_flag) return;
+        if (clock64() - t0 > kWaitLimitCycles) {
+            *abort_flag = 1;
+            record_timeout(site, aux);
+            return;
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------
 // TMA (bulk tensor copy global -> shared, completion on an mbarrier).  One CTA, no cluster forms.
 // ---------------------------------------------------------------------------------------------

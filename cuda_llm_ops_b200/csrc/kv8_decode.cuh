@@ -321,7 +321,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     if (grp == 0 && lane == 0) {
                         const int rows = (p.G - gblk * kRows) < kRows ? (p.G - gblk * kRows) : kRows;
                         const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(kvh) * p.G + gblk * kRows;
-                        mbar_wait(q_empty_bar(q_slot), q_phase ^ 1u, abort_flag, SITE_KV8_Q_EMPTY, q_slot);
+                        mbar_wait_idle(q_empty_bar(q_slot), q_phase ^ 1u, abort_flag, SITE_KV8_Q_EMPTY, q_slot);
                         mbar_arrive_expect_tx(q_full_bar(q_slot), rows * kD * 2);
                         for (int r = 0; r < rows; ++r)
                             bulk_load(base + kSmemQ + q_slot * kQBytes + r * kQPitch, p.q + (head0 + r) * kD, kD * 2, q_full_bar(q_slot));
@@ -330,7 +330,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     const float* row = scales + (static_cast<long long>(b) * p.Hkv + kvh) * p.n_blocks;
 #pragma unroll 1
                     for (tile += (grp - turn + kGroups) % kGroups; tile < tile_end; tile += kGroups) {
-                        mbar_wait(empty_bar(slot), phase ^ 1u, abort_flag, SITE_KV8_EMPTY, slot);
+                        mbar_wait_idle(empty_bar(slot), phase ^ 1u, abort_flag, SITE_KV8_EMPTY, slot);
                         const int s0 = tile * kTok;
                         int blk = (s0 + quarter * 16) >> p.block_shift;
                         blk = blk < p.n_blocks ? blk : p.n_blocks - 1;  // a quarter behind the cache: any scale, nobody uses it
@@ -419,7 +419,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         // Q fragments: k-step (j, w) takes dims 16 (tig + 4 j) + 4 w + {0,1} and + {2,3}
         uint32_t qf[8][4];
         float mul0, mul1;  // |scale| * log2(e) * 2^-shift of the two rows
-        mbar_wait(q_full_bar(q_slot), q_phase, abort_flag, SITE_KV8_Q_FULL, q_slot);
+        mbar_wait_idle(q_full_bar(q_slot), q_phase, abort_flag, SITE_KV8_Q_FULL, q_slot);
         __syncwarp();
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -458,7 +458,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         const int n_here = tile_end - tile;
 #pragma unroll 1
         for (tile += (grp - turn + kGroups) % kGroups; tile < tile_end; tile += kGroups) {
-            mbar_wait(full_bar(slot), phase, abort_flag, SITE_KV8_FULL, slot);
+            mbar_wait_idle(full_bar(slot), phase, abort_flag, SITE_KV8_FULL, slot);
             __syncwarp();
             const uint32_t kb = base + slot * kStageBytes, vb = kb + kTileBytes;
             const int tok0 = tile * kTok + sub * kSubTok;

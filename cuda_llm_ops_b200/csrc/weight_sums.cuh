@@ -20,12 +20,15 @@
 // form per sequence.  A unit cut between blocks leaves one fp32 partial per key and block; the last block to arrive adds
 // them up in block order.
 //
-// Warps: 0-3 key tile 0, 4-7 key tile 1 (one key per thread), 8 TMA producer, 9 MMA issuer, 10 lse loader, 11 idle.
-// Tensor memory: two 128-column accumulators per key tile.  Shared memory: K 2 x 64 KB (the next unit's keys arrive during
-// this one's steps), Q 2 x 32 KB, lse 4 x 512 B.
+// Warps: 0-15 the exponentials, one key per thread -- warpgroups 0 and 2 key tile 0, 1 and 3 key tile 1, each 64 of a step's
+// queries: four warps per scheduler, so that one's tensor-memory load hides behind the others' exponentials -- 16 TMA
+// producer, 17 MMA issuer, 18 lse loader, 19 idle.
+// Tensor memory: two 128-column accumulators per key tile.  Shared memory: K 3 x 32 KB (the next unit's first keys arrive
+// during this one's steps), Q 3 x 32 KB (with two the copies' latency showed), lse 16 x 512 B (eight steps on their way).
 #pragma once
 
 #include "gqa_prefill.cuh"
+#include "kv8_decode.cuh"
 #include "kv8_format.cuh"
 
 namespace cllo {
@@ -34,21 +37,23 @@ namespace sums {
 constexpr int kD = 128;
 constexpr int kKeys = 128, kTiles = 2, kPair = kKeys * kTiles;  // keys per tile and unit
 constexpr int kQ = 128;                                          // queries per step
-constexpr int kThreads = 384;
+constexpr int kHalves = 2;                                       // warpgroups per key tile: 64 queries of a step each
+constexpr int kEpiWarps = kTiles * kHalves * 4;
+constexpr int kThreads = (kEpiWarps + 4) * 32;
 constexpr int kUnitCost = 2;
 constexpr int kSlabBytes = 128 * 128;         // [128 rows][64 dims] bf16, one swizzled slab
 constexpr int kTileBytes = 2 * kSlabBytes;
-constexpr int kKStageBytes = kTiles * kTileBytes;
-constexpr int kKStages = 2, kQStages = 2, kLseStages = 4;
+constexpr int kKStages = 3, kQStages = 3, kLseStages = 16, kLseAhead = 8;
 constexpr int kSmemK = 0;
-constexpr int kSmemQ = kKStages * kKStageBytes;
+constexpr int kSmemQ = kKStages * kTileBytes;
 constexpr int kSmemLse = kSmemQ + kQStages * kTileBytes;
 constexpr int kSmemBar = kSmemLse + kLseStages * kQ * 4;
 constexpr int kNumBars = 2 * kKStages + 2 * kQStages + 2 * kLseStages + 4 * kTiles + 1;
-constexpr int kSmemMisc = kSmemBar + kNumBars * 8;
+constexpr int kSmemHalf = kSmemBar + kNumBars * 8;  // the second half's sum of every key
+constexpr int kSmemMisc = kSmemHalf + kPair * 4;
 constexpr int kSmemBytes = kSmemMisc + 32 + 1024;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kEpiThreads = kTiles * 128;
+constexpr int kEpiThreads = kEpiWarps * 32;
 
 enum : int {
     SITE_SUMS_K = 90, SITE_SUMS_Q = 91, SITE_SUMS_LSE = 92, SITE_SUMS_D = 93, SITE_SUMS_DRAIN = 94,
@@ -160,6 +165,8 @@ struct Walk {
         const int own = prm.causal ? p * kPair - prm.q_start : 0;
         return (own > seq.i_lo ? own : seq.i_lo) + j * kQ;
     }
+    // key tiles of the unit that hold keys: a second one without any is not loaded
+    __device__ __forceinline__ int key_tiles() const { return p * kPair + kKeys < seq.len ? 2 : 1; }
     // whether key tile t of the unit has anything to do with the query tile at row i0
     __device__ __forceinline__ bool sees(const Params& prm, int t, int i0) const {
         const int key0 = p * kPair + t * kKeys;
@@ -254,18 +261,18 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         }
         for (int s = 0; s < kLseStages; ++s) {
             mbar_init(lse_full(s), 32);
-            mbar_init(lse_empty(s), kEpiThreads / 32);
+            mbar_init(lse_empty(s), kEpiWarps);
         }
         for (int t = 0; t < sums::kTiles; ++t)
             for (int s = 0; s < 2; ++s) {
                 mbar_init(d_full(t, s), 1);
-                mbar_init(d_empty(t, s), 4);
+                mbar_init(d_empty(t, s), 4 * kHalves);
             }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 9) {
+    if (warp == kEpiWarps + 1) {
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
     }
@@ -275,30 +282,17 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    if (warp == 8) {
-        // ------------------------------- TMA producer -------------------------------
+    if (warp == kEpiWarps) {
+        // ------------------------------- Q producer -------------------------------
         if (lane == 0) {
             tma_prefetch_desc(&tm_q);
-            tma_prefetch_desc(&tm_k);
-            int ks = 0, qs = 0, n_k = 0, n_q = 0;
-            uint32_t kp = 0, qp = 0;
+            int qs = 0;
+            uint32_t qp = 0;
             for (; !w.done(); w.next(p)) {
                 if (!w.active()) continue;
-                mbar_wait(k_empty(ks), kp ^ 1u, abort_flag, SITE_SUMS_K, ks);
-                const int n_tiles = w.p * kPair + kKeys < w.seq.len ? 2 : 1;  // a second tile without keys is not loaded
-                mbar_arrive_expect_tx(k_full(ks), n_tiles * sums::kTileBytes);
-                for (int t = 0; t < n_tiles; ++t)
-                    for (int d = 0; d < 2; ++d)
-                        tma_load_4d(base + sums::kSmemK + ks * kKStageBytes + t * sums::kTileBytes + d * kSlabBytes, &tm_k, k_full(ks),
-                                    d * 64, w.p * kPair + t * kKeys, w.kvh, w.b);
-                if (++ks == kKStages) {
-                    ks = 0;
-                    kp ^= 1u;
-                }
-                ++n_k;
                 int g = w.s_lo / w.n, j = w.s_lo - g * w.n;
                 for (int s = w.s_lo; s < w.s_hi; ++s) {
-                    mbar_wait(q_empty(qs), qp ^ 1u, abort_flag, SITE_SUMS_Q, qs);
+                    mbar_wait_idle(q_empty(qs), qp ^ 1u, abort_flag, SITE_SUMS_Q, qs);
                     mbar_arrive_expect_tx(q_full(qs), sums::kTileBytes);
                     for (int d = 0; d < 2; ++d)
                         tma_load_4d(base + sums::kSmemQ + qs * sums::kTileBytes + d * kSlabBytes, &tm_q, q_full(qs), d * 64,
@@ -307,7 +301,6 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                         qs = 0;
                         qp ^= 1u;
                     }
-                    ++n_q;
                     if (++j == w.n) {
                         j = 0;
                         ++g;
@@ -317,15 +310,39 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             if (*abort_flag) {
                 // a wait gave up somewhere: let the copies already issued land before the block retires
                 const long long t0 = clock64();
-                auto drain = [&](uint32_t bar, uint32_t parity) {
-                    while (!mbar_try_wait(bar, parity) && clock64() - t0 < kWaitLimitCycles / 64) {
+                for (int s = 0; s < kQStages; ++s)
+                    while (!mbar_try_wait(q_full(s), s < qs ? qp : qp ^ 1u) && clock64() - t0 < kWaitLimitCycles / 64) {
                     }
-                };
-                for (int s = 0; s < kKStages; ++s) drain(k_full(s), s < ks ? kp : kp ^ 1u);
-                for (int s = 0; s < kQStages; ++s) drain(q_full(s), s < qs ? qp : qp ^ 1u);
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == kEpiWarps + 3) {
+        // ------------- K producer: on its own, so that the next unit's keys are under way during this one's steps -------------
+        if (lane == 0) {
+            tma_prefetch_desc(&tm_k);
+            int ks = 0;
+            uint32_t kp = 0;
+            for (; !w.done(); w.next(p)) {
+                if (!w.active()) continue;
+                for (int t = 0; t < w.key_tiles(); ++t) {
+                    mbar_wait_idle(k_empty(ks), kp ^ 1u, abort_flag, SITE_SUMS_K, ks);
+                    mbar_arrive_expect_tx(k_full(ks), sums::kTileBytes);
+                    for (int d = 0; d < 2; ++d)
+                        tma_load_4d(base + sums::kSmemK + ks * sums::kTileBytes + d * kSlabBytes, &tm_k, k_full(ks), d * 64,
+                                    w.p * kPair + t * kKeys, w.kvh, w.b);
+                    if (++ks == kKStages) {
+                        ks = 0;
+                        kp ^= 1u;
+                    }
+                }
+            }
+            if (*abort_flag) {
+                const long long t0 = clock64();
+                for (int s = 0; s < kKStages; ++s)
+                    while (!mbar_try_wait(k_full(s), s < ks ? kp : kp ^ 1u) && clock64() - t0 < kWaitLimitCycles / 64) {
+                    }
+            }
+        }
+    } else if (warp == kEpiWarps + 1) {
         // -------------------------------- MMA issuer --------------------------------
         // the whole warp runs the loop and the leader lane's predicate guards the MMAs (see tc_mma_ss_lo_if)
         const uint32_t leader = lane == 0 ? 1u : 0u;
@@ -334,19 +351,30 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         uint32_t kp = 0, qp = 0, dp[sums::kTiles] = {0, 0};
         for (; !w.done(); w.next(p)) {
             if (!w.active()) continue;
-            if (lane == 0) mbar_wait(k_full(ks), kp, abort_flag, SITE_SUMS_K, ks);
+            int k_stage[sums::kTiles] = {0, 0};
+            const int n_tiles = w.key_tiles();
+#pragma unroll
+            for (int t = 0; t < sums::kTiles; ++t) {
+                if (t >= n_tiles) continue;
+                if (lane == 0) mbar_wait_idle(k_full(ks), kp, abort_flag, SITE_SUMS_K, ks);
+                k_stage[t] = ks;
+                if (++ks == kKStages) {
+                    ks = 0;
+                    kp ^= 1u;
+                }
+            }
             __syncwarp();
             int j = w.s_lo % w.n;
             for (int s = w.s_lo; s < w.s_hi; ++s) {
-                if (lane == 0) mbar_wait(q_full(qs), qp, abort_flag, SITE_SUMS_Q, qs);
+                if (lane == 0) mbar_wait_idle(q_full(qs), qp, abort_flag, SITE_SUMS_Q, qs);
                 const int i0 = w.row0(p, j);
 #pragma unroll
                 for (int t = 0; t < sums::kTiles; ++t) {
                     if (!w.sees(p, t, i0)) continue;
-                    if (lane == 0) mbar_wait(d_empty(t, ds[t]), dp[t] ^ 1u, abort_flag, SITE_SUMS_D, t);
+                    if (lane == 0) mbar_wait_idle(d_empty(t, ds[t]), dp[t] ^ 1u, abort_flag, SITE_SUMS_D, t);
                     __syncwarp();
                     tc_fence_after();
-                    const uint32_t a = smem_desc_lo(base + sums::kSmemK + ks * kKStageBytes + t * sums::kTileBytes, 16);
+                    const uint32_t a = smem_desc_lo(base + sums::kSmemK + k_stage[t] * sums::kTileBytes, 16);
                     const uint32_t bq = smem_desc_lo(base + sums::kSmemQ + qs * sums::kTileBytes, 16);
                     const uint32_t d = tmem_base + (t * 2 + ds[t]) * kQ;
                     tc_mma_ss_lo_if<false>(leader, d, a, bq, hi, kIdescQK);
@@ -365,17 +393,13 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 }
                 if (++j == w.n) j = 0;
             }
-            tc_commit_if(leader, k_empty(ks));
-            if (++ks == kKStages) {
-                ks = 0;
-                kp ^= 1u;
-            }
+            for (int t = 0; t < n_tiles; ++t) tc_commit_if(leader, k_empty(k_stage[t]));
         }
         __syncwarp();
         if (lane == 0) {
             // everything issued must have retired before tensor memory is released
             tc_commit(drain_bar);
-            mbar_wait(drain_bar, 0, abort_flag, SITE_SUMS_DRAIN, 0);
+            mbar_wait_idle(drain_bar, 0, abort_flag, SITE_SUMS_DRAIN, 0);
             if (*abort_flag) {
                 const long long t0 = clock64();
                 while (!mbar_try_wait(drain_bar, 0) && clock64() - t0 < kWaitLimitCycles / 64) {
@@ -383,31 +407,38 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             }
         }
         __syncwarp();
-    } else if (warp == 10) {
+    } else if (warp == kEpiWarps + 2) {
         // -------------------------------- lse loader --------------------------------
-        // -lse * log2(e) of the step's 128 queries; -inf (no contribution) for rows that saw no key
-        int ls = 0;
-        uint32_t lp = 0;
+        // Copies the steps' lse values (four per lane) eight steps ahead, and turns each lane's own four into
+        // -lse * log2(e) once they have landed; -inf (no contribution) for rows that saw no key.  Values behind the last
+        // counted row are never looked at.
+        int put = 0, got = 0;  // steps issued, steps handed over
+        auto hand_over = [&]() {
+            const int slot = got % kLseStages;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float* x = lse_buf + slot * kQ + e * 32 + lane;
+                *x = *x == -INFINITY ? -INFINITY : -*x * sums::kLog2e;
+            }
+            mbar_arrive(lse_full(slot));
+            ++got;
+        };
         for (; !w.done(); w.next(p)) {
             if (!w.active()) continue;
             int g = w.s_lo / w.n, j = w.s_lo - g * w.n;
             for (int s = w.s_lo; s < w.s_hi; ++s) {
-                const int i0 = w.row0(p, j);
+                const int i0 = w.row0(p, j), slot = put % kLseStages;
                 const float* src = p.lse + (static_cast<long long>(w.b) * p.Hq + w.kvh * p.G + g) * p.Sq;
-                float x[4];
+                mbar_wait_idle(lse_empty(slot), (static_cast<uint32_t>(put / kLseStages) & 1u) ^ 1u, abort_flag, SITE_SUMS_LSE, slot);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = i0 + e * 32 + lane;
-                    x[e] = i < w.seq.i_hi ? __ldg(src + i) : -INFINITY;
-                    x[e] = x[e] == -INFINITY ? -INFINITY : -x[e] * sums::kLog2e;
+                    kv8::cp_async_4(smem_u32(lse_buf + slot * kQ + e * 32 + lane), src + (i < w.seq.i_hi ? i : i0));
                 }
-                mbar_wait(lse_empty(ls), lp ^ 1u, abort_flag, SITE_SUMS_LSE, ls);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) lse_buf[ls * kQ + e * 32 + lane] = x[e];
-                mbar_arrive(lse_full(ls));
-                if (++ls == kLseStages) {
-                    ls = 0;
-                    lp ^= 1u;
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (++put > kLseAhead) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kLseAhead) : "memory");
+                    hand_over();
                 }
                 if (++j == w.n) {
                     j = 0;
@@ -415,10 +446,13 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 }
             }
         }
-    } else if (warp < 8) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        while (got < put) hand_over();
+    } else if (warp < kEpiWarps) {
         // ------------------------- exponentials and sums (one key per thread) -------------------------
-        const int t = warp >> 2;
-        const int key_in_pair = threadIdx.x;  // 0..255
+        const int t = (warp >> 2) & 1, half = warp >> 3;
+        const int key_in_pair = threadIdx.x & (kPair - 1);
+        float* other = reinterpret_cast<float*>(gen_base + sums::kSmemHalf);
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         int ls = 0, dsl = 0;
         uint32_t lp = 0, dph = 0;
@@ -427,54 +461,68 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             float* out = p.out + (static_cast<long long>(w.b) * p.Hkv + w.kvh) * p.Skv + key;
             if (!w.active()) {
                 // a unit without steps: whoever holds its first cell clears its sums
-                if (w.steps == 0 && w.unit_lo >= w.lo && key < p.Skv && !p.accumulate) *out = 0.f;
+                if (half == 0 && w.steps == 0 && w.unit_lo >= w.lo && key < p.Skv && !p.accumulate) *out = 0.f;
                 continue;
             }
             float total = 0.f;
+            // In the unit's own terms: query tile j starts at row r0 + 128 j, and the key tile sees tiles j >= j_sees (none if
+            // it holds no keys).
+            const int key0 = w.p * kPair + t * kKeys, r0 = w.row0(p, 0);
+            const int ahead = p.causal ? key0 - p.q_start - r0 : 0;  // rows between r0 and the key tile's own first query
+            const int j_sees = key0 >= w.seq.len ? 0x7fffffff : (ahead > 0 ? ahead / kQ : 0);
+            const int rows = w.seq.i_hi - r0;
+            // the first column of tile 0 that this key sees; without a causal mask every one, for all keys of a warp alike
+            const int own = p.causal ? ahead + static_cast<int>(threadIdx.x & (kKeys - 1)) : lane - 31;
+            const float scale = p.scale_log2;
+            const float* lse_half = lse_buf + half * (kQ / kHalves);
+            const uint32_t acc = tmem_base + lane_base + t * 2 * kQ + half * (kQ / kHalves);
             int j = w.s_lo % w.n;
-            for (int s = w.s_lo; s < w.s_hi; ++s) {
-                const int i0 = w.row0(p, j);
-                if (++j == w.n) j = 0;
-                mbar_wait(lse_full(ls), lp, abort_flag, SITE_SUMS_LSE, ls);
-                if (w.sees(p, t, i0)) {
-                    mbar_wait(d_full(t, dsl), dph, abort_flag, SITE_SUMS_D, t);
+#pragma unroll 1
+            for (int left = w.s_hi - w.s_lo; left > 0; --left) {
+                mbar_wait_idle(lse_full(ls), lp, abort_flag, SITE_SUMS_LSE, ls);
+                if (j >= j_sees) {
+                    mbar_wait_idle(d_full(t, dsl), dph, abort_flag, SITE_SUMS_D, t);
                     __syncwarp();
                     tc_fence_after();
-                    const int n_cols = w.seq.i_hi - i0 < kQ ? w.seq.i_hi - i0 : kQ;
-                    const int key0 = w.p * kPair + t * kKeys;
-                    // columns [c_lo, n_cols) of this key's row count
-                    const int c_lo = p.causal ? key - p.q_start - i0 : 0;
-                    const bool need_mask = n_cols < kQ || (p.causal && p.q_start + i0 < key0 + kKeys - 1);
-                    const uint64_t c2 = pk2(p.scale_log2, p.scale_log2);
-                    uint64_t sum2 = pk2(0.f, 0.f), sum3 = sum2;
+                    const float* nl = lse_half + ls * kQ;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    // columns of this warpgroup's share that count: from the warp's keys' own first ones up to i_hi
+                    const int lo = own - j * kQ - half * (kQ / kHalves), hi = rows - j * kQ - half * (kQ / kHalves);
+                    const int lo_first = lo - lane, lo_last = lo_first + 31;  // of the warp's lowest and highest key
+                    auto add_chunk = [&](const float (&x)[32], const float* l) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 l4 = *reinterpret_cast<const float4*>(l + e);
+                            sum[0] += fast_exp2(fmaf(x[e], scale, l4.x));
+                            sum[1] += fast_exp2(fmaf(x[e + 1], scale, l4.y));
+                            sum[2] += fast_exp2(fmaf(x[e + 2], scale, l4.z));
+                            sum[3] += fast_exp2(fmaf(x[e + 3], scale, l4.w));
+                        }
+                    };
+                    if (lo_last <= 0 && hi >= kQ / kHalves) {
+#pragma unroll
+                        for (int c = 0; c < kQ / kHalves; c += 32) {
+                            float x[32];
+                            tmem_ld32_wait(acc + dsl * kQ + c, x);
+                            add_chunk(x, nl + c);
+                        }
+                    } else {
 #pragma unroll 1
-                    for (int c = 0; c < n_cols; c += 32) {
-                        float x[32];
-                        tmem_ld32_wait(tmem_base + lane_base + (t * 2 + dsl) * kQ + c, x);
-                        const float4* nl = reinterpret_cast<const float4*>(lse_buf + ls * kQ + c);
-                        if (need_mask) {
-#pragma unroll
-                            for (int e = 0; e < 32; e += 4) {
-                                const float4 l4 = nl[e >> 2];
-                                const float l[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-                                for (int f = 0; f < 4; ++f) {
-                                    const int col = c + e + f;
-                                    x[e + f] = col >= c_lo && col < n_cols && l[f] != -INFINITY
-                                                   ? fast_exp2(fmaf(x[e + f], p.scale_log2, l[f])) : 0.f;
-                                }
-                                sum2 = add2(sum2, pk2(x[e], x[e + 1]));
-                                sum3 = add2(sum3, pk2(x[e + 2], x[e + 3]));
+                        for (int c = 0; c < kQ / kHalves; c += 32) {
+                            if (c >= hi || lo_first >= c + 32) continue;  // nothing for any key of the warp
+                            float x[32];
+                            tmem_ld32_wait(acc + dsl * kQ + c, x);
+                            if (lo_last <= c && hi >= c + 32) {
+                                add_chunk(x, nl + c);
+                                continue;
                             }
-                        } else {
+                            // bit e: the chunk's column e counts for this key.  What does not count may be anything, NaN too
+                            const uint32_t seen = (lo <= c ? 0xffffffffu : lo < c + 32 ? 0xffffffffu << (lo - c) : 0u) &
+                                                  (hi >= c + 32 ? 0xffffffffu : (1u << (hi - c)) - 1u);
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) {
-                                const float4 l4 = nl[e >> 2];
-                                float y0, y1, y2, y3;
-                                upk2(fma2(pk2(x[e], x[e + 1]), c2, pk2(l4.x, l4.y)), y0, y1);
-                                upk2(fma2(pk2(x[e + 2], x[e + 3]), c2, pk2(l4.z, l4.w)), y2, y3);
-                                sum2 = add2(sum2, pk2(fast_exp2(y0), fast_exp2(y1)));
-                                sum3 = add2(sum3, pk2(fast_exp2(y2), fast_exp2(y3)));
+                            for (int e = 0; e < 32; ++e) {
+                                const float y = fmaf(x[e], scale, nl[c + e]);
+                                sum[e & 3] += fast_exp2(seen >> e & 1u ? y : -INFINITY);
                             }
                         }
                     }
@@ -482,9 +530,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                     __syncwarp();
                     if (lane == 0) mbar_arrive(d_empty(t, dsl));
                     if ((dsl ^= 1) == 0) dph ^= 1u;
-                    float a0, a1;
-                    upk2(add2(sum2, sum3), a0, a1);
-                    total += a0 + a1;
+                    total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(lse_empty(ls));
@@ -492,14 +538,20 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                     ls = 0;
                     lp ^= 1u;
                 }
+                if (++j == w.n) j = 0;
             }
             if (key >= w.seq.len) total = 0.f;  // whatever lies behind the sequence
+            // the two halves of a key meet; the barrier also keeps the next unit's value out until this one has been read
+            if (half == 1) other[key_in_pair] = total;
+            named_bar_sync(1, kEpiThreads);
+            if (half == 0) total += other[key_in_pair];
+            named_bar_sync(1, kEpiThreads);
             if (w.s_lo == 0 && w.s_hi == w.steps) {
-                if (key < p.Skv) *out = p.accumulate ? *out + total : total;
+                if (half == 0 && key < p.Skv) *out = p.accumulate ? *out + total : total;
                 continue;
             }
             // this block's part of the unit goes to the workspace; the last block to arrive adds the parts up
-            p.slots[(static_cast<long long>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * kPair + key_in_pair] = total;
+            if (half == 0) p.slots[(static_cast<long long>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * kPair + key_in_pair] = total;
             const long long w_first = worker_of_tile(w.unit_lo + kUnitCost, w.T, w.W);
             const long long w_last = worker_of_tile(w.unit_lo + kUnitCost + w.steps - 1, w.T, w.W);
             const int n_pieces = static_cast<int>(w_last - w_first) + 1;
@@ -513,7 +565,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 *misc = last ? 1 : 0;
             }
             named_bar_sync(1, kEpiThreads);
-            if (*misc != 0) {
+            if (*misc != 0 && half == 0) {
                 const int which_first = worker_lo(w_first, w.T, w.W) >= w.unit_lo ? 0 : 1;
                 float sum = 0.f;
                 for (int i = 0; i < n_pieces; ++i)
@@ -525,7 +577,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     }
 
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kEpiWarps + 1) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
     }
