@@ -40,6 +40,7 @@ struct DeviceInfo {
     std::atomic<bool> mla_attr_set{false};
     std::atomic<bool> one_tile_attr_set{false};
     std::atomic<bool> sums_attr_set{false};
+    std::atomic<bool> kv8_select_attr_set{false};
     std::atomic<bool> kv8_decode_attr_set[4]{};  // one per format and with / without scores
     void* legacy_ws = nullptr;  // scratch cached by the source-compatibility wrapper only
     size_t legacy_ws_bytes = 0;

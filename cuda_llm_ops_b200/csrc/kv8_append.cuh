@@ -27,83 +27,108 @@ struct AppendParams {
     RowStrides stride;
     const int* seq_lens;
     const int* new_lens;  // nullable
-    int T, capacity, Hkv, n_blocks, blocks_touched;
+    int T, capacity, Hkv, n_blocks, blocks_touched, per_cta;
 };
+
+// a block of 128 tokens is two registers' worth of rows too many to hold twice
+template <int kBlock>
+constexpr bool kPrefetch = true;
 
 template <int kFmt, int kBlock>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
-    __shared__ float warp_amax[kAppendThreads / 32];
-    long long id = blockIdx.x;
+    __shared__ float warp_amax[2][kAppendThreads / 32];
     const int which = blockIdx.y;
-    const int j = static_cast<int>(id % p.blocks_touched);
-    id /= p.blocks_touched;
-    const int h = static_cast<int>(id % p.Hkv), b = static_cast<int>(id / p.Hkv);
-    const int held = clamp_len(p.seq_lens[b], p.capacity);
-    int n = p.new_lens ? clamp_len(p.new_lens[b], p.T) : p.T;
+    const int ctas = (p.blocks_touched + p.per_cta - 1) / p.per_cta;  // of a (batch, kv head)
+    // kv heads next to each other: with tokens before heads in memory they share DRAM pages
+    const int h = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
+    const int b = at / ctas, first = (at % ctas) * p.per_cta, row = b * p.Hkv + h;
+    const int held = clamp_len(__ldg(p.seq_lens + b), p.capacity);
+    int n = p.new_lens ? clamp_len(__ldg(p.new_lens + b), p.T) : p.T;
     if (n > p.capacity - held) n = p.capacity - held;
-    const int blk = held / kBlock + j;
-    const int row0 = blk * kBlock;  // first position of the cache block
-    if (n <= 0 || row0 >= held + n) return;
+    if (n <= 0) return;
+    const int end = held + n;
+    int blk = held / kBlock + first;
+    const int blk_end = first + p.per_cta < p.blocks_touched ? blk + p.per_cta : blk + p.blocks_touched - first;
 
     const int r_in = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
+    const long long src_token = p.src_stride[which].token;
     const __nv_bfloat16* src = p.src[which] + b * p.src_stride[which].batch + h * p.src_stride[which].head + c8;
     uint8_t* dst = p.cache[which] + b * p.stride.batch + h * p.stride.head + c8;
-    float* scale = p.scale[which] + (static_cast<long long>(b) * p.Hkv + h) * p.n_blocks + blk;
+    float* scales = p.scale[which] + static_cast<long long>(row) * p.n_blocks;
 
     constexpr int kPasses = kBlock / kRowsPerPass;
-    uint4 x[kPasses];
-    float amax = 0.f;
+    // the next block's rows are on their way while this one's are turned into codes
+    uint4 next[kPasses];
+    auto fetch = [&](int at) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        const int pos = row0 + i * kRowsPerPass + r_in;
-        x[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (pos >= held && pos < held + n)
-            x[i] = __ldg(reinterpret_cast<const uint4*>(src + (pos - held) * p.src_stride[which].token));
-    }
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            amax = fmaxf(amax, fmaxf(finite_abs(bf16_lo(w[e])), finite_abs(bf16_hi(w[e]))));
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if ((threadIdx.x & 31) == 0) warp_amax[threadIdx.x >> 5] = amax;
-    const bool has_old = row0 < held;
-    const float old_scale = has_old ? *scale : 0.f;
-    __syncthreads();  // also: every thread has read the old scale before one of them writes the new one
-#pragma unroll
-    for (int i = 0; i < kAppendThreads / 32; ++i) amax = fmaxf(amax, warp_amax[i]);
-    const int e_new = scale_exp<kFmt>(amax);
-    float s = exp2_int(e_new), inv = exp2_int(-e_new);
-    if (has_old && old_scale >= s) {
-        s = old_scale;
-        inv = 1.f / old_scale;
-    }
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        const int pos = row0 + i * kRowsPerPass + r_in;
-        uint2* at = reinterpret_cast<uint2*>(dst + pos * p.stride.token);
-        if (pos >= held && pos < held + n) {
-            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            uint2 c;
-            c.x = encode4<kFmt>(bf16_lo(w[0]) * inv, bf16_hi(w[0]) * inv, bf16_lo(w[1]) * inv, bf16_hi(w[1]) * inv);
-            c.y = encode4<kFmt>(bf16_lo(w[2]) * inv, bf16_hi(w[2]) * inv, bf16_lo(w[3]) * inv, bf16_hi(w[3]) * inv);
-            *at = c;
-        } else if (has_old && pos < held && s != old_scale) {
-            const uint2 c = *at;
-            const float ratio = old_scale * inv;
-            float v[8];
-            decode4<kFmt>(c.x, *reinterpret_cast<float(*)[4]>(v));
-            decode4<kFmt>(c.y, *reinterpret_cast<float(*)[4]>(v + 4));
-            uint2 d;
-            d.x = encode4<kFmt>(v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio);
-            d.y = encode4<kFmt>(v[4] * ratio, v[5] * ratio, v[6] * ratio, v[7] * ratio);
-            *at = d;
+        for (int i = 0; i < kPasses; ++i) {
+            const int pos = at * kBlock + i * kRowsPerPass + r_in;
+            next[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (pos >= held && pos < end) next[i] = __ldg(reinterpret_cast<const uint4*>(src + (pos - held) * src_token));
         }
+    };
+    if (blk * kBlock < end) fetch(blk);
+#pragma unroll 1
+    for (; blk < blk_end && blk * kBlock < end; ++blk) {
+        const int row0 = blk * kBlock, buf = blk & 1;
+        uint4 x[kPasses];
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) x[i] = next[i];
+        const bool has_old = row0 < held;
+        const float old_scale = has_old ? scales[blk] : 0.f;
+        if (kPrefetch<kBlock> && blk + 1 < blk_end && row0 + kBlock < end) fetch(blk + 1);
+        // the largest magnitude of the new rows, as bf16 bits; infinities and NaN, which do not take part, lie above all numbers
+        uint32_t top = 0u;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i)
+            top = max_u16x2(max_u16x2(top, max_u16x2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu)),
+                            max_u16x2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
+        float amax = fmaxf(finite_abs(bf16_lo(top)), finite_abs(bf16_hi(top)));
+        if ((top & 0x7fffu) >= 0x7f80u || (top >> 16) >= 0x7f80u) {
+            amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fmaxf(finite_abs(bf16_lo(w[e])), finite_abs(bf16_hi(w[e]))));
+            }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if ((threadIdx.x & 31) == 0) warp_amax[buf][threadIdx.x >> 5] = amax;
+        __syncthreads();  // also: every thread has read the old scale before one of them writes the new one
+#pragma unroll
+        for (int i = 0; i < kAppendThreads / 32; ++i) amax = fmaxf(amax, warp_amax[buf][i]);
+        const int e_new = scale_exp<kFmt>(amax);
+        float s = exp2_int(e_new), inv = exp2_int(-e_new);
+        if (has_old && old_scale >= s) {
+            s = old_scale;
+            inv = 1.f / old_scale;
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int pos = row0 + i * kRowsPerPass + r_in;
+            uint2* at = reinterpret_cast<uint2*>(dst + pos * p.stride.token);
+            if (pos >= held && pos < end) {
+                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                uint2 c;
+                c.x = encode4<kFmt>(bf16_lo(w[0]) * inv, bf16_hi(w[0]) * inv, bf16_lo(w[1]) * inv, bf16_hi(w[1]) * inv);
+                c.y = encode4<kFmt>(bf16_lo(w[2]) * inv, bf16_hi(w[2]) * inv, bf16_lo(w[3]) * inv, bf16_hi(w[3]) * inv);
+                *at = c;
+            } else if (has_old && pos < held && s != old_scale) {
+                const uint2 c = *at;
+                const float ratio = old_scale * inv;
+                float v[8];
+                decode4<kFmt>(c.x, *reinterpret_cast<float(*)[4]>(v));
+                decode4<kFmt>(c.y, *reinterpret_cast<float(*)[4]>(v + 4));
+                uint2 d;
+                d.x = encode4<kFmt>(v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio);
+                d.y = encode4<kFmt>(v[4] * ratio, v[5] * ratio, v[6] * ratio, v[7] * ratio);
+                *at = d;
+            }
+        }
+        if (threadIdx.x == 0) scales[blk] = s;
     }
-    if (threadIdx.x == 0) *scale = s;
 }
 
 template <int kFmt>
@@ -154,7 +179,10 @@ static int append_launch(const void* k_new, const long long* k_strides, const vo
     // T tokens starting anywhere inside a block reach this many blocks at most
     const int touched = (T - 1 + block - 1) / block + 1;
     p.blocks_touched = touched < p.n_blocks ? touched : p.n_blocks;
-    const long long blocks = static_cast<long long>(B) * Hkv * p.blocks_touched;
+    // cache blocks per thread block: several where there are enough to fill the GPU all the same
+    const long long per_cta = static_cast<long long>(B) * Hkv * p.blocks_touched * 2 / (static_cast<long long>(di->sm_count) * 16);
+    p.per_cta = static_cast<int>(per_cta < 1 ? 1 : (per_cta > 8 ? 8 : per_cta));
+    const long long blocks = static_cast<long long>(B) * Hkv * ((p.blocks_touched + p.per_cta - 1) / p.per_cta);
     if (blocks > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(blocks), 2);
     if (format == CLLO_FMT_E4M3)

@@ -4,9 +4,9 @@
 // between them the budget - sink - recent with the largest weight (of equal weights the one that comes first; a NaN counts as
 // larger than any number).  What stays keeps its order and moves to another cache; a row within its budget moves whole.
 //
-// select_kernel finds the threshold weight by radix selection (four passes of 8 bits over order-preserving integers) and
-// writes the kept positions in order; gather_kernel moves the rows: codes -> values (exact: a product with a power of
-// two) -> amax of the new block -> codes in the new scale.
+// select_kernel finds the threshold weight by radix selection (three passes over order-preserving integers) and writes the
+// kept positions in order; gather_kernel moves the rows: codes -> values (exact: a product with a power of two) -> amax of
+// the new block -> codes in the new scale.
 #pragma once
 
 #include "host_util.cuh"
@@ -37,165 +37,339 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 }
 
 constexpr int kSelectThreads = 1024;
+constexpr int kDigitBits = 11, kBins = 1 << kDigitBits;      // three passes: 11, 11 and 10 bits
+constexpr int kMaxCluster = 8;
+constexpr int kKeysInSmem = 48 * 1024;                         // of a block's chunk; what is longer is read again in each pass
+constexpr int kSelectUnroll = 8;
 
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(const EvictParams p) {
-    __shared__ int hist[256];
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a word of another block's shared memory, at the address it has in this block's
+__device__ __forceinline__ int cluster_load(const int* p, uint32_t rank) {
+    uint32_t remote;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void cluster_load2(const int* p, uint32_t rank, int& x, int& y) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(remote) : "memory");
+}
+
+// One cluster of blocks per (batch, kv head) row, each block a contiguous chunk of the row.  The chunk's weights are read
+// once and stay in shared memory as integers; a pass counts the digits of the keys that share the prefix found so far
+// (equal digits of a warp are added together first: weights cluster in few exponents, and ties share every digit), the
+// blocks add up each other's counts over distributed shared memory, and every block finds the same digit.  Bound by the
+// latency of its passes: 4 cluster barriers, 8 block barriers.
+__global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictParams p) {
+    extern __shared__ uint32_t keys[];
+    __shared__ __align__(8) int hist[2][kBins];
     __shared__ int warp_sum[kSelectThreads / 32];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_need, s_total;
+    __shared__ int s_digit, s_need;
+    __shared__ int s_counts[2];  // this block's tokens that stay whatever the others hold, and those at the threshold
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int h = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
+    const int C = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+    const int row = blockIdx.x / C;
+    const int h = row % p.Hkv, b = row / p.Hkv;
     const int len = clamp_len(p.seq_lens[b], p.capacity);
-    int* idx = p.indices + static_cast<long long>(blockIdx.x) * p.budget;
+    int* idx = p.indices + static_cast<long long>(row) * p.budget;
     const int kept = len < p.budget ? len : p.budget;
-    if (h == 0 && tid == 0) p.new_lens[b] = kept;
-    if (len <= p.budget) {
-        for (int j = tid; j < p.budget; j += kSelectThreads) idx[j] = j < len ? j : -1;
+    if (h == 0 && tid == 0 && rank == 0) p.new_lens[b] = kept;
+    for (int j = kept + rank * kSelectThreads + tid; j < p.budget; j += C * kSelectThreads) idx[j] = -1;
+    if (len <= p.budget) {  // the whole cluster alike
+        for (int j = rank * kSelectThreads + tid; j < len; j += C * kSelectThreads) idx[j] = j;
         return;
     }
-    const float* w = p.weights + static_cast<long long>(blockIdx.x) * p.capacity;
-    const int lo = p.sink, hi = len - p.recent;
-    if (tid == 0) {
-        s_prefix = 0u;
-        s_need = p.budget - p.sink - p.recent;  // how many of the keys that share the prefix are kept
-    }
-    // a row within a budget of forced tokens alone keeps nothing between them: the threshold is never looked at
-    uint32_t mask = 0u;
-    for (int shift = 24; shift >= 0 && p.budget > p.sink + p.recent; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
-        __syncthreads();
-        const uint32_t prefix = s_prefix;
-        for (int t = lo + tid; t < hi; t += kSelectThreads) {
-            const uint32_t key = order_key(w[t]);
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1);
+    const int chunk = (len + C - 1) / C;
+    const int t0 = chunk * rank < len ? chunk * rank : len;
+    const int n = t0 + chunk < len ? chunk : len - t0;
+    const float* w = p.weights + static_cast<long long>(row) * p.capacity + t0;
+    const int lo = p.sink - t0, hi = len - p.recent - t0;  // candidates [lo, hi) in the chunk's own terms
+    const int n_smem = n < kKeysInSmem ? n : kKeysInSmem;
+    for (int i0 = tid; i0 < n_smem; i0 += kSelectThreads * kSelectUnroll) {
+        float x[kSelectUnroll];
+#pragma unroll
+        for (int u = 0; u < kSelectUnroll; ++u) {
+            const int i = i0 + u * kSelectThreads;
+            x[u] = i < n_smem ? __ldg(w + i) : 0.f;
         }
-        __syncthreads();
-        if (tid == 0) {
-            int need = s_need, d = 255;
-            while (d > 0 && hist[d] < need) need -= hist[d--];
-            s_need = need;
-            s_prefix = prefix | (static_cast<uint32_t>(d) << shift);
+#pragma unroll
+        for (int u = 0; u < kSelectUnroll; ++u) {
+            const int i = i0 + u * kSelectThreads;
+            if (i < n_smem) keys[i] = order_key(x[u]);
         }
-        mask |= 255u << shift;
-        __syncthreads();
     }
-    __syncthreads();
-    const uint32_t thr = s_prefix;
-    const int quota = s_need;  // keys equal to the threshold that are kept, the first ones
+    auto key_at = [&](int i) { return i < n_smem ? keys[i] : order_key(__ldg(w + i)); };
+
     const bool any = p.budget > p.sink + p.recent;
-    int above_before = 0, equal_before = 0;
-    for (int t0 = 0; t0 < len; t0 += kSelectThreads) {
-        const int t = t0 + tid;
-        bool above = false, equal = false;
-        if (t < len) {
-            if (t < lo || t >= hi)
-                above = true;
-            else if (any) {
-                const uint32_t key = order_key(w[t]);
-                above = key > thr;
-                equal = key == thr;
+    uint32_t prefix = 0u, mask = 0u;
+    int need = p.budget - p.sink - p.recent;  // how many of the keys that share the prefix are kept
+    if (any) {
+        int buf = 0;
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t digits = pass == 2 ? 0x3ffu : 0x7ffu;
+            for (int i = tid; i < kBins; i += kSelectThreads) hist[buf][i] = 0;
+            __syncthreads();  // also: the keys are in place
+            const int steps = (n + kSelectThreads - 1) / kSelectThreads;
+#pragma unroll 4
+            for (int k = 0; k < steps; ++k) {
+                const int i = k * kSelectThreads + tid;
+                const uint32_t key = i < n && i >= lo && i < hi ? key_at(i) : 0u;
+                const bool in = i < n && i >= lo && i < hi && (key & mask) == prefix;
+                const unsigned active = __ballot_sync(0xffffffffu, in);
+                if (active == 0u) continue;
+                const int first = __ffs(active) - 1;
+                const int d = static_cast<int>((key >> shift) & digits), d0 = __shfl_sync(0xffffffffu, d, first);
+                if (__all_sync(0xffffffffu, !in || d == d0)) {
+                    if (lane == first) atomicAdd(&hist[buf][d0], __popc(active));  // ties, or one exponent for all
+                } else if (in) {
+                    atomicAdd(&hist[buf][d], 1);
+                }
             }
-        }
-        const unsigned ba = __ballot_sync(0xffffffffu, above), be = __ballot_sync(0xffffffffu, equal);
-        if (lane == 0) warp_sum[warp] = __popc(ba) | (__popc(be) << 16);
-        __syncthreads();
-        if (warp == 0) {
-            const int mine = warp_sum[lane];
-            int v = mine;
+            cluster_sync();
+            // sum over the cluster, then the largest digit at which the count from the top reaches `need`: two bins a thread,
+            // highest first
+            int part[kMaxCluster][2], c[2] = {0, 0};
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {
+                part[r][0] = part[r][1] = 0;
+                if (r < C) cluster_load2(&hist[buf][kBins - 2 - 2 * tid], r, part[r][1], part[r][0]);
+            }
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {
+                c[0] += part[r][0];
+                c[1] += part[r][1];
+            }
+            int v = c[0] + c[1];
+            const int mine = v;
             for (int o = 1; o < 32; o <<= 1) {
                 const int u = __shfl_up_sync(0xffffffffu, v, o);
                 if (lane >= o) v += u;
             }
-            warp_sum[lane] = v - mine;
-            if (lane == 31) s_total = v;
+            if (lane == 31) warp_sum[warp] = v;
+            __syncthreads();
+            int others = lane < warp ? warp_sum[lane] : 0;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) others += __shfl_xor_sync(0xffffffffu, others, o);
+            int before = others + v - mine;  // keys in higher bins
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (before < need && need <= before + c[u]) {
+                    s_digit = kBins - 1 - (2 * tid + u);
+                    s_need = need - before;
+                }
+                before += c[u];
+            }
+            __syncthreads();
+            prefix |= static_cast<uint32_t>(s_digit) << shift;
+            mask |= digits << shift;
+            need = s_need;
+            buf ^= 1;  // the others may still be reading this pass's counts
         }
-        __syncthreads();
-        const unsigned below = (1u << lane) - 1u;
-        const int a = above_before + (warp_sum[warp] & 0xffff) + __popc(ba & below);
-        const int e = equal_before + (warp_sum[warp] >> 16) + __popc(be & below);
-        if (above || (equal && e < quota)) idx[a + (e < quota ? e : quota)] = t;
-        above_before += s_total & 0xffff;
-        equal_before += s_total >> 16;
-        __syncthreads();
     }
+
+    // positions in order: how many stay and how many sit at the threshold before each token
+    auto classify = [&](int i, bool& above, bool& equal) {
+        above = equal = false;
+        if (i >= n) return;
+        if (i < lo || i >= hi) {
+            above = true;
+        } else if (any) {
+            const uint32_t key = key_at(i);
+            above = key > prefix;
+            equal = key == prefix;
+        }
+    };
+    // a warp owns a contiguous stretch of the chunk, so that only the warps' totals have to meet
+    const int per_warp = ((n + kSelectThreads / 32 - 1) / (kSelectThreads / 32) + 31) / 32 * 32;
+    const int w_lo = warp * per_warp, w_hi = w_lo + per_warp < n ? w_lo + per_warp : n;
+    int n_above = 0, n_equal = 0;
+#pragma unroll 4
+    for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
+        bool above, equal;
+        classify(i0 + lane, above, equal);
+        n_above += __popc(__ballot_sync(0xffffffffu, above));
+        n_equal += __popc(__ballot_sync(0xffffffffu, equal));
+    }
+    int* totals = hist[0];  // two ints per warp; the last counts to be read were hist[0] of the third pass
+    cluster_sync();
+    if (lane == 0) {
+        totals[2 * warp] = n_above;
+        totals[2 * warp + 1] = n_equal;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int a = totals[2 * lane], e = totals[2 * lane + 1];
+        for (int o = 16; o; o >>= 1) {
+            a += __shfl_xor_sync(0xffffffffu, a, o);
+            e += __shfl_xor_sync(0xffffffffu, e, o);
+        }
+        if (lane == 0) {
+            s_counts[0] = a;
+            s_counts[1] = e;
+        }
+    }
+    cluster_sync();
+    int a_before = 0, e_before = 0;
+    for (int r = 0; r < rank; ++r) {
+        a_before += cluster_load(&s_counts[0], r);
+        e_before += cluster_load(&s_counts[1], r);
+    }
+    {
+        int a = lane < warp ? totals[2 * lane] : 0, e = lane < warp ? totals[2 * lane + 1] : 0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            a += __shfl_xor_sync(0xffffffffu, a, o);
+            e += __shfl_xor_sync(0xffffffffu, e, o);
+        }
+        a_before += a;
+        e_before += e;
+    }
+    const unsigned below = (1u << lane) - 1u;
+#pragma unroll 2
+    for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
+        bool above, equal;
+        classify(i0 + lane, above, equal);
+        const unsigned ba = __ballot_sync(0xffffffffu, above), be = __ballot_sync(0xffffffffu, equal);
+        const int a = a_before + __popc(ba & below), e = e_before + __popc(be & below);
+        // of the tokens at the threshold the first `need` stay
+        if (above || (equal && e < need)) idx[a + (e < need ? e : need)] = t0 + i0 + lane;
+        a_before += __popc(ba);
+        e_before += __popc(be);
+    }
+    cluster_sync();  // no block leaves while another may still read its counts
 }
 
-constexpr int kGatherThreads = 128;
+// eight lanes per row, two rows of K and of V per lane
+__host__ __device__ constexpr int gather_threads(int block) { return block * 4; }
 
+// One thread block per block of the second cache: K and V rows of its tokens, 16 bytes per lane and eight lanes per row, all
+// loads in flight before the first is looked at; values -> amax -> new scale -> codes.  Bound by memory: 2 x 128 bytes read
+// and written per token.
 template <int kFmt, int kBlock>
-__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const EvictParams p) {
-    __shared__ float warp_amax[kGatherThreads / 32];
-    const int which = blockIdx.y;
-    const int row = blockIdx.x / p.n_blocks_to, blk = blockIdx.x % p.n_blocks_to;
-    const int h = row % p.Hkv, b = row / p.Hkv;
+__global__ void __launch_bounds__(gather_threads(kBlock)) gather_kernel(const EvictParams p) {
+    constexpr int kThreads = gather_threads(kBlock);
+    __shared__ float warp_amax[2][kThreads / 32];
+    // kv heads next to each other: with tokens before heads in memory they share DRAM pages
+    const int h = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
+    const int b = at / p.n_blocks_to, blk = at % p.n_blocks_to, row = b * p.Hkv + h;
     const int len = clamp_len(p.seq_lens[b], p.capacity);
     const int kept = len < p.budget ? len : p.budget;
     const int j0 = blk * kBlock;
     if (j0 >= kept) return;
     const int* idx = p.indices + static_cast<long long>(row) * p.budget;
-    const uint8_t* from = p.from[which] + b * p.stride_from.batch + h * p.stride_from.head;
-    uint8_t* to = p.to[which] + b * p.stride_to.batch + h * p.stride_to.head;
-    const float* scale_from = p.scale_from[which] + static_cast<long long>(row) * p.n_blocks_from;
-    constexpr int kRows = kGatherThreads / 16, kPasses = kBlock / kRows;
-    const int r_in = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
-    uint2 c[kPasses];
-    float s[kPasses], amax = 0.f;
+    constexpr int kRowsPerStep = kThreads / 8, kSteps = kBlock / kRowsPerStep;
+    const int r_in = threadIdx.x >> 3, c16 = (threadIdx.x & 7) * 16;
+    int t[kSteps];
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        const int j = j0 + i * kRows + r_in;
-        c[i] = make_uint2(0u, 0u);
-        s[i] = 0.f;
-        if (j < kept) {
-            const int t = idx[j];
-            c[i] = __ldg(reinterpret_cast<const uint2*>(from + t * p.stride_from.token + c8));
-            s[i] = scale_from[t >> p.block_shift];
-            if (which == 0 && p.weights_to && (threadIdx.x & 15) == 0)
-                p.weights_to[static_cast<long long>(row) * p.capacity_to + j] =
-                    p.weights[static_cast<long long>(row) * p.capacity + t];
+    for (int i = 0; i < kSteps; ++i) {
+        const int j = j0 + i * kRowsPerStep + r_in;
+        t[i] = j < kept ? __ldcg(idx + j) : -1;
+    }
+    uint4 c[2][kSteps];
+    float s[2][kSteps];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        const uint8_t* from = p.from[which] + b * p.stride_from.batch + h * p.stride_from.head + c16;
+        const float* scale_from = p.scale_from[which] + static_cast<long long>(row) * p.n_blocks_from;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            c[which][i] = make_uint4(0u, 0u, 0u, 0u);
+            s[which][i] = 0.f;
+            if (t[i] >= 0) {
+                c[which][i] = __ldg(reinterpret_cast<const uint4*>(from + t[i] * p.stride_from.token));
+                s[which][i] = __ldg(scale_from + (t[i] >> p.block_shift));
+            }
         }
     }
-    auto values = [&](int i, float (&v)[8]) {
-        decode4<kFmt>(c[i].x, *reinterpret_cast<float(*)[4]>(v));
-        decode4<kFmt>(c[i].y, *reinterpret_cast<float(*)[4]>(v + 4));
+    if (p.weights_to && (threadIdx.x & 7) == 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= s[i];
-    };
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        float v[8];
-        values(i, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(v[e]));
+        for (int i = 0; i < kSteps; ++i)
+            if (t[i] >= 0)
+                p.weights_to[static_cast<long long>(row) * p.capacity_to + j0 + i * kRowsPerStep + r_in] =
+                    __ldg(p.weights + static_cast<long long>(row) * p.capacity + t[i]);
     }
+    // codes -> f16 pairs, which hold them exactly; the rows' largest magnitudes times their scales give the block's
+    uint32_t f[2][kSteps][8];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if ((threadIdx.x & 31) == 0) warp_amax[threadIdx.x >> 5] = amax;
+    for (int which = 0; which < 2; ++which) {
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const uint32_t w[4] = {c[which][i].x, c[which][i].y, c[which][i].z, c[which][i].w};
+            uint32_t top = 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                decode4_f16<kFmt>(w[k], f[which][i][2 * k], f[which][i][2 * k + 1]);
+                top = max_f16x2(top, max_f16x2(f[which][i][2 * k] & 0x7fff7fffu, f[which][i][2 * k + 1] & 0x7fff7fffu));
+            }
+            amax = fmaxf(amax, finite_abs(f16_max_of_pair(top) * s[which][i]));  // a NaN does not take part
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if ((threadIdx.x & 31) == 0) warp_amax[which][threadIdx.x >> 5] = amax;
+    }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kGatherThreads / 32; ++i) amax = fmaxf(amax, warp_amax[i]);
-    const int e_new = scale_exp<kFmt>(amax);
-    const float inv = exp2_int(-e_new);
+    for (int which = 0; which < 2; ++which) {
+        float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        const int j = j0 + i * kRows + r_in;
-        if (j >= kept) continue;
-        float v[8];
-        values(i, v);
-        uint2 d;
-        d.x = encode4<kFmt>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-        d.y = encode4<kFmt>(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-        *reinterpret_cast<uint2*>(to + j * p.stride_to.token + c8) = d;
+        for (int i = 0; i < kThreads / 32; ++i) amax = fmaxf(amax, warp_amax[which][i]);
+        const int e_new = scale_exp<kFmt>(amax);
+        const float inv = exp2_int(-e_new);
+        uint8_t* to = p.to[which] + b * p.stride_to.batch + h * p.stride_to.head + c16;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            if (t[i] < 0) continue;
+            uint32_t d[4];
+            // Scales are powers of two: the code times their ratio is exact in f16 where it can still round to a code other
+            // than zero, so one rounding, to the new code, is all there is.  A ratio beyond f16 (a block of nothing but
+            // codes at the very bottom of e4m3) or scales that are no powers of two go through fp32.
+            const float ratio = s[which][i] * inv;
+            if ((__float_as_uint(ratio) & 0x7fffffu) == 0u && fabsf(ratio) <= 32768.f) {
+                const uint32_t r = pack_f16x2(ratio, ratio);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) d[k] = requant4<kFmt>(f[which][i][2 * k], f[which][i][2 * k + 1], r);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float v[4];
+                    f16x2_to_f32(f[which][i][2 * k], v[0], v[1]);
+                    f16x2_to_f32(f[which][i][2 * k + 1], v[2], v[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = v[e] * s[which][i] * inv;
+                    d[k] = encode4<kFmt>(v[0], v[1], v[2], v[3]);
+                }
+            }
+            *reinterpret_cast<uint4*>(to + (j0 + i * kRowsPerStep + r_in) * p.stride_to.token) = make_uint4(d[0], d[1], d[2], d[3]);
+        }
+        if (threadIdx.x == 0) p.scale_to[which][static_cast<long long>(row) * p.n_blocks_to + blk] = exp2_int(e_new);
     }
-    if (threadIdx.x == 0) p.scale_to[which][static_cast<long long>(row) * p.n_blocks_to + blk] = exp2_int(e_new);
 }
 
 template <int kFmt>
-static void gather_dispatch(const EvictParams& p, int block, dim3 grid, cudaStream_t st) {
+static void gather_dispatch(const EvictParams& p, int block, unsigned grid, cudaStream_t st) {
     switch (block) {
-        case 16: gather_kernel<kFmt, 16><<<grid, kGatherThreads, 0, st>>>(p); break;
-        case 32: gather_kernel<kFmt, 32><<<grid, kGatherThreads, 0, st>>>(p); break;
-        case 64: gather_kernel<kFmt, 64><<<grid, kGatherThreads, 0, st>>>(p); break;
-        default: gather_kernel<kFmt, 128><<<grid, kGatherThreads, 0, st>>>(p); break;
+        case 16: gather_kernel<kFmt, 16><<<grid, gather_threads(16), 0, st>>>(p); break;
+        case 32: gather_kernel<kFmt, 32><<<grid, gather_threads(32), 0, st>>>(p); break;
+        case 64: gather_kernel<kFmt, 64><<<grid, gather_threads(64), 0, st>>>(p); break;
+        default: gather_kernel<kFmt, 128><<<grid, gather_threads(128), 0, st>>>(p); break;
     }
 }
 
@@ -260,9 +434,31 @@ static int evict_launch(const void* k, const void* v, const float* k_scale, cons
     p.block_shift = block_shift_of(block);
     const long long blocks = static_cast<long long>(rows) * p.n_blocks_to;
     if (blocks > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
-    select_kernel<<<static_cast<unsigned>(rows), kSelectThreads, 0, st>>>(p);
-    CLLO_CUDA_TRY(cudaGetLastError());
-    const dim3 grid(static_cast<unsigned>(blocks), 2);
+    // blocks per row: enough to fill the GPU, chunks of at least 2048 tokens
+    int cluster = 1;
+    while (cluster < kMaxCluster && rows * cluster * 2 <= static_cast<size_t>(di->sm_count) && capacity / (cluster * 2) >= 2048) cluster *= 2;
+    // rows longer than what one block holds in shared memory are shared out even on a full GPU
+    while (cluster < kMaxCluster && capacity / cluster > kKeysInSmem) cluster *= 2;
+    const int chunk = (capacity + cluster - 1) / cluster;
+    const int smem = (chunk < kKeysInSmem ? chunk : kKeysInSmem) * 4;
+    if (rows * cluster > 0x7fffffffULL) return CLLO_E_UNSUPPORTED;
+    if (!di->kv8_select_attr_set) {
+        CLLO_CUDA_TRY(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeysInSmem * 4));
+        di->kv8_select_attr_set = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster));
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    CLLO_CUDA_TRY(cudaLaunchKernelEx(&cfg, select_kernel, p));
+    const unsigned grid = static_cast<unsigned>(blocks);
     if (format == CLLO_FMT_E4M3)
         gather_dispatch<CLLO_FMT_E4M3>(p, block, grid, st);
     else

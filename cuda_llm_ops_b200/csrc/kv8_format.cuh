@@ -71,19 +71,69 @@ __device__ __forceinline__ void decode4_f16(uint32_t w, uint32_t& lo, uint32_t& 
     }
 }
 
+__device__ __forceinline__ void f16x2_to_f32(uint32_t h, float& lo, float& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+        : "=f"(lo), "=f"(hi)
+        : "r"(h));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// the larger of each half; of a number and a NaN the number
+__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float f16_max_of_pair(uint32_t h) {
+    float lo, hi;
+    f16x2_to_f32(h, lo, hi);
+    return fmaxf(lo, hi);
+}
+
 template <int kFmt>
 __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
     uint32_t h[2];
     decode4_f16<kFmt>(w, h[0], h[1]);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
-            : "=f"(x[2 * i]), "=f"(x[2 * i + 1])
-            : "r"(h[i]));
+    f16x2_to_f32(h[0], x[0], x[1]);
+    f16x2_to_f32(h[1], x[2], x[3]);
+}
+
+// two f16 pairs times the f16 pair r -> four codes (round to nearest even).  The products must not pass the largest code.
+template <int kFmt>
+__device__ __forceinline__ uint32_t requant4(uint32_t lo, uint32_t hi, uint32_t r) {
+    uint32_t d;
+    if (kFmt == CLLO_FMT_E4M3) {
+        asm("{\n\t.reg .b32 x, y;\n\t.reg .b16 a, b;\n\t"
+            "mul.rn.f16x2 x, %1, %3;\n\tmul.rn.f16x2 y, %2, %3;\n\t"
+            "cvt.rn.satfinite.e4m3x2.f16x2 a, x;\n\tcvt.rn.satfinite.e4m3x2.f16x2 b, y;\n\t"
+            "mov.b32 %0, {a, b};\n\t}"
+            : "=r"(d)
+            : "r"(lo), "r"(hi), "r"(r));
+    } else {
+        // x r + 1536 in f16, whose step there is 1: rounded to an integer, which the low byte holds
+        uint32_t x, y;
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(x) : "r"(lo), "r"(r), "r"(0x66006600u));
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(hi), "r"(r), "r"(0x66006600u));
+        d = __byte_perm(x, y, 0x6420);
+    }
+    return d;
 }
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// asynchronous copy of one thread, global -> shared
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 
 // element strides of a cache row (b, t, h) and its start
 struct RowStrides {
