@@ -53,7 +53,7 @@ constexpr int kConsumerWarps = kGroups * kWarpsPerGroup;
 // and scores of their tokens beside them; at the 168 registers that 384 threads get they would spill.  The pool is what
 // the block was launched with; asking for more in total would never return.
 constexpr int kDecodeThreads = (kConsumerWarps + 4) * 32;
-constexpr int kLaunchRegs = 168, kConsumerRegs = 232, kProducerRegs = 40;
+constexpr int kLaunchRegs = 168, kConsumerRegs = 224, kProducerRegs = 56;
 static_assert(2 * kConsumerRegs + kProducerRegs <= 3 * kLaunchRegs, "setmaxnreg budget exceeds the block's register pool");
 static_assert(kConsumerWarps == 8 && kDecodeThreads == 384, "the register budget is for three warpgroups");
 constexpr int kTileBytes = kTok * kD;           // K or V of one stage
@@ -77,6 +77,7 @@ static_assert(kDecodeSmemBytes <= 227 * 1024, "shared memory of a block");
 // What a unit costs beyond its tiles (its query rows, the merge of the eight states, the output), in tiles.  The shares of
 // the blocks are cut in these units, so that a block that gets many short sequences is not the last one to finish: 17
 // sequences of 0 to 16384 tokens, 8 kv heads: 81 us at 0, 61 at 4, 55 at 6, 49 at 12, 53 at 16; no effect on full batches.
+// Held to the tiles that a block gets on average: where there are fewer than that, spreading the tiles comes first.
 constexpr int kUnitCost = 10;
 constexpr float kLazy = 4.f;                 // a reference may lag behind the true maximum by this much (log2)
 constexpr float kPShift = 15.f - kLazy;      // p' <= 2^15
@@ -100,12 +101,19 @@ struct DecodeParams {
     int B, Hq, Hkv, G, n_gblk, capacity, n_blocks, block_shift, kv_layout;
 };
 
-using decode::worker_lo;
-using decode::worker_of_tile;
+// tiles of a sequence; an empty one has one, so that its output is written
+__device__ __forceinline__ int tiles_of(int len) { return len <= 0 ? 1 : (len + kTok - 1) / kTok; }
 
-// cells of a unit in the index space that the blocks share: kUnitCost without a tile, then one per tile; an empty
-// sequence has one tile, so that its output is written
-__device__ __forceinline__ int cells_of(int len) { return kUnitCost + (len <= 0 ? 1 : (len + kTok - 1) / kTok); }
+// a / b for non-negative values; most of them fit 32 bits, where a division costs a quarter
+__device__ __forceinline__ long long div_nonneg(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+// the cells [cell_lo(w), cell_lo(w + 1)) of block w, and the block that holds cell c
+__device__ __forceinline__ long long cell_lo(long long w, long long T, long long W) { return div_nonneg(w * T, W); }
+__device__ __forceinline__ long long block_of_cell(long long c, long long T, long long W) {
+    return div_nonneg((c + 1) * W - 1, T);
+}
 
 // sum over the warp's 32 lanes and inclusive prefix
 __device__ __forceinline__ long long warp_incl_sum(long long v, int lane) {
@@ -117,8 +125,10 @@ __device__ __forceinline__ long long warp_incl_sum(long long v, int lane) {
     return v;
 }
 
+// The index space that the blocks share: per unit `cost` cells without a tile, then one cell per tile.
 struct Share {
     long long T, W, lo, hi;   // all cells, blocks that take part, this block's range
+    int cost;
     int b;                    // the sequence that holds cell lo
     long long seq_lo;         // index of that sequence's first cell
 };
@@ -127,16 +137,20 @@ struct Share {
 __device__ __forceinline__ Share find_share(const DecodeParams& p, int lane) {
     const int U = p.Hkv * p.n_gblk;
     Share s;
-    long long sum = 0;
-    for (int i = lane; i < p.B; i += 32) sum += cells_of(clamp_len(__ldg(p.seq_lens + i), p.capacity));
-    s.T = __shfl_sync(0xffffffffu, warp_incl_sum(sum, lane), 31) * U;
+    long long tiles = 0;
+    for (int i = lane; i < p.B; i += 32) tiles += tiles_of(clamp_len(__ldg(p.seq_lens + i), p.capacity));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    const long long per_block = div_nonneg(tiles * U, gridDim.x);
+    s.cost = per_block < kUnitCost ? static_cast<int>(per_block) : kUnitCost;
+    s.T = (tiles + static_cast<long long>(s.cost) * p.B) * U;
     // no more blocks than cells: every block between the first and the last tile of a unit then holds some of its tiles,
     // which the count of pieces relies on
     s.W = gridDim.x < s.T ? gridDim.x : s.T;
     s.lo = s.hi = 0;
     if (blockIdx.x < s.W) {
-        s.lo = worker_lo(blockIdx.x, s.T, s.W);
-        s.hi = worker_lo(blockIdx.x + 1, s.T, s.W);
+        s.lo = cell_lo(blockIdx.x, s.T, s.W);
+        s.hi = cell_lo(blockIdx.x + 1, s.T, s.W);
     }
     s.b = 0;
     s.seq_lo = 0;
@@ -144,7 +158,7 @@ __device__ __forceinline__ Share find_share(const DecodeParams& p, int lane) {
     long long before = 0;
     for (int i0 = 0; i0 < p.B; i0 += 32) {
         const int i = i0 + lane;
-        const long long n = i < p.B ? static_cast<long long>(cells_of(clamp_len(__ldg(p.seq_lens + i), p.capacity))) * U : 0;
+        const long long n = i < p.B ? static_cast<long long>(s.cost + tiles_of(clamp_len(__ldg(p.seq_lens + i), p.capacity))) * U : 0;
         const long long end = before + warp_incl_sum(n, lane);
         const unsigned holds = __ballot_sync(0xffffffffu, s.lo < end);
         if (holds) {
@@ -199,9 +213,8 @@ __device__ __forceinline__ float rcp_approx(float x) {
 }
 
 // log-sum-exp merge of the pieces of one unit, 8 columns of one row per thread; pieces in worker order
-template <typename RowPtr>
+template <int kBatch, typename RowPtr>
 __device__ __forceinline__ void merge_pieces(int n, int c8, RowPtr row_ptr, float (&acc)[8], float& m_out, float& l_out) {
-    constexpr int kBatch = 4;
     float mrun = -INFINITY, lrun = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
@@ -289,9 +302,9 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                 tma_prefetch_desc(&tm_v);
             }
             int b = share.b;
-            int n_cells = cells_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
+            int n_cells = share.cost + tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
             const long long pos = lo - share.seq_lo;
-            int unit = static_cast<int>(pos / n_cells);
+            int unit = static_cast<int>(div_nonneg(pos, n_cells));
             int cell = static_cast<int>(pos - static_cast<long long>(unit) * n_cells);  // of the unit, next to look at
             int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
             int slot = grp, q_slot = 0;
@@ -305,7 +318,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 #pragma unroll 1
             while (left > 0) {
                 const int here = static_cast<int>(left < n_cells - cell ? left : n_cells - cell);  // of this unit
-                int tile = cell - kUnitCost;
+                int tile = cell - share.cost;
                 const int tile_end = tile + here;
                 if (tile < 0) tile = 0;
                 if (tile < tile_end) {
@@ -348,7 +361,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     gblk = 0;
                     if (++kvh == p.Hkv) {
                         kvh = 0;
-                        if (++b < p.B) n_cells = cells_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
+                        if (++b < p.B) n_cells = share.cost + tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
                     }
                 }
             }
@@ -386,8 +399,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
     int b = share.b;
     int len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
-    int n_cells = cells_of(len);
-    int unit = static_cast<int>((lo - share.seq_lo) / n_cells);  // within the sequence
+    int n_cells = share.cost + tiles_of(len);
+    int unit = static_cast<int>(div_nonneg(lo - share.seq_lo, n_cells));  // within the sequence
     long long unit_lo = share.seq_lo + static_cast<long long>(unit) * n_cells;
     bool first_unit = true;
     int turn = 0;    // the group whose turn the next tile is
@@ -398,10 +411,10 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
 #pragma unroll 1
     while (unit_lo < hi) {
-        const int n_t = n_cells - kUnitCost;
+        const int n_t = n_cells - share.cost;
         // this block's tiles of the unit
-        int tile = lo > unit_lo + kUnitCost ? static_cast<int>(lo - unit_lo) - kUnitCost : 0;
-        const int tile_end = hi < unit_lo + n_cells ? static_cast<int>(hi - unit_lo) - kUnitCost : n_t;
+        int tile = lo > unit_lo + share.cost ? static_cast<int>(lo - unit_lo) - share.cost : 0;
+        const int tile_end = hi < unit_lo + n_cells ? static_cast<int>(hi - unit_lo) - share.cost : n_t;
         const bool whole = tile == 0 && tile_end == n_t;
         if (tile < tile_end) {
         const int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
@@ -677,8 +690,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         if (!whole) {
             // this block's piece of the unit is in the workspace: count it in; the last one to arrive merges
             const long long W = share.W;
-            const long long w_first = worker_of_tile(unit_lo + kUnitCost, share.T, W);
-            const long long w_last = worker_of_tile(unit_lo + n_cells - 1, share.T, W);
+            const long long w_first = block_of_cell(unit_lo + share.cost, share.T, W);
+            const long long w_last = block_of_cell(unit_lo + n_cells - 1, share.T, W);
             const int n_pieces = static_cast<int>(w_last - w_first) + 1;
             unsigned* counter = p.counters + w_first;
             named_bar_sync(1, kConsumerWarps * 32);
@@ -692,14 +705,16 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
             named_bar_sync(1, kConsumerWarps * 32);
             if (misc[0] != 0) {
                 const int mrow = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
-                const int which_first = worker_lo(w_first, share.T, W) >= unit_lo ? 0 : 1;
+                const int which_first = cell_lo(w_first, share.T, W) >= unit_lo ? 0 : 1;
                 if (mrow < rows) {
                     float mg[8], mm, ll;
-                    merge_pieces(n_pieces, c8,
-                                 [&](int i) {
-                                     return p.slots + ((w_first + i) * 2 + (i == 0 ? which_first : 0)) * kSlotFloats + mrow * kPW;
-                                 },
-                                 mg, mm, ll);
+                    auto piece = [&](int i) {
+                        return p.slots + ((w_first + i) * 2 + (i == 0 ? which_first : 0)) * kSlotFloats + mrow * kPW;
+                    };
+                    if (n_pieces <= 4)
+                        merge_pieces<4>(n_pieces, c8, piece, mg, mm, ll);
+                    else
+                        merge_pieces<8>(n_pieces, c8, piece, mg, mm, ll);
                     const float inv = ll == 0.f ? 0.f : 1.f / ll;
                     uint4 pk;
                     pk.x = pack_bf16x2(mg[0] * inv, mg[1] * inv);
@@ -724,7 +739,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
             unit = 0;
             if (++b >= p.B) break;
             len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
-            n_cells = cells_of(len);
+            n_cells = share.cost + tiles_of(len);
         }
     }
 }
@@ -849,6 +864,9 @@ static int decode_launch(const void* q, const void* k, const void* v, const floa
     rc = make_decode_plan(B, capacity, Hq, Hkv, D, weights != nullptr, num_workers, di->sm_count, &plan);
     if (rc != CLLO_OK) return rc;
     if (!workspace || workspace_bytes < plan.bytes || !aligned_to(workspace, 256)) return CLLO_E_WORKSPACE;
+    const int n_chunks = (capacity + kWeightTok - 1) / kWeightTok;
+    const long long weight_blocks = static_cast<long long>(B) * Hkv * n_chunks;
+    if (weights && weight_blocks > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
     char* ws = static_cast<char*>(workspace);
     DecodeParams p;
     p.q = static_cast<const __nv_bfloat16*>(q);
@@ -883,10 +901,7 @@ static int decode_launch(const void* q, const void* k, const void* v, const floa
         rc = weights ? decode_launch_kernel<CLLO_FMT_INT8, true>(tm_k, tm_v, p, plan.W, attr + 2, st)
                      : decode_launch_kernel<CLLO_FMT_INT8, false>(tm_k, tm_v, p, plan.W, attr + 3, st);
     if (rc != CLLO_OK || !weights) return rc;
-    const int n_chunks = (capacity + kWeightTok - 1) / kWeightTok;
-    const long long blocks = static_cast<long long>(B) * Hkv * n_chunks;
-    if (blocks > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
-    decode_weights_kernel<<<static_cast<unsigned>(blocks), kWeightThreads, 0, st>>>(p, weights, n_chunks);
+    decode_weights_kernel<<<static_cast<unsigned>(weight_blocks), kWeightThreads, 0, st>>>(p, weights, n_chunks);
     CLLO_CUDA_TRY(cudaGetLastError());
     return CLLO_OK;
 }

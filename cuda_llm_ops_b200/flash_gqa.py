@@ -28,6 +28,8 @@ PARTIAL_WIDTH = HEAD_DIM + 2
 
 _workspaces = {}
 _workspaces_lock = threading.Lock()
+# every dict of cached workspaces whose arrival counters a kernel that gave up may have left non-zero
+_counted_workspaces = [_workspaces]
 
 
 def _stream_ptr():
@@ -678,6 +680,7 @@ def device_status():
     if rc != 0:
         # a kernel gave up half-way: the cached workspaces may hold counts of pieces that never got merged
         with _workspaces_lock:
-            for ws in _workspaces.values():
-                ws.zero_()
+            for cached in _counted_workspaces:
+                for ws in list(cached.values()):
+                    ws.zero_()
     return rc, list(detail)

@@ -14,6 +14,7 @@ Sequence lengths are int32 tensors on the device and are never read by the host,
 graph and follows the lengths at replay.  None of the calls changes a length; ``kv8_evict`` returns the new ones.
 (Upstream has no counterpart of these operators.)
 """
+import contextlib
 import ctypes
 import math
 import threading
@@ -21,10 +22,23 @@ import threading
 import torch
 
 from . import _lib
-from .flash_gqa import HEAD_DIM, KV_BHSD, KV_BSHD, _require_cuda_bf16, _stream_ptr
+from .flash_gqa import HEAD_DIM, KV_BHSD, KV_BSHD, _counted_workspaces, _require_cuda_bf16
 
 _FORMATS = {torch.float8_e4m3fn: _lib.FMT_E4M3, torch.int8: _lib.FMT_INT8}
 BLOCK_TOKENS = (16, 32, 64, 128)
+_MAX_POSITIONS = 1 << 30
+
+# A decoding step's calls take a few microseconds on the GPU: the device switch and the stream look-up of torch.cuda cost
+# as much again per call, so the switch is skipped where the device is current and the stream comes from the raw getter.
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(device):
+    return _NO_SWITCH if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+def _stream_ptr(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class KV8Cache:
@@ -88,7 +102,7 @@ def _check_lens(name, t, batch, device):
 
 
 def _check_fp32(name, t, shape, device):
-    if t.dtype != torch.float32 or t.shape != shape or t.device != device or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError("%s must be a contiguous fp32 tensor of shape %s on the same device" % (name, list(shape)))
 
 
@@ -97,9 +111,12 @@ def _require_cuda(cache):
         raise RuntimeError("the cache must be on a CUDA device: this library has no CPU path")
 
 
-def _row_strides(t, kv_layout):
-    b, x, y, _ = t.stride()
-    return (ctypes.c_longlong * 3)(b, x, y) if kv_layout == KV_BSHD else (ctypes.c_longlong * 3)(b, y, x)
+_Strides = ctypes.c_longlong * 3
+
+
+def _row_strides(s, kv_layout):
+    """{batch, token, head} of a [B,T,H,D] or [B,H,T,D] tensor's strides."""
+    return _Strides(s[0], s[1], s[2]) if kv_layout == KV_BSHD else _Strides(s[0], s[2], s[1])
 
 
 def kv8_append(cache, k_new, v_new, seq_lens, new_lens=None):
@@ -124,8 +141,8 @@ def kv8_append(cache, k_new, v_new, seq_lens, new_lens=None):
         raise ValueError("k_new and v_new must match the cache's batch, kv heads and head_dim")
     if k_new.device != device or v_new.device != device:
         raise ValueError("k_new and v_new must be on the cache's device")
-    for name, t in (("k_new", k_new), ("v_new", v_new)):
-        s = t.stride()
+    k_strides, v_strides = k_new.stride(), v_new.stride()
+    for name, t, s in (("k_new", k_new, k_strides), ("v_new", v_new, v_strides)):
         if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16:
             raise ValueError("%s must have contiguous, 16-byte aligned rows" % name)
     _check_lens("seq_lens", seq_lens, B, device)
@@ -133,17 +150,18 @@ def kv8_append(cache, k_new, v_new, seq_lens, new_lens=None):
         _check_lens("new_lens", new_lens, B, device)
     if T == 0:
         return
-    with torch.cuda.device(device):
+    with _on(device):
         rc = _lib.load().cllo_kv8_append_bf16(
-            k_new.data_ptr(), _row_strides(k_new, cache.kv_layout), v_new.data_ptr(),
-            _row_strides(v_new, cache.kv_layout), seq_lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
+            k_new.data_ptr(), _row_strides(k_strides, cache.kv_layout), v_new.data_ptr(),
+            _row_strides(v_strides, cache.kv_layout), seq_lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
             cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), B, T,
-            cache.capacity, H, D, cache.kv_layout, cache.block_tokens, cache.format, _stream_ptr())
+            cache.capacity, H, D, cache.kv_layout, cache.block_tokens, cache.format, _stream_ptr(device))
     _lib.check(rc, "cllo_kv8_append_bf16")
 
 
 _workspaces = {}
 _workspaces_lock = threading.Lock()
+_counted_workspaces.append(_workspaces)
 
 
 def _workspace(kind, device, nbytes):
@@ -153,13 +171,15 @@ def _workspace(kind, device, nbytes):
     counters zero.  A call that is being captured gets a tensor of its own from the graph's pool, and the call clears the
     counters at every replay: two graphs may be replayed at the same time.
     """
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device), 0
-    key = (kind, device.index, _stream_ptr())
-    with _workspaces_lock:
-        ws = _workspaces.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = _workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+    key = (kind, device.index, _stream_ptr(device))
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        with _workspaces_lock:
+            ws = _workspaces.get(key)
+            if ws is None or ws.numel() < nbytes:
+                ws = _workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
     return ws, _lib.WS_COUNTERS_ZERO
 
 
@@ -182,6 +202,8 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
     if Hq == 0 or Hq % H != 0:
         raise ValueError("Query heads must be divisible by KV heads")
     _check_lens("seq_lens", seq_lens, B, device)
+    if not 0 <= num_workers <= _MAX_POSITIONS:
+        raise ValueError("num_workers must not be negative")
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if out is None:
@@ -193,7 +215,7 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
     if weights is not None:
         _check_fp32("weights", weights, (B, H, cache.capacity), device)
     lib = _lib.load()
-    with torch.cuda.device(device):
+    with _on(device):
         nbytes = _decode_workspace_bytes(device, B, cache.capacity, Hq, H, weights is not None, num_workers)
         flag = 0
         if workspace is None:
@@ -203,7 +225,7 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
             seq_lens.data_ptr(), scale, out.data_ptr(), None if lse is None else lse.data_ptr(),
             None if weights is None else weights.data_ptr(), workspace.data_ptr(),
             workspace.numel() * workspace.element_size(), B, cache.capacity, Hq, H, D, cache.kv_layout | flag,
-            cache.block_tokens, cache.format, num_workers, _stream_ptr())
+            cache.block_tokens, cache.format, num_workers, _stream_ptr(device))
     _lib.check(rc, "cllo_kv8_decode_bf16")
     return out
 
@@ -253,8 +275,8 @@ def attention_weight_sums(q, k, lse, scale=None, causal=True, q_start=0, seq_len
         _check_lens("seq_lens", seq_lens, B, device)
     if window is not None and window < 1:
         raise ValueError("window must be positive")
-    if q_start < 0:
-        raise ValueError("q_start must not be negative")
+    if not 0 <= q_start <= _MAX_POSITIONS // 2:
+        raise ValueError("q_start must not be negative or beyond 2^29")
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
@@ -264,15 +286,15 @@ def attention_weight_sums(q, k, lse, scale=None, causal=True, q_start=0, seq_len
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     lib = _lib.load()
-    with torch.cuda.device(device):
+    with _on(device):
         flags = _lib.SUMS_ACCUMULATE if accumulate else 0
         if workspace is None:
             workspace, zero = _workspace("sums", device, int(lib.cllo_attn_weight_sums_workspace_bytes()))
             flags |= zero
         rc = lib.cllo_attn_weight_sums_bf16(
             q.data_ptr(), k.data_ptr(), lse.data_ptr(), None if seq_lens is None else seq_lens.data_ptr(), scale,
-            1 if causal else 0, q_start, window or 0, flags, out.data_ptr(), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), B, Sq, Skv, Hq, H, D, _stream_ptr())
+            1 if causal else 0, q_start, min(window or 0, _MAX_POSITIONS), flags, out.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), B, Sq, Skv, Hq, H, D, _stream_ptr(device))
     _lib.check(rc, "cllo_attn_weight_sums_bf16")
     return out
 
@@ -289,8 +311,8 @@ def kv8_evict(cache, weights, seq_lens, budget, sink=0, recent=0, out=None, out_
     _require_cuda(cache)
     device = cache.k.device
     B, H = cache.batch, cache.num_kv_heads
-    if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget:
-        raise ValueError("budget must be positive and hold the sink and recent tokens")
+    if not 1 <= budget <= _MAX_POSITIONS or sink < 0 or recent < 0 or sink + recent > budget:
+        raise ValueError("budget must be positive (at most 2^30) and hold the sink and recent tokens")
     _check_fp32("weights", weights, (B, H, cache.capacity), device)
     _check_lens("seq_lens", seq_lens, B, device)
     if out is None:
@@ -304,7 +326,7 @@ def kv8_evict(cache, weights, seq_lens, budget, sink=0, recent=0, out=None, out_
         out_weights = torch.zeros((B, H, out.capacity), dtype=torch.float32, device=device)
     else:
         _check_fp32("out_weights", out_weights, (B, H, out.capacity), device)
-    with torch.cuda.device(device):
+    with _on(device):
         new_lens = torch.empty(B, dtype=torch.int32, device=device)
         indices = torch.empty((B, H, budget), dtype=torch.int32, device=device)
         rc = _lib.load().cllo_kv8_evict(
@@ -312,6 +334,6 @@ def kv8_evict(cache, weights, seq_lens, budget, sink=0, recent=0, out=None, out_
             weights.data_ptr(), seq_lens.data_ptr(), out.k.data_ptr(), out.v.data_ptr(), out.k_scale.data_ptr(),
             out.v_scale.data_ptr(), out_weights.data_ptr(), new_lens.data_ptr(), indices.data_ptr(), B, cache.capacity,
             out.capacity, H, HEAD_DIM, budget, sink, recent, cache.kv_layout, cache.block_tokens, cache.format,
-            _stream_ptr())
+            _stream_ptr(device))
     _lib.check(rc, "cllo_kv8_evict")
     return out, out_weights, new_lens, indices

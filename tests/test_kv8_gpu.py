@@ -500,6 +500,144 @@ def test_evict_makes_its_own_tensors_and_holds_lengths_to_the_cache():
 
 
 # ------------------------------------------------------------------------------------------------------------------
+# beyond 32 bits, captured, on other streams
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("layout", [0, 1])
+def test_offsets_beyond_32_bits(layout):
+    """A cache of 5 GB for K and 5 GB for V: the second sequence lies behind 2^31 bytes, its last heads behind 2^32."""
+    ops = _ops()
+    B, H, S, G, block = 2, 8, 2400000, 2, 64
+    cache = ops.kv8_cache(B, S, H, torch.int8, layout, block)
+    for i, t in enumerate((cache.k, cache.v)):
+        t.random_(-127, 128, generator=_gen(i + 1))
+    cache.k_scale.fill_(2.0 ** -6)
+    cache.v_scale.fill_(2.0 ** -5)
+    # the last rows come from an append
+    held = [5, S - 70]
+    rows = [_rows(3 + i, *_shape(layout, B, 70, H)) for i in range(2)]
+    ops.kv8_append(cache, rows[0], rows[1], _ints(held))
+    lens = _ints([75, S])
+    q = torch.randn(B, H * G, D, generator=_gen(5), device="cuda").to(torch.bfloat16)
+    weights = torch.zeros(B, H, S, device="cuda")
+    lse = torch.empty(B, H * G, device="cuda")
+    out = ops.kv8_decode(q, cache, lens, lse=lse, weights=weights)
+    new, new_weights, new_lens, indices = ops.kv8_evict(cache, weights, lens, 300, sink=2, recent=80)
+    assert new_lens.tolist() == [75, 300]
+    for h in (0, 5, H - 1):
+        one = [ref.heads_first(t, layout)[1:, h:h + 1].contiguous() for t in (cache.k, cache.v)]
+        sub = ops.KV8Cache(one[0], one[1], *(t[1:, h:h + 1].contiguous() for t in (cache.k_scale, cache.v_scale)),
+                           kv_layout=1, block_tokens=block)
+        heads = slice(h * G, (h + 1) * G)
+        _check_decode(sub, q[1:, heads], lens[1:], SCALE, out[1:, heads], lse[1:, heads],
+                      added=(torch.zeros(1, 1, S, device="cuda"), weights[1:, h:h + 1]))
+        w = weights[1, h].clone()
+        w[:2], w[S - 80:] = math.inf, math.inf
+        want = torch.sort(torch.sort(w, descending=True, stable=True).indices[:300]).values
+        assert torch.equal(indices[1, h].long(), want)
+        k, v = ref.values(sub)
+        for vals, codes, scales in ((k, new.k, new.k_scale), (v, new.v, new.v_scale)):
+            got = ref.heads_first(codes, layout)[1, h].double()
+            s = scales[1, h].double().repeat_interleave(block)[:300, None]
+            x = vals[0, 0][want]
+            assert ((got * s - x).abs() <= s / 2).all()  # one rounding to the new scale
+    assert_clean_status()
+
+
+def test_every_call_in_one_graph_on_another_stream():
+    """Append, decode with weights, weight sums and eviction captured into one graph; replayed twice with other inputs and
+    compared with eager calls."""
+    ops = _ops()
+    B, H, Hq, cap, block = 2, 2, 8, 256, 32
+    lens = _ints([100, 37])
+    caches = [_filled_cache(60, B, cap, H, torch.float8_e4m3fn, 1, block, [cap, cap]) for _ in range(2)]
+    kn, vn = _rows(61, B, H, 3, D), _rows(62, B, H, 3, D)
+    q = torch.randn(B, Hq, D, generator=_gen(63), device="cuda").to(torch.bfloat16)
+    qp = torch.randn(B, Hq, cap, D, generator=_gen(64), device="cuda").to(torch.bfloat16)
+    kp = torch.randn(B, H, cap, D, generator=_gen(65), device="cuda").to(torch.bfloat16)
+    lse = torch.full((B, Hq, cap), 6.0, device="cuda")
+    after = torch.empty_like(lens)
+    results = [dict(w=torch.zeros(B, H, cap, device="cuda")) for _ in range(2)]
+
+    def work(cache, r):
+        ops.kv8_append(cache, kn, vn, lens)
+        torch.add(lens, 3, out=after)
+        r["out"] = ops.kv8_decode(q, cache, after, weights=r["w"])
+        ops.attention_weight_sums(qp, kp, lse, seq_lens=after, out=r["w"], accumulate=True)
+        r["evicted"] = ops.kv8_evict(cache, r["w"], after, 40, sink=1, recent=8)
+
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        work(caches[0], results[0])
+    for step in range(2):
+        kn.normal_()
+        q.normal_()
+        for c in results:
+            c["w"].zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        work(caches[1], results[1])
+        torch.cuda.synchronize()
+        a, b = results
+        assert torch.equal(a["out"].view(torch.int16), b["out"].view(torch.int16)) and torch.equal(a["w"], b["w"])
+        assert torch.equal(a["evicted"][3], b["evicted"][3]) and torch.equal(a["evicted"][2], b["evicted"][2])
+        n = int(b["evicted"][2].min())
+        assert torch.equal(a["evicted"][0].k.view(torch.uint8)[:, :, :n], b["evicted"][0].k.view(torch.uint8)[:, :, :n])
+        lens.copy_(_ints([200, 0]))
+    assert_clean_status()
+
+
+def test_weight_sums_on_two_streams_and_in_parts():
+    ops = _ops()
+    q = torch.randn(1, 8, 3000, D, generator=_gen(1), device="cuda").to(torch.bfloat16)
+    k = torch.randn(1, 2, 3000, D, generator=_gen(2), device="cuda").to(torch.bfloat16)
+    lse = torch.full((1, 8, 3000), 7.0, device="cuda")
+    want = ops.attention_weight_sums(q, k, lse)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ops.attention_weight_sums(q, k, lse))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    # a prompt in two chunks adds up to the whole one
+    parts = ops.attention_weight_sums(q[:, :, :1111].contiguous(), k, lse[:, :, :1111].contiguous())
+    ops.attention_weight_sums(q[:, :, 1111:].contiguous(), k, lse[:, :, 1111:].contiguous(), q_start=1111, out=parts,
+                              accumulate=True)
+    _check_sums(parts, q, k, lse, SCALE, True)
+    assert_clean_status()
+
+
+def test_own_workspaces():
+    """A caller's workspace may hold anything; one too small or none of its size is refused."""
+    ops = _ops()
+    from cuda_llm_ops_b200 import _lib
+    lib = _lib.load()
+    lens = [3000, 2000]
+    cache = _filled_cache(6, 2, 3000, 2, torch.int8, 0, 64, lens)
+    q = torch.randn(2, 16, D, generator=_gen(10), device="cuda").to(torch.bfloat16)
+    n = int(lib.cllo_kv8_decode_workspace_bytes(2, 3000, 16, 2, D, 1, 0))
+    ws = torch.randint(0, 256, (n,), generator=_gen(1), device="cuda").to(torch.uint8)
+    weights = torch.zeros(2, 2, 3000, device="cuda")
+    out = ops.kv8_decode(q, cache, _ints(lens), weights=weights, workspace=ws)
+    _check_decode(cache, q, _ints(lens), SCALE, out, added=(torch.zeros_like(weights), weights))
+    with pytest.raises(RuntimeError, match="workspace"):
+        ops.kv8_decode(q, cache, _ints(lens), weights=weights, workspace=ws[:n - 256])
+    n = int(lib.cllo_attn_weight_sums_workspace_bytes())
+    qp = torch.randn(1, 4, 700, D, generator=_gen(1), device="cuda").to(torch.bfloat16)
+    lse = torch.full((1, 4, 700), 6.0, device="cuda")
+    ws = torch.randint(0, 256, (n,), generator=_gen(1), device="cuda").to(torch.uint8)
+    got = ops.attention_weight_sums(qp, qp[:, :2].contiguous(), lse, workspace=ws)
+    _check_sums(got, qp, qp[:, :2].contiguous(), lse, SCALE, True)
+    with pytest.raises(RuntimeError, match="workspace"):
+        ops.attention_weight_sums(qp, qp[:, :2].contiguous(), lse, workspace=ws[:n - 256])
+
+
+# ------------------------------------------------------------------------------------------------------------------
 # together
 # ------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ref.DTYPES)
