@@ -14,22 +14,23 @@
 // a cut unit through the workspace by the last block to arrive.  All SMs take part: at 8 stages (128 KB) the bytes in
 // flight stay below what slows the memory system (12 stages: 5 % slower on 148 SMs), and it is the arithmetic that bounds.
 //
-// Arithmetic on codes.  The codes become f16, which holds every e4m3 and int8 value exactly, and feed mma.sync
-// m16n8k16 with fp32 accumulation; the scales never touch the codes:
-//   * a query row is brought to [2^14, 2^15) by a power of two before it becomes f16 (exact for every bf16 value within
-//     2^28 of the row's largest, and below 2^-39 of it otherwise), which is taken back in the factor of the scores;
-//   * the K scale is part of that factor: 16 tokens of a warp lie in one block of the cache (blocks are multiples of 16);
-//   * the V scale goes into the exponent: with lv = log2 vscale, p'_t = 2^(s_t + lv_t - m + 11), m = max(s_t + lv_t), so
-//     that O = sum p' v8 needs no scaling and l = sum p'_t / vscale_t.  p' is rounded to f16 for the product (half a step:
-//     2^-11 relative, 2^-25 absolute below f16's normal range), l is summed in fp32 before rounding.  The reference m may
-//     lag behind the true maximum by 2^4 (kLazy), so the largest p' lies in [2^11, 2^15] and the absolute part is at most
-//     2^-36 of it.
+// Arithmetic on codes.  The codes become f16, which holds every e4m3 and int8 value exactly, and feed mma.sync m16n8k16 with
+// fp32 accumulation; the scales never touch the codes.  (mma.sync on e4m3 operands is carried out as two f16 products on
+// this part: with the query split into two e4m3 terms the scores cost 16 more of them per 16 tokens, 121 us instead of 105.)
+//   * a query row is brought to [2^14, 2^15) by a power of two before it becomes f16: exact for every bf16 value within
+//     2^28 of the row's largest, and below 2^-39 of it otherwise;
+//   * the factor of the query row and the K scale multiply the fp32 scores: 16 tokens of a warp lie in one block of the
+//     cache (blocks are multiples of 16);
+//   * the V codes become f16 for m16n8k16, and the V scale goes into the exponent: with lv = log2 vscale,
+//     p'_t = 2^(s_t + lv_t - m + 11), m = max(s_t + lv_t), so that O = sum p' v8 needs no scaling and
+//     l = sum p'_t / vscale_t.  p' is rounded to f16 for the product (half a step: 2^-11 relative, 2^-25 absolute below f16's
+//     normal range), l is summed in fp32 before rounding.  The reference m may lag behind the true maximum by 2^4 (kLazy),
+//     so the largest p' lies in [2^11, 2^15] and the absolute part is at most 2^-36 of it.
 //
-// Layout without transposes.  K: a lane reads 2 x 16 bytes of its token's row; dims may be permuted freely as long as Q
-// uses the same permutation, so each 4-byte word is one k-step of the B operand.  V: ldmatrix.trans on 16-bit pairs of
-// dims hands a lane {token a: d, d+1 | token b: d, d+1}; one byte permutation makes {a,b} pairs for dim d and for dim d + 1,
-// the B operands of an "even" and an "odd" n-block.  Tokens of an 8-row block are taken in the order 0,4,1,5,2,6,3,7,
-// which makes the 16-byte K reads free of bank conflicts under the TMA swizzle.
+// Layout without transposes.  K: a lane reads 32 consecutive bytes of its token's row as the B operand; the k index may be
+// permuted freely as long as Q uses the same permutation.  V: the transposing 8-bit load hands a lane four tokens of one
+// dim, two B operand registers once they are f16.  The tokens of the score columns are ordered so that a lane's
+// probabilities are of those same four tokens.
 #pragma once
 
 #include "gqa_decode.cuh"
@@ -53,7 +54,7 @@ constexpr int kConsumerWarps = kGroups * kWarpsPerGroup;
 // and scores of their tokens beside them; at the 168 registers that 384 threads get they would spill.  The pool is what
 // the block was launched with; asking for more in total would never return.
 constexpr int kDecodeThreads = (kConsumerWarps + 4) * 32;
-constexpr int kLaunchRegs = 168, kConsumerRegs = 224, kProducerRegs = 56;
+constexpr int kLaunchRegs = 168, kConsumerRegs = 232, kProducerRegs = 40;
 static_assert(2 * kConsumerRegs + kProducerRegs <= 3 * kLaunchRegs, "setmaxnreg budget exceeds the block's register pool");
 static_assert(kConsumerWarps == 8 && kDecodeThreads == 384, "the register budget is for three warpgroups");
 constexpr int kTileBytes = kTok * kD;           // K or V of one stage
@@ -93,10 +94,11 @@ struct DecodeParams {
     const int* seq_lens;
     __nv_bfloat16* o;
     float* lse;       // nullable
-    float* scores;    // nullable: [B, Hq, capacity] scaled scores in log2 units, for the weights
+    float* scores;    // nullable: [B, Hq, score_pitch] scaled scores in log2 units, for the weights
     float* lse2;      // with scores: [B, Hq] log2 of the normaliser
     float* slots;     // [W][2][16][kPW]
     unsigned* counters;
+    long long score_pitch;  // capacity rounded up to whole tiles
     float scale_log2;
     int B, Hq, Hkv, G, n_gblk, capacity, n_blocks, block_shift, kv_layout;
 };
@@ -177,6 +179,13 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Two 16 x 16 byte matrices, transposed: of the first, r0 holds rows 4 (lane % 4) .. + 3 of column lane / 4 and r1 the same
+// rows of column lane / 4 + 8; r2 and r3 of the second.  Lanes 0-15 give the rows of the first, 16-31 of the second.
+__device__ __forceinline__ void ldmatrix_b8_x2_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 r;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
@@ -190,11 +199,6 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
 // an arrival on a barrier once this thread's earlier asynchronous copies have landed
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ uint2 lds64u(uint32_t addr) {
-    uint2 r;
-    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(addr));
-    return r;
 }
 // untiled asynchronous copy, 16-byte aligned, size a multiple of 16
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -389,13 +393,18 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
     const int g = lane >> 2, tig = lane & 3;
     const int grp = warp / kWarpsPerGroup, sub = warp % kWarpsPerGroup;
-    // this lane's rows of a 16-token slice: K row of n-block nt is nt * 8 + tok_g; score columns are tokens
-    // nt * 8 + tig and nt * 8 + tig + 4
-    const int tok_g = (g >> 1) | ((g & 1) << 2);
-    // ldmatrix row pointers of V: lanes 0-7 rows of the first 8 tokens, 8-15 of the second, 16-31 the same of the next chunk
-    const int v_row_in = ((lane & 7) >> 1) | ((lane & 1) << 2);
-    const uint32_t v_row = static_cast<uint32_t>(sub * kSubTok + ((lane >> 3) & 1) * 8 + v_row_in);
-    const uint32_t k_row = static_cast<uint32_t>(sub * kSubTok + tok_g);
+    // Tokens of a 16-token part: column n of score n-block nt is token 4 (n >> 1) + 2 nt + (n & 1), so that a lane's four score
+    // columns are the tokens 4 tig .. 4 tig + 3, which is also what the transposing load of V hands it.
+    // Byte offsets in a tile: K row of n-block nt, 16-byte chunk 2 tig (chunk 2 tig + 1 differs in bit 4; the lanes of a quarter
+    // warp touch all eight chunks of the swizzled rows), and the V row this lane addresses, its chunk 0 or 1.
+    uint32_t k_off[2];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+        const uint32_t row = static_cast<uint32_t>(sub * kSubTok + 4 * (g >> 1) + 2 * nt + (g & 1));
+        k_off[nt] = row * 128u + ((static_cast<uint32_t>(2 * tig) ^ (row & 7u)) << 4);
+    }
+    const uint32_t v_row = static_cast<uint32_t>(sub * kSubTok + (lane & 15));
+    const uint32_t v_off = v_row * 128u, v_swz = (v_row & 7u) ^ static_cast<uint32_t>(lane >> 4);
 
     int b = share.b;
     int len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
@@ -421,33 +430,39 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         const int rows = (p.G - gblk * kRows) < kRows ? (p.G - gblk * kRows) : kRows;
         const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(kvh) * p.G + gblk * kRows;
 
-        // Q fragments: k-step (j, w) takes dims 16 (tig + 4 j) + 4 w + {0,1} and + {2,3}
+        // Q fragments: a lane's K codes of a token are dims 32 tig .. 32 tig + 31, and so are its dims of a query row; four dims
+        // make a k-step
         uint32_t qf[8][4];
-        float mul0, mul1;  // |scale| * log2(e) * 2^-shift of the two rows
+        float mul0, mul1;  // |scale| * log2(e) / the rows' factors
         mbar_wait_idle(q_full_bar(q_slot), q_phase, abort_flag, SITE_KV8_Q_FULL, q_slot);
         __syncwarp();
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            uint2 raw[8];
+            uint4 raw[4];
             float amax = 0.f;
             const bool ok = g + 8 * r < rows;
-            const uint32_t src = base + kSmemQ + q_slot * kQBytes + (g + 8 * r) * kQPitch + tig * 32;
+            const uint32_t src = base + kSmemQ + q_slot * kQBytes + (g + 8 * r) * kQPitch + tig * 64;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) raw[i] = ok ? lds64u(src + (i >> 2) * 128 + (i & 3) * 8) : make_uint2(0u, 0u);
+            for (int i = 0; i < 4; ++i) raw[i] = ok ? lds128(src + i * 16) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(bf16_lo(raw[i].x)), finite_abs(bf16_hi(raw[i].x))),
-                                         fmaxf(finite_abs(bf16_lo(raw[i].y)), finite_abs(bf16_hi(raw[i].y)))));
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fmaxf(finite_abs(bf16_lo(w[e])), finite_abs(bf16_hi(w[e]))));
+            }
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
-            e = e < -100 ? -100 : e;  // rows below 2^-100 (zero among them): their scores vanish either way
-            const float f = copysignf(exp2_int(14 - e), p.scale_log2);  // the sign of the scale goes with the query
-            (r ? mul1 : mul0) = fabsf(p.scale_log2) * exp2_int(e - 14);
+            e -= 14;  // the row's largest magnitude goes to [2^14, 2^15)
+            e = e < -100 ? -100 : e;  // rows below 2^-100 or so (zero among them): their scores vanish either way
+            const float f = copysignf(exp2_int(-e), p.scale_log2);  // the sign of the scale goes with the query
+            (r ? mul1 : mul0) = fabsf(p.scale_log2) * exp2_int(e);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                qf[i][r] = pack_f16x2(bf16_lo(raw[i].x) * f, bf16_hi(raw[i].x) * f);
-                qf[i][r + 2] = pack_f16x2(bf16_lo(raw[i].y) * f, bf16_hi(raw[i].y) * f);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    qf[2 * i + (c >> 1)][(c & 1) * 2 + r] = pack_f16x2(bf16_lo(w[c]) * f, bf16_hi(w[c]) * f);
             }
         }
         __syncwarp();
@@ -480,46 +495,47 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                 float s[kParts][2][4];
 #pragma unroll
                 for (int u = 0; u < kParts; ++u) {
-                    uint4 kw[2][2];
+                    uint32_t kw[2][8];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int nt = 0; nt < 2; ++nt)
-                            kw[nt][j] = lds128(kb + (k_row + u * 16 + nt * 8) * 128u +
-                                               ((static_cast<uint32_t>(tig + 4 * j) ^ (k_row & 7u)) << 4));
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const uint4 x = lds128(kb + u * 2048 + k_off[nt]), y = lds128(kb + u * 2048 + (k_off[nt] ^ 16u));
+                        kw[nt][0] = x.x;
+                        kw[nt][1] = x.y;
+                        kw[nt][2] = x.z;
+                        kw[nt][3] = x.w;
+                        kw[nt][4] = y.x;
+                        kw[nt][5] = y.y;
+                        kw[nt][6] = y.z;
+                        kw[nt][7] = y.w;
+                    }
                     float s2[2][4];
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[u][nt][e] = s2[nt][e] = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
+                    for (int i = 0; i < 8; ++i)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                            for (int nt = 0; nt < 2; ++nt) {
-                                const uint32_t ww[4] = {kw[nt][j].x, kw[nt][j].y, kw[nt][j].z, kw[nt][j].w};
-                                uint32_t b0, b1;
-                                decode4_f16<kFmt>(ww[i], b0, b1);
-                                mma_f16_16816((i & 1) ? s2[nt] : s[u][nt], qf[j * 4 + i], b0, b1);
-                            }
+                        for (int nt = 0; nt < 2; ++nt) {
+                            uint32_t b0, b1;
+                            decode4_f16<kFmt>(kw[nt][i], b0, b1);
+                            mma_f16_16816((i & 1) ? s2[nt] : s[u][nt], qf[i], b0, b1);
                         }
-                    }
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[u][nt][e] += s2[nt][e];
                 }
                 if (valid < kSubTok) {
-                    // tokens behind the sequence have no score, a half without tokens no scales that anybody wrote
-                    if (kParts > 1 && valid <= 16) ksc[kParts - 1] = vsc[kParts - 1] = 1.f;
+                    // tokens behind the sequence have no score, a part without tokens no scales that anybody wrote
+                    if (valid <= 16) ksc[kParts - 1] = vsc[kParts - 1] = 1.f;
 #pragma unroll
                     for (int u = 0; u < kParts; ++u)
 #pragma unroll
                         for (int nt = 0; nt < 2; ++nt) {
-                            const int c = u * 16 + nt * 8 + tig;
+                            const int c = u * 16 + 4 * tig + 2 * nt;
                             if (c >= valid) s[u][nt][0] = s[u][nt][2] = -INFINITY;
-                            if (c + 4 >= valid) s[u][nt][1] = s[u][nt][3] = -INFINITY;
+                            if (c + 1 >= valid) s[u][nt][1] = s[u][nt][3] = -INFINITY;
                         }
                 }
                 // ---- online softmax on the raw scores: y = s * f, V scale in the exponent ----
@@ -534,19 +550,17 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     mn1 = fmaxf(mn1, fmaf(fmaxf(fmaxf(s[u][0][2], s[u][0][3]), fmaxf(s[u][1][2], s[u][1][3])), f1[u], lv[u]));
                 }
                 if (kScores) {
+                    // the pitch has room for whole tiles; what is written behind the sequence is never read
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         if (g + 8 * r < rows) {
-                            float* dst = p.scores + (head0 + g + 8 * r) * p.capacity + tok0 + tig;
+                            float* dst = p.scores + (head0 + g + 8 * r) * p.score_pitch + tok0 + 4 * tig;
 #pragma unroll
-                            for (int u = 0; u < kParts; ++u)
-#pragma unroll
-                                for (int nt = 0; nt < 2; ++nt) {
-                                    const int c = u * 16 + nt * 8;
-                                    const float f = r ? f1[u] : f0[u];
-                                    if (c + tig < valid) dst[c] = s[u][nt][2 * r] * f;
-                                    if (c + tig + 4 < valid) dst[c + 4] = s[u][nt][2 * r + 1] * f;
-                                }
+                            for (int u = 0; u < kParts; ++u) {
+                                const float f = r ? f1[u] : f0[u];
+                                *reinterpret_cast<float4*>(dst + u * 16) =
+                                    make_float4(s[u][0][2 * r] * f, s[u][0][2 * r + 1] * f, s[u][1][2 * r] * f, s[u][1][2 * r + 1] * f);
+                            }
                         }
                     }
                 }
@@ -572,11 +586,20 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                 }
 #pragma unroll
                 for (int u = 0; u < kParts; ++u) {
+                    // V codes: word i of a load is dim 32 cp + 8 i + g of the tokens 4 tig .. 4 tig + 3
                     uint32_t vw[4][4];
 #pragma unroll
                     for (int cp = 0; cp < 4; ++cp)
-                        ldmatrix_x4_trans(vb + (v_row + u * 16) * 128u + ((static_cast<uint32_t>(cp * 2 + (lane >> 4)) ^ (v_row & 7u)) << 4),
-                                          vw[cp][0], vw[cp][1], vw[cp][2], vw[cp][3]);
+                        ldmatrix_b8_x2_trans(vb + u * 2048 + v_off + ((v_swz ^ static_cast<uint32_t>(cp * 2)) << 4), vw[cp]);
+                    if (valid < kSubTok) {
+                        // values of tokens behind the sequence may be NaN codes, which a zero probability does not silence
+                        const int n = valid - (u * 16 + 4 * tig);
+                        const uint32_t keep = n >= 4 ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * n)) - 1u);
+#pragma unroll
+                        for (int cp = 0; cp < 4; ++cp)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) vw[cp][i] &= keep;
+                    }
                     const float iv = rcp_approx(vsc[u]);
                     const float c0 = lv[u] + kPShift - m0, c1 = lv[u] + kPShift - m1;
                     const float p00 = fast_exp2(fmaf(s[u][0][0], f0[u], c0)), p01 = fast_exp2(fmaf(s[u][0][1], f0[u], c0));
@@ -590,22 +613,12 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     pa[1] = pack_f16x2(p02, p03);
                     pa[2] = pack_f16x2(p10, p11);
                     pa[3] = pack_f16x2(p12, p13);
-                    // ---- O += P V: {a: d, d+1 | b: d, d+1} -> {a.d, b.d, a.d+1, b.d+1} -> f16 pairs ----
-                    uint32_t sel_lo = 0x3120u, sel_hi = 0x3120u;
-                    if (valid < kSubTok) {
-                        // values of tokens behind the sequence may be NaN codes, which a zero probability does not
-                        // silence: zero bytes in their place
-                        const int c = u * 16 + tig;
-                        sel_lo = (c < valid ? 0x0100u : 0x0404u) | (c + 4 < valid ? 0x3020u : 0x4040u);
-                        sel_hi = (c + 8 < valid ? 0x0100u : 0x0404u) | (c + 12 < valid ? 0x3020u : 0x4040u);
-                    }
+                    // ---- O += P V ----
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        uint32_t e0, e1, d0, d1;
-                        decode4_f16<kFmt>(__byte_perm(vw[c >> 1][2 * (c & 1)], 0u, sel_lo), e0, d0);
-                        decode4_f16<kFmt>(__byte_perm(vw[c >> 1][2 * (c & 1) + 1], 0u, sel_hi), e1, d1);
-                        mma_f16_16816(o[c * 2], pa, e0, e1);
-                        mma_f16_16816(o[c * 2 + 1], pa, d0, d1);
+                    for (int c = 0; c < 16; ++c) {
+                        uint32_t b0, b1;
+                        decode4_f16<kFmt>(vw[c >> 2][c & 3], b0, b1);
+                        mma_f16_16816(o[c], pa, b0, b1);
                     }
                 }
             }
@@ -618,23 +631,20 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         }
         turn = (turn + n_here) % kGroups;
 
-        // ---- merge the private states: every warp posts its (m, l) and, two 16-dim chunks at a time, its O; a warp
-        // sums two values per lane and round over the warps, in fixed order and with each one's factor: chunk 2 rd + (warp >> 2), row
-        // half (warp >> 1) & 1, and of the 32 lanes' quads the half that (warp & 1) says ----
+        // ---- merge the private states: every warp posts its (m, l) and, four 8-dim n-blocks at a time, its O; a warp sums two
+        // values per lane and round over the warps, in fixed order and with each one's factor: n-block 4 rd + (warp >> 1), row
+        // half warp & 1 ----
         *reinterpret_cast<float4*>(stat + (warp * 32 + lane) * 4) = make_float4(m0, m1, l0, l1);
-        float4* post = reinterpret_cast<float4*>(xchg);
-        const int half = (warp >> 1) & 1, my_chunk = warp >> 2;
+        float2* post = reinterpret_cast<float2*>(xchg);
+        const int half = warp & 1;
         float f[kConsumerWarps], ms = -INFINITY, lt = 0.f, acc[4][2];
 #pragma unroll
         for (int rd = 0; rd < 4; ++rd) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {  // dims 16 (2 rd + c) + 4 tig + {0..3} of row g + 8 r
-                    const int b0 = 2 * (2 * rd + c);
-                    post[((warp * 2 + c) * 2 + r) * 32 + lane] =
-                        make_float4(o[b0][2 * r], o[b0 + 1][2 * r], o[b0][2 * r + 1], o[b0 + 1][2 * r + 1]);
-                }
+                for (int r = 0; r < 2; ++r)
+                    post[((warp * 4 + c) * 2 + r) * 32 + lane] = make_float2(o[4 * rd + c][2 * r], o[4 * rd + c][2 * r + 1]);
             named_bar_sync(1, kConsumerWarps * 32);
             if (rd == 0) {
 #pragma unroll
@@ -653,8 +663,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
             float a0 = 0.f, a1 = 0.f;
 #pragma unroll
             for (int sw = 0; sw < kConsumerWarps; ++sw) {
-                const float2 x = *reinterpret_cast<const float2*>(
-                    reinterpret_cast<const float*>(&post[((sw * 2 + my_chunk) * 2 + half) * 32 + lane]) + 2 * (warp & 1));
+                const float2 x = post[((sw * 4 + (warp >> 1)) * 2 + half) * 32 + lane];
                 a0 += x.x * f[sw];
                 a1 += x.y * f[sw];
             }
@@ -663,17 +672,16 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
             named_bar_sync(1, kConsumerWarps * 32);
         }
 
-        // ---- every warp writes its share: dims 32 rd + 16 (warp >> 2) + 4 tig + 2 (warp & 1) + {0, 1} of row g + 8 half ----
-        const int col0 = my_chunk * 16 + 4 * tig + 2 * (warp & 1), row = g + 8 * half;
+        // ---- every warp writes its share: dims 32 rd + 8 (warp >> 1) + 2 tig + {0, 1} of row g + 8 half ----
+        const int col0 = (warp >> 1) * 8 + 2 * tig, row = g + 8 * half;
         if (row < rows) {
-            const bool head_of_row = tig == 0 && (warp & 5) == 0;
             if (whole) {
                 const float inv = lt == 0.f ? 0.f : 1.f / lt;
 #pragma unroll
                 for (int rd = 0; rd < 4; ++rd)
                     *reinterpret_cast<uint32_t*>(p.o + (head0 + row) * kD + rd * 32 + col0) =
                         pack_bf16x2(acc[rd][0] * inv, acc[rd][1] * inv);
-                if (head_of_row) {
+                if (col0 == 0) {
                     const float l2 = lt == 0.f ? -INFINITY : ms - kPShift + log2f(lt);
                     if (p.lse) p.lse[head0 + row] = l2 * kLn2;
                     if (kScores) p.lse2[head0 + row] = l2;
@@ -683,7 +691,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 #pragma unroll
                 for (int rd = 0; rd < 4; ++rd)
                     *reinterpret_cast<float2*>(dst + rd * 32 + col0) = make_float2(acc[rd][0], acc[rd][1]);
-                if (head_of_row) *reinterpret_cast<float2*>(dst + kD) = make_float2(ms, lt);
+                if (col0 == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(ms, lt);
             }
         }
 
@@ -757,7 +765,7 @@ __global__ void __launch_bounds__(kWeightThreads) decode_weights_kernel(const De
     const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(h) * p.G;
     for (int g = 0; g < p.G; ++g) {
         const float l2 = __ldg(p.lse2 + head0 + g);
-        const float* src = p.scores + (head0 + g) * p.capacity;
+        const float* src = p.scores + (head0 + g) * p.score_pitch;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int t = t0 + i * kWeightThreads + threadIdx.x;
@@ -782,6 +790,8 @@ struct DecodePlan {
     size_t slot_offset, lse2_offset, score_offset, bytes;
 };
 
+static long long score_pitch(int capacity) { return (static_cast<long long>(capacity) + kTok - 1) / kTok * kTok; }
+
 static int make_decode_plan(int B, int capacity, int Hq, int Hkv, int D, bool with_weights, int num_workers, int sm_count,
                             DecodePlan* plan) {
     if (B <= 0 || capacity <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || num_workers < 0 || Hq % Hkv != 0) return CLLO_E_BAD_ARG;
@@ -800,7 +810,7 @@ static int make_decode_plan(int B, int capacity, int Hq, int Hkv, int D, bool wi
     plan->lse2_offset = plan->slot_offset + static_cast<size_t>(W) * 2 * kSlotFloats * sizeof(float);
     const size_t rows = static_cast<size_t>(B) * Hq;
     plan->score_offset = plan->lse2_offset + (with_weights ? (rows * sizeof(float) + 255) / 256 * 256 : 0);
-    plan->bytes = plan->score_offset + (with_weights ? rows * capacity * sizeof(float) : 0);
+    plan->bytes = plan->score_offset + (with_weights ? rows * score_pitch(capacity) * sizeof(float) : 0);
     return CLLO_OK;
 }
 
@@ -876,6 +886,7 @@ static int decode_launch(const void* q, const void* k, const void* v, const floa
     p.o = static_cast<__nv_bfloat16*>(o);
     p.lse = lse;
     p.scores = weights ? reinterpret_cast<float*>(ws + plan.score_offset) : nullptr;
+    p.score_pitch = score_pitch(capacity);
     p.lse2 = reinterpret_cast<float*>(ws + plan.lse2_offset);
     p.slots = reinterpret_cast<float*>(ws + plan.slot_offset);
     p.counters = reinterpret_cast<unsigned*>(ws);
