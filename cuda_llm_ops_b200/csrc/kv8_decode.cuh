@@ -73,7 +73,8 @@ constexpr int kSmemBar = kSmemQ + 2 * kQBytes;
 constexpr int kNumBars = 2 * kStages + 4;
 constexpr int kSmemScale = kSmemBar + kNumBars * 8;
 constexpr int kSmemMisc = kSmemScale + kStages * 2 * kQuarters * 4;
-constexpr int kDecodeSmemBytes = kSmemMisc + 16 + 1024;
+constexpr int kSmemShare = (kSmemMisc + 16 + 7) / 8 * 8;
+constexpr int kDecodeSmemBytes = kSmemShare + 64 + 1024;
 static_assert(kDecodeSmemBytes <= 227 * 1024, "shared memory of a block");
 // What a unit costs beyond its tiles (its query rows, the merge of the eight states, the output), in tiles.  The shares of
 // the blocks are cut in these units, so that a block that gets many short sequences is not the last one to finish: 17
@@ -135,7 +136,7 @@ struct Share {
     long long seq_lo;         // index of that sequence's first cell
 };
 
-// Every warp of the block finds the block's share for itself: two passes over the lengths, the second from L1.
+// One warp finds the block's share: two passes over the lengths, the second from L1.
 __device__ __forceinline__ Share find_share(const DecodeParams& p, int lane) {
     const int U = p.Hkv * p.n_gblk;
     Share s;
@@ -286,9 +287,15 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         *abort_flag = 0;
         fence_mbar_init();
     }
-    const Share share = find_share(p, lane);
+    // found once and kept in shared memory: what only the merge of a cut unit needs takes no registers in between
+    volatile Share& share = *reinterpret_cast<volatile Share*>(gen_base + kSmemShare);
+    if (warp == kConsumerWarps) {
+        const Share found = find_share(p, lane);
+        if (lane == 0) *reinterpret_cast<Share*>(gen_base + kSmemShare) = found;
+    }
     __syncthreads();
     const long long lo = share.lo, hi = share.hi;
+    const int cost = share.cost;
     if (lo >= hi) return;
     const int U = p.Hkv * p.n_gblk;
 
@@ -306,7 +313,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                 tma_prefetch_desc(&tm_v);
             }
             int b = share.b;
-            int n_cells = share.cost + tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
+            int n_cells = cost + tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
             const long long pos = lo - share.seq_lo;
             int unit = static_cast<int>(div_nonneg(pos, n_cells));
             int cell = static_cast<int>(pos - static_cast<long long>(unit) * n_cells);  // of the unit, next to look at
@@ -322,7 +329,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 #pragma unroll 1
             while (left > 0) {
                 const int here = static_cast<int>(left < n_cells - cell ? left : n_cells - cell);  // of this unit
-                int tile = cell - share.cost;
+                int tile = cell - cost;
                 const int tile_end = tile + here;
                 if (tile < 0) tile = 0;
                 if (tile < tile_end) {
@@ -365,7 +372,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     gblk = 0;
                     if (++kvh == p.Hkv) {
                         kvh = 0;
-                        if (++b < p.B) n_cells = share.cost + tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
+                        if (++b < p.B) n_cells = cost + tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
                     }
                 }
             }
@@ -408,7 +415,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
     int b = share.b;
     int len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
-    int n_cells = share.cost + tiles_of(len);
+    int n_cells = cost + tiles_of(len);
     int unit = static_cast<int>(div_nonneg(lo - share.seq_lo, n_cells));  // within the sequence
     long long unit_lo = share.seq_lo + static_cast<long long>(unit) * n_cells;
     bool first_unit = true;
@@ -420,10 +427,10 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
 #pragma unroll 1
     while (unit_lo < hi) {
-        const int n_t = n_cells - share.cost;
+        const int n_t = n_cells - cost;
         // this block's tiles of the unit
-        int tile = lo > unit_lo + share.cost ? static_cast<int>(lo - unit_lo) - share.cost : 0;
-        const int tile_end = hi < unit_lo + n_cells ? static_cast<int>(hi - unit_lo) - share.cost : n_t;
+        int tile = lo > unit_lo + cost ? static_cast<int>(lo - unit_lo) - cost : 0;
+        const int tile_end = hi < unit_lo + n_cells ? static_cast<int>(hi - unit_lo) - cost : n_t;
         const bool whole = tile == 0 && tile_end == n_t;
         if (tile < tile_end) {
         const int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
@@ -697,9 +704,9 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
         if (!whole) {
             // this block's piece of the unit is in the workspace: count it in; the last one to arrive merges
-            const long long W = share.W;
-            const long long w_first = block_of_cell(unit_lo + share.cost, share.T, W);
-            const long long w_last = block_of_cell(unit_lo + n_cells - 1, share.T, W);
+            const long long T = share.T, W = share.W;
+            const long long w_first = block_of_cell(unit_lo + cost, T, W);
+            const long long w_last = block_of_cell(unit_lo + n_cells - 1, T, W);
             const int n_pieces = static_cast<int>(w_last - w_first) + 1;
             unsigned* counter = p.counters + w_first;
             named_bar_sync(1, kConsumerWarps * 32);
@@ -713,7 +720,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
             named_bar_sync(1, kConsumerWarps * 32);
             if (misc[0] != 0) {
                 const int mrow = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
-                const int which_first = cell_lo(w_first, share.T, W) >= unit_lo ? 0 : 1;
+                const int which_first = cell_lo(w_first, T, W) >= unit_lo ? 0 : 1;
                 if (mrow < rows) {
                     float mg[8], mm, ll;
                     auto piece = [&](int i) {
@@ -747,7 +754,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
             unit = 0;
             if (++b >= p.B) break;
             len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
-            n_cells = share.cost + tiles_of(len);
+            n_cells = cost + tiles_of(len);
         }
     }
 }
