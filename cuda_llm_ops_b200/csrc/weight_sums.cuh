@@ -20,8 +20,8 @@
 // form per sequence.  A unit cut between blocks leaves one fp32 partial per key and block; the last block to arrive adds
 // them up in block order.
 //
-// Warps: 0-15 the exponentials, one key per thread -- warpgroups 0 and 2 key tile 0, 1 and 3 key tile 1, each 64 of a step's
-// queries: four warps per scheduler, so that one's tensor-memory load hides behind the others' exponentials -- 16 TMA
+// Warps: 0-15 the exponentials, one key per thread -- warpgroups 0 and 2 key tile 0, 1 and 3 key tile 1, taking its
+// steps in turn: four warps per scheduler, so that one's tensor-memory load hides behind the others' exponentials -- 16 TMA
 // producer, 17 MMA issuer, 18 lse loader, 19 idle.
 // Tensor memory: two 128-column accumulators per key tile.  Shared memory: K 3 x 32 KB (the next unit's first keys arrive
 // during this one's steps), Q 3 x 32 KB (with two the copies' latency showed), lse 16 x 512 B (eight steps on their way).
@@ -37,8 +37,8 @@ namespace sums {
 constexpr int kD = 128;
 constexpr int kKeys = 128, kTiles = 2, kPair = kKeys * kTiles;  // keys per tile and unit
 constexpr int kQ = 128;                                          // queries per step
-constexpr int kHalves = 2;                                       // warpgroups per key tile: 64 queries of a step each
-constexpr int kEpiWarps = kTiles * kHalves * 4;
+constexpr int kTurns = 2;                                        // warpgroups per key tile: they take its steps in turn
+constexpr int kEpiWarps = kTiles * kTurns * 4;
 constexpr int kThreads = (kEpiWarps + 4) * 32;
 constexpr int kUnitCost = 2;
 constexpr int kSlabBytes = 128 * 128;         // [128 rows][64 dims] bf16, one swizzled slab
@@ -49,7 +49,7 @@ constexpr int kSmemQ = kKStages * kTileBytes;
 constexpr int kSmemLse = kSmemQ + kQStages * kTileBytes;
 constexpr int kSmemBar = kSmemLse + kLseStages * kQ * 4;
 constexpr int kNumBars = 2 * kKStages + 2 * kQStages + 2 * kLseStages + 4 * kTiles + 1;
-constexpr int kSmemHalf = kSmemBar + kNumBars * 8;  // the second half's sum of every key
+constexpr int kSmemHalf = kSmemBar + kNumBars * 8;  // the second warpgroup's sum of every key
 constexpr int kSmemMisc = kSmemHalf + kPair * 4;
 constexpr int kSmemBytes = kSmemMisc + 32 + 1024;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -266,7 +266,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         for (int t = 0; t < sums::kTiles; ++t)
             for (int s = 0; s < 2; ++s) {
                 mbar_init(d_full(t, s), 1);
-                mbar_init(d_empty(t, s), 4 * kHalves);
+                mbar_init(d_empty(t, s), 4);
             }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -450,18 +450,20 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         while (got < put) hand_over();
     } else if (warp < kEpiWarps) {
         // ------------------------- exponentials and sums (one key per thread) -------------------------
-        const int t = (warp >> 2) & 1, half = warp >> 3;
+        // warpgroup 2 * turn + t: key tile t, those of its steps whose product lands in accumulator `turn`
+        const int t = (warp >> 2) & 1, turn = warp >> 3;
         const int key_in_pair = threadIdx.x & (kPair - 1);
         float* other = reinterpret_cast<float*>(gen_base + sums::kSmemHalf);
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        int ls = 0, dsl = 0;
+        const uint32_t acc = tmem_base + lane_base + (t * 2 + turn) * kQ;
+        int ls = 0, next_turn = 0;
         uint32_t lp = 0, dph = 0;
         for (; !w.done(); w.next(p)) {
             const int key = w.p * kPair + key_in_pair;
             float* out = p.out + (static_cast<long long>(w.b) * p.Hkv + w.kvh) * p.Skv + key;
             if (!w.active()) {
                 // a unit without steps: whoever holds its first cell clears its sums
-                if (half == 0 && w.steps == 0 && w.unit_lo >= w.lo && key < p.Skv && !p.accumulate) *out = 0.f;
+                if (turn == 0 && w.steps == 0 && w.unit_lo >= w.lo && key < p.Skv && !p.accumulate) *out = 0.f;
                 continue;
             }
             float total = 0.f;
@@ -474,20 +476,21 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             // the first column of tile 0 that this key sees; without a causal mask every one, for all keys of a warp alike
             const int own = p.causal ? ahead + static_cast<int>(threadIdx.x & (kKeys - 1)) : lane - 31;
             const float scale = p.scale_log2;
-            const float* lse_half = lse_buf + half * (kQ / kHalves);
-            const uint32_t acc = tmem_base + lane_base + t * 2 * kQ + half * (kQ / kHalves);
             int j = w.s_lo % w.n;
 #pragma unroll 1
             for (int left = w.s_hi - w.s_lo; left > 0; --left) {
                 mbar_wait_idle(lse_full(ls), lp, abort_flag, SITE_SUMS_LSE, ls);
-                if (j >= j_sees) {
-                    mbar_wait_idle(d_full(t, dsl), dph, abort_flag, SITE_SUMS_D, t);
+                const bool mine = j >= j_sees && next_turn == turn;
+                if (j >= j_sees) next_turn ^= 1;
+                if (mine) {
+                    mbar_wait_idle(d_full(t, turn), dph, abort_flag, SITE_SUMS_D, t);
+                    dph ^= 1u;
                     __syncwarp();
                     tc_fence_after();
-                    const float* nl = lse_half + ls * kQ;
+                    const float* nl = lse_buf + ls * kQ;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    // columns of this warpgroup's share that count: from the warp's keys' own first ones up to i_hi
-                    const int lo = own - j * kQ - half * (kQ / kHalves), hi = rows - j * kQ - half * (kQ / kHalves);
+                    // columns that count: from the warp's keys' own first ones up to i_hi
+                    const int lo = own - j * kQ, hi = rows - j * kQ;
                     const int lo_first = lo - lane, lo_last = lo_first + 31;  // of the warp's lowest and highest key
                     auto add_chunk = [&](const float (&x)[32], const float* l) {
 #pragma unroll
@@ -499,19 +502,19 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                             sum[3] += fast_exp2(fmaf(x[e + 3], scale, l4.w));
                         }
                     };
-                    if (lo_last <= 0 && hi >= kQ / kHalves) {
+                    if (lo_last <= 0 && hi >= kQ) {
 #pragma unroll
-                        for (int c = 0; c < kQ / kHalves; c += 32) {
+                        for (int c = 0; c < kQ; c += 32) {
                             float x[32];
-                            tmem_ld32_wait(acc + dsl * kQ + c, x);
+                            tmem_ld32_wait(acc + c, x);
                             add_chunk(x, nl + c);
                         }
                     } else {
 #pragma unroll 1
-                        for (int c = 0; c < kQ / kHalves; c += 32) {
+                        for (int c = 0; c < kQ; c += 32) {
                             if (c >= hi || lo_first >= c + 32) continue;  // nothing for any key of the warp
                             float x[32];
-                            tmem_ld32_wait(acc + dsl * kQ + c, x);
+                            tmem_ld32_wait(acc + c, x);
                             if (lo_last <= c && hi >= c + 32) {
                                 add_chunk(x, nl + c);
                                 continue;
@@ -528,8 +531,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(d_empty(t, dsl));
-                    if ((dsl ^= 1) == 0) dph ^= 1u;
+                    if (lane == 0) mbar_arrive(d_empty(t, turn));
                     total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 }
                 __syncwarp();
@@ -541,17 +543,17 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 if (++j == w.n) j = 0;
             }
             if (key >= w.seq.len) total = 0.f;  // whatever lies behind the sequence
-            // the two halves of a key meet; the barrier also keeps the next unit's value out until this one has been read
-            if (half == 1) other[key_in_pair] = total;
+            // the two warpgroups' sums of a key meet; the barrier also keeps the next unit's value out until this one has been read
+            if (turn == 1) other[key_in_pair] = total;
             named_bar_sync(1, kEpiThreads);
-            if (half == 0) total += other[key_in_pair];
+            if (turn == 0) total += other[key_in_pair];
             named_bar_sync(1, kEpiThreads);
             if (w.s_lo == 0 && w.s_hi == w.steps) {
-                if (half == 0 && key < p.Skv) *out = p.accumulate ? *out + total : total;
+                if (turn == 0 && key < p.Skv) *out = p.accumulate ? *out + total : total;
                 continue;
             }
             // this block's part of the unit goes to the workspace; the last block to arrive adds the parts up
-            if (half == 0) p.slots[(static_cast<long long>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * kPair + key_in_pair] = total;
+            if (turn == 0) p.slots[(static_cast<long long>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * kPair + key_in_pair] = total;
             const long long w_first = worker_of_tile(w.unit_lo + kUnitCost, w.T, w.W);
             const long long w_last = worker_of_tile(w.unit_lo + kUnitCost + w.steps - 1, w.T, w.W);
             const int n_pieces = static_cast<int>(w_last - w_first) + 1;
@@ -565,7 +567,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 *misc = last ? 1 : 0;
             }
             named_bar_sync(1, kEpiThreads);
-            if (*misc != 0 && half == 0) {
+            if (*misc != 0 && turn == 0) {
                 const int which_first = worker_lo(w_first, w.T, w.W) >= w.unit_lo ? 0 : 1;
                 float sum = 0.f;
                 for (int i = 0; i < n_pieces; ++i)
