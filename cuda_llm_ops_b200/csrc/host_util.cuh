@@ -113,6 +113,20 @@ static int encode_bf16_4d(CUtensorMap* map, const void* base, const uint64_t dim
     return CLLO_OK;
 }
 
+// Launch configuration of a kernel that may become resident while the one before it in the stream still runs (it waits for
+// that one's end by pdl_wait_prior_grid).  `attr` has to live as long as the configuration.
+static inline cudaLaunchConfig_t dependent_launch(cudaLaunchAttribute* attr, unsigned blocks, unsigned threads, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr->val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+
 static inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 }  // namespace cllo

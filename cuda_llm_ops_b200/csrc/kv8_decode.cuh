@@ -274,6 +274,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     auto q_full_bar = [&](int s) { return bar_base + (2 * kStages + s) * 8; };
     auto q_empty_bar = [&](int s) { return bar_base + (2 * kStages + 2 + s) * 8; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (kScores) pdl_launch_dependents();  // the weights kernel's blocks may take their places; they wait for this grid's end
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -762,6 +763,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 // weights[b, h, t] += sum over the group's heads, in order, of 2^(score - lse2); one thread per token
 constexpr int kWeightThreads = 256, kWeightTok = 1024;
 __global__ void __launch_bounds__(kWeightThreads) decode_weights_kernel(const DecodeParams p, float* weights, int n_chunks) {
+    pdl_wait_prior_grid();  // scores and normalisers; by every block, so that this grid never ends before the decode's
     const int chunk = blockIdx.x % n_chunks, row = blockIdx.x / n_chunks;  // row = (b, h)
     const int b = row / p.Hkv, h = row - b * p.Hkv;
     const int len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
@@ -919,8 +921,9 @@ static int decode_launch(const void* q, const void* k, const void* v, const floa
         rc = weights ? decode_launch_kernel<CLLO_FMT_INT8, true>(tm_k, tm_v, p, plan.W, attr + 2, st)
                      : decode_launch_kernel<CLLO_FMT_INT8, false>(tm_k, tm_v, p, plan.W, attr + 3, st);
     if (rc != CLLO_OK || !weights) return rc;
-    decode_weights_kernel<<<static_cast<unsigned>(weight_blocks), kWeightThreads, 0, st>>>(p, weights, n_chunks);
-    CLLO_CUDA_TRY(cudaGetLastError());
+    cudaLaunchAttribute dependent;
+    const cudaLaunchConfig_t cfg = dependent_launch(&dependent, static_cast<unsigned>(weight_blocks), kWeightThreads, st);
+    CLLO_CUDA_TRY(cudaLaunchKernelEx(&cfg, decode_weights_kernel, p, weights, n_chunks));
     return CLLO_OK;
 }
 

@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
     __shared__ int warp_sum[kSelectThreads / 32];
     __shared__ int s_digit, s_need;
     __shared__ int s_counts[2];  // this block's tokens that stay whatever the others hold, and those at the threshold
+    pdl_launch_dependents();  // the moving blocks may take their places; they wait for this grid's end
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int C = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
     const int row = blockIdx.x / C;
@@ -266,6 +267,7 @@ template <int kFmt, int kBlock>
 __global__ void __launch_bounds__(gather_threads(kBlock)) gather_kernel(const EvictParams p) {
     constexpr int kThreads = gather_threads(kBlock);
     __shared__ float warp_amax[2][kThreads / 32];
+    pdl_wait_prior_grid();  // the positions; by every block, so that this grid never ends before the one that writes them
     // kv heads next to each other: with tokens before heads in memory they share DRAM pages
     const int h = blockIdx.x % p.Hkv, at = blockIdx.x / p.Hkv;
     const int b = at / p.n_blocks_to, blk = at % p.n_blocks_to, row = b * p.Hkv + h;
@@ -364,12 +366,14 @@ __global__ void __launch_bounds__(gather_threads(kBlock)) gather_kernel(const Ev
 }
 
 template <int kFmt>
-static void gather_dispatch(const EvictParams& p, int block, unsigned grid, cudaStream_t st) {
+static cudaError_t gather_dispatch(const EvictParams& p, int block, unsigned grid, cudaStream_t st) {
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = dependent_launch(&attr, grid, static_cast<unsigned>(gather_threads(block)), st);
     switch (block) {
-        case 16: gather_kernel<kFmt, 16><<<grid, gather_threads(16), 0, st>>>(p); break;
-        case 32: gather_kernel<kFmt, 32><<<grid, gather_threads(32), 0, st>>>(p); break;
-        case 64: gather_kernel<kFmt, 64><<<grid, gather_threads(64), 0, st>>>(p); break;
-        default: gather_kernel<kFmt, 128><<<grid, gather_threads(128), 0, st>>>(p); break;
+        case 16: return cudaLaunchKernelEx(&cfg, gather_kernel<kFmt, 16>, p);
+        case 32: return cudaLaunchKernelEx(&cfg, gather_kernel<kFmt, 32>, p);
+        case 64: return cudaLaunchKernelEx(&cfg, gather_kernel<kFmt, 64>, p);
+        default: return cudaLaunchKernelEx(&cfg, gather_kernel<kFmt, 128>, p);
     }
 }
 
@@ -459,11 +463,7 @@ static int evict_launch(const void* k, const void* v, const float* k_scale, cons
     cfg.numAttrs = 1;
     CLLO_CUDA_TRY(cudaLaunchKernelEx(&cfg, select_kernel, p));
     const unsigned grid = static_cast<unsigned>(blocks);
-    if (format == CLLO_FMT_E4M3)
-        gather_dispatch<CLLO_FMT_E4M3>(p, block, grid, st);
-    else
-        gather_dispatch<CLLO_FMT_INT8>(p, block, grid, st);
-    CLLO_CUDA_TRY(cudaGetLastError());
+    CLLO_CUDA_TRY((format == CLLO_FMT_E4M3 ? gather_dispatch<CLLO_FMT_E4M3> : gather_dispatch<CLLO_FMT_INT8>)(p, block, grid, st));
     return CLLO_OK;
 }
 
