@@ -257,12 +257,12 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
     cluster_sync();  // no block leaves while another may still read its counts
 }
 
-// eight lanes per row, two rows of K and of V per lane
+// four lanes per row, 32 bytes of K and of V per lane
 __host__ __device__ constexpr int gather_threads(int block) { return block * 4; }
 
-// One thread block per block of the second cache: K and V rows of its tokens, 16 bytes per lane and eight lanes per row, all
-// loads in flight before the first is looked at; values -> amax -> new scale -> codes.  Bound by memory: 2 x 128 bytes read
-// and written per token.
+// One thread block per block of the second cache, one row per four lanes: all loads in flight before the first is looked at;
+// values -> amax -> new scale -> codes.  Bound by the latency of its gathers (position, then 128-byte rows) and by issue: what
+// a row costs besides its values (addresses, scales) is as much as the values cost, so a lane takes 32 bytes of each.
 template <int kFmt, int kBlock>
 __global__ void __launch_bounds__(gather_threads(kBlock)) gather_kernel(const EvictParams p) {
     constexpr int kThreads = gather_threads(kBlock);
@@ -275,59 +275,45 @@ __global__ void __launch_bounds__(gather_threads(kBlock)) gather_kernel(const Ev
     const int kept = len < p.budget ? len : p.budget;
     const int j0 = blk * kBlock;
     if (j0 >= kept) return;
-    const int* idx = p.indices + static_cast<long long>(row) * p.budget;
-    constexpr int kRowsPerStep = kThreads / 8, kSteps = kBlock / kRowsPerStep;
-    const int r_in = threadIdx.x >> 3, c16 = (threadIdx.x & 7) * 16;
-    int t[kSteps];
+    const int j = j0 + (threadIdx.x >> 2), c32 = (threadIdx.x & 3) * 32;
+    const bool live = j < kept;
+    uint4 c[2][2];
+    float s[2] = {0.f, 0.f};
+    c[0][0] = c[0][1] = c[1][0] = c[1][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (live) {
+        const int t = __ldcg(p.indices + static_cast<long long>(row) * p.budget + j);
+        const long long from = b * p.stride_from.batch + h * p.stride_from.head + t * p.stride_from.token + c32;
+        const long long scale_at = static_cast<long long>(row) * p.n_blocks_from + (t >> p.block_shift);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const int j = j0 + i * kRowsPerStep + r_in;
-        t[i] = j < kept ? __ldcg(idx + j) : -1;
-    }
-    uint4 c[2][kSteps];
-    float s[2][kSteps];
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        const uint8_t* from = p.from[which] + b * p.stride_from.batch + h * p.stride_from.head + c16;
-        const float* scale_from = p.scale_from[which] + static_cast<long long>(row) * p.n_blocks_from;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            c[which][i] = make_uint4(0u, 0u, 0u, 0u);
-            s[which][i] = 0.f;
-            if (t[i] >= 0) {
-                c[which][i] = __ldg(reinterpret_cast<const uint4*>(from + t[i] * p.stride_from.token));
-                s[which][i] = __ldg(scale_from + (t[i] >> p.block_shift));
-            }
+        for (int which = 0; which < 2; ++which) {
+            const uint4* src = reinterpret_cast<const uint4*>(p.from[which] + from);
+            c[which][0] = __ldg(src);
+            c[which][1] = __ldg(src + 1);
+            s[which] = __ldg(p.scale_from[which] + scale_at);
         }
-    }
-    if (p.weights_to && (threadIdx.x & 7) == 0) {
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-            if (t[i] >= 0)
-                p.weights_to[static_cast<long long>(row) * p.capacity_to + j0 + i * kRowsPerStep + r_in] =
-                    __ldg(p.weights + static_cast<long long>(row) * p.capacity + t[i]);
+        if (p.weights_to && (threadIdx.x & 3) == 0)
+            p.weights_to[static_cast<long long>(row) * p.capacity_to + j] =
+                __ldg(p.weights + static_cast<long long>(row) * p.capacity + t);
     }
     // codes -> f16 pairs, which hold them exactly; the rows' largest magnitudes times their scales give the block's
-    uint32_t f[2][kSteps][8];
+    uint32_t f[2][16];
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-        float amax = 0.f;
+        const uint32_t w[8] = {c[which][0].x, c[which][0].y, c[which][0].z, c[which][0].w,
+                               c[which][1].x, c[which][1].y, c[which][1].z, c[which][1].w};
+        uint32_t top = 0u;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const uint32_t w[4] = {c[which][i].x, c[which][i].y, c[which][i].z, c[which][i].w};
-            uint32_t top = 0u;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                decode4_f16<kFmt>(w[k], f[which][i][2 * k], f[which][i][2 * k + 1]);
-                top = max_f16x2(top, max_f16x2(f[which][i][2 * k] & 0x7fff7fffu, f[which][i][2 * k + 1] & 0x7fff7fffu));
-            }
-            amax = fmaxf(amax, finite_abs(f16_max_of_pair(top) * s[which][i]));  // a NaN does not take part
+        for (int k = 0; k < 8; ++k) {
+            decode4_f16<kFmt>(w[k], f[which][2 * k], f[which][2 * k + 1]);
+            top = max_f16x2(top, max_f16x2(f[which][2 * k] & 0x7fff7fffu, f[which][2 * k + 1] & 0x7fff7fffu));
         }
+        float amax = finite_abs(f16_max_of_pair(top) * s[which]);  // a NaN does not take part
 #pragma unroll
         for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         if ((threadIdx.x & 31) == 0) warp_amax[which][threadIdx.x >> 5] = amax;
     }
     __syncthreads();
+    const long long to = b * p.stride_to.batch + h * p.stride_to.head + j * p.stride_to.token + c32;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         float amax = 0.f;
@@ -335,33 +321,31 @@ __global__ void __launch_bounds__(gather_threads(kBlock)) gather_kernel(const Ev
         for (int i = 0; i < kThreads / 32; ++i) amax = fmaxf(amax, warp_amax[which][i]);
         const int e_new = scale_exp<kFmt>(amax);
         const float inv = exp2_int(-e_new);
-        uint8_t* to = p.to[which] + b * p.stride_to.batch + h * p.stride_to.head + c16;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            if (t[i] < 0) continue;
-            uint32_t d[4];
-            // Scales are powers of two: the code times their ratio is exact in f16 where it can still round to a code other
-            // than zero, so one rounding, to the new code, is all there is.  A ratio beyond f16 (a block of nothing but
-            // codes at the very bottom of e4m3) or scales that are no powers of two go through fp32.
-            const float ratio = s[which][i] * inv;
-            if ((__float_as_uint(ratio) & 0x7fffffu) == 0u && fabsf(ratio) <= 32768.f) {
-                const uint32_t r = pack_f16x2(ratio, ratio);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) d[k] = requant4<kFmt>(f[which][i][2 * k], f[which][i][2 * k + 1], r);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float v[4];
-                    f16x2_to_f32(f[which][i][2 * k], v[0], v[1]);
-                    f16x2_to_f32(f[which][i][2 * k + 1], v[2], v[3]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = v[e] * s[which][i] * inv;
-                    d[k] = encode4<kFmt>(v[0], v[1], v[2], v[3]);
-                }
-            }
-            *reinterpret_cast<uint4*>(to + (j0 + i * kRowsPerStep + r_in) * p.stride_to.token) = make_uint4(d[0], d[1], d[2], d[3]);
-        }
         if (threadIdx.x == 0) p.scale_to[which][static_cast<long long>(row) * p.n_blocks_to + blk] = exp2_int(e_new);
+        if (!live) continue;
+        uint32_t d[8];
+        // Scales are powers of two: the code times their ratio is exact in f16 where it can still round to a code other than
+        // zero, so one rounding, to the new code, is all there is.  A ratio beyond f16 (a block of nothing but codes at the
+        // very bottom of e4m3) or scales that are no powers of two go through fp32.
+        const float ratio = s[which] * inv;
+        if ((__float_as_uint(ratio) & 0x7fffffu) == 0u && fabsf(ratio) <= 32768.f) {
+            const uint32_t r = pack_f16x2(ratio, ratio);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) d[k] = requant4<kFmt>(f[which][2 * k], f[which][2 * k + 1], r);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                float v[4];
+                f16x2_to_f32(f[which][2 * k], v[0], v[1]);
+                f16x2_to_f32(f[which][2 * k + 1], v[2], v[3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = v[e] * s[which] * inv;
+                d[k] = encode4<kFmt>(v[0], v[1], v[2], v[3]);
+            }
+        }
+        uint4* dst = reinterpret_cast<uint4*>(p.to[which] + to);
+        dst[0] = make_uint4(d[0], d[1], d[2], d[3]);
+        dst[1] = make_uint4(d[4], d[5], d[6], d[7]);
     }
 }
 
