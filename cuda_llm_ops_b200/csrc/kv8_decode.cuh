@@ -73,7 +73,7 @@ constexpr int kSmemBar = kSmemQ + 2 * kQBytes;
 constexpr int kNumBars = 2 * kStages + 4;
 constexpr int kSmemScale = kSmemBar + kNumBars * 8;
 constexpr int kSmemMisc = kSmemScale + kStages * 2 * kQuarters * 4;
-constexpr int kSmemShare = (kSmemMisc + 16 + 7) / 8 * 8;
+constexpr int kSmemShare = kSmemMisc + 32;
 constexpr int kDecodeSmemBytes = kSmemShare + 64 + 1024;
 static_assert(kDecodeSmemBytes <= 227 * 1024, "shared memory of a block");
 // What a unit costs beyond its tiles (its query rows, the merge of the eight states, the output), in tiles.  The shares of
@@ -81,8 +81,17 @@ static_assert(kDecodeSmemBytes <= 227 * 1024, "shared memory of a block");
 // sequences of 0 to 16384 tokens, 8 kv heads: 81 us at 0, 61 at 4, 55 at 6, 49 at 12, 53 at 16; no effect on full batches.
 // Held to the tiles that a block gets on average: where there are fewer than that, spreading the tiles comes first.
 constexpr int kUnitCost = 10;
+// A unit that many blocks share (one long sequence, few kv heads) is merged in two steps, kFan pieces each: one block that
+// reads 148 pieces of 16 rows takes longer than the attention (16384 tokens of one kv head, 148 blocks: 41 us in one
+// step, 22.5 in two).  Up to kFlatPieces one step is as fast: the second costs another round of arrivals.
+constexpr int kFlatPieces = 24, kFan = 12;
+constexpr int kMaxWorkers = 512;  // two sets of arrival counters in the first 4 KB of the workspace
+static_assert(2 * kMaxWorkers <= decode::kFixedCounters, "the counters' place in the workspace");
 constexpr float kLazy = 4.f;                 // a reference may lag behind the true maximum by this much (log2)
 constexpr float kPShift = 15.f - kLazy;      // p' <= 2^15
+// A V scale of 0 (a block that nothing was written to, all codes 0) has no logarithm and no reciprocal; 2^-80 keeps the sum of
+// 2^30 tokens' p' / vscale inside fp32.
+constexpr float kMinVScale = 8.271806e-25f;
 constexpr float kMinFactor = 7.888609e-31f;  // 2^-100: a score is at most 2^31 times its factor, so this much is nothing
 static_assert(kStages % kGroups == 0, "a stage buffer must always belong to the same consumer group");
 
@@ -107,67 +116,71 @@ struct DecodeParams {
 // tiles of a sequence; an empty one has one, so that its output is written
 __device__ __forceinline__ int tiles_of(int len) { return len <= 0 ? 1 : (len + kTok - 1) / kTok; }
 
-// a / b for non-negative values; most of them fit 32 bits, where a division costs a quarter
-__device__ __forceinline__ long long div_nonneg(long long a, long long b) {
-    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-    return a / b;
-}
-// the cells [cell_lo(w), cell_lo(w + 1)) of block w, and the block that holds cell c
-__device__ __forceinline__ long long cell_lo(long long w, long long T, long long W) { return div_nonneg(w * T, W); }
-__device__ __forceinline__ long long block_of_cell(long long c, long long T, long long W) {
-    return div_nonneg((c + 1) * W - 1, T);
+// The cells [cell_lo(w), cell_lo(w + 1)) of block w, cell_lo(w) = floor(w T / W), and the block that holds cell c.  T is below
+// 2^31 and W at most kMaxWorkers, so that all but the second's product fits 32 bits.
+__device__ __forceinline__ int cell_lo(int w, int T, int W) { return w * (T / W) + w * (T % W) / W; }
+__device__ __forceinline__ int block_of_cell(int c, int T, int W) {
+    const unsigned long long x = (c + 1ull) * W - 1;
+    return static_cast<int>(x >> 32 == 0 ? static_cast<uint32_t>(x) / T : x / T);
 }
 
-// sum over the warp's 32 lanes and inclusive prefix
-__device__ __forceinline__ long long warp_incl_sum(long long v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-    }
-    return v;
+// counts an arrival: what this block wrote before is visible to whoever counts later, what the others wrote to this block
+__device__ __forceinline__ unsigned atomic_inc_acq_rel(unsigned* p) {
+    unsigned old;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+    return old;
 }
 
 // The index space that the blocks share: per unit `cost` cells without a tile, then one cell per tile.
 struct Share {
-    long long T, W, lo, hi;   // all cells, blocks that take part, this block's range
+    int T, W, lo, hi;  // all cells, blocks that take part, this block's range
     int cost;
-    int b;                    // the sequence that holds cell lo
-    long long seq_lo;         // index of that sequence's first cell
+    int b, len;        // the sequence that holds cell lo, and its tokens
+    int unit, unit_lo; // the unit of that sequence that does, and the index of its first cell
 };
 
-// One warp finds the block's share: two passes over the lengths, the second from L1.
+// One warp finds the block's share: two passes over the lengths, the second from registers or L1.
 __device__ __forceinline__ Share find_share(const DecodeParams& p, int lane) {
-    const int U = p.Hkv * p.n_gblk;
+    const int U = p.Hkv * p.n_gblk, grid = static_cast<int>(gridDim.x);
+    const int len0 = lane < p.B ? clamp_len(__ldg(p.seq_lens + lane), p.capacity) : 0;  // of the first 32 sequences
+    auto len_of = [&](int i) { return i < 32 ? len0 : clamp_len(__ldg(p.seq_lens + i), p.capacity); };
     Share s;
-    long long tiles = 0;
-    for (int i = lane; i < p.B; i += 32) tiles += tiles_of(clamp_len(__ldg(p.seq_lens + i), p.capacity));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-    const long long per_block = div_nonneg(tiles * U, gridDim.x);
-    s.cost = per_block < kUnitCost ? static_cast<int>(per_block) : kUnitCost;
-    s.T = (tiles + static_cast<long long>(s.cost) * p.B) * U;
+    int tiles = 0;
+    for (int i = lane; i < p.B; i += 32) tiles += tiles_of(len_of(i));
+    tiles = __reduce_add_sync(0xffffffffu, tiles);
+    s.cost = tiles * U >= kUnitCost * grid ? kUnitCost : tiles * U / grid;
+    s.T = (tiles + s.cost * p.B) * U;
     // no more blocks than cells: every block between the first and the last tile of a unit then holds some of its tiles,
     // which the count of pieces relies on
-    s.W = gridDim.x < s.T ? gridDim.x : s.T;
+    s.W = grid < s.T ? grid : s.T;
     s.lo = s.hi = 0;
-    if (blockIdx.x < s.W) {
-        s.lo = cell_lo(blockIdx.x, s.T, s.W);
-        s.hi = cell_lo(blockIdx.x + 1, s.T, s.W);
-    }
-    s.b = 0;
-    s.seq_lo = 0;
+    s.b = s.len = s.unit = s.unit_lo = 0;
+    const int w = static_cast<int>(blockIdx.x);
+    if (w >= s.W) return s;
+    const int edge = cell_lo(w + (lane & 1), s.T, s.W);  // both ends at once
+    s.lo = __shfl_sync(0xffffffffu, edge, 0);
+    s.hi = __shfl_sync(0xffffffffu, edge, 1);
     if (s.lo >= s.hi) return s;
-    long long before = 0;
+    int before = 0;
     for (int i0 = 0; i0 < p.B; i0 += 32) {
         const int i = i0 + lane;
-        const long long n = i < p.B ? static_cast<long long>(s.cost + tiles_of(clamp_len(__ldg(p.seq_lens + i), p.capacity))) * U : 0;
-        const long long end = before + warp_incl_sum(n, lane);
+        const int len = i < p.B ? len_of(i) : 0;
+        const int n = i < p.B ? (s.cost + tiles_of(len)) * U : 0;
+        int end = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end += u;
+        }
+        end += before;
         const unsigned holds = __ballot_sync(0xffffffffu, s.lo < end);
         if (holds) {
             const int at = __ffs(holds) - 1;
             s.b = i0 + at;
-            s.seq_lo = __shfl_sync(0xffffffffu, end - n, at);
+            s.len = __shfl_sync(0xffffffffu, len, at);
+            const int seq_lo = __shfl_sync(0xffffffffu, end - n, at), n_cells = s.cost + tiles_of(s.len);
+            s.unit = (s.lo - seq_lo) / n_cells;
+            s.unit_lo = seq_lo + s.unit * n_cells;
             break;
         }
         before = __shfl_sync(0xffffffffu, end, 31);
@@ -206,15 +219,27 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
+// log2 of a normal positive x, exact for powers of two: the exponent apart, the approximation sees [1, 2) only
 __device__ __forceinline__ float log2_approx(float x) {
+    const uint32_t bits = __float_as_uint(x);
     float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u)));
+    return y + static_cast<float>(static_cast<int>(bits >> 23) - 127);
 }
 __device__ __forceinline__ float rcp_approx(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// log2 of the softmax's normaliser, m - kPShift + log2(l).  Small V scales make m small and l large: l's exponent is added to m
+// first, which leaves no rounding at the size of either.
+__device__ __forceinline__ float log2_of_sum(float m, float l) {
+    if (l == 0.f) return -INFINITY;
+    const uint32_t bits = __float_as_uint(l);
+    const int e = static_cast<int>(bits >> 23 & 0xffu) - 127;
+    if (e == 128) return l;  // infinite or NaN
+    return (m + (static_cast<float>(e) - kPShift)) + log2f(__uint_as_float((bits & 0x7fffffu) | 0x3f800000u));
 }
 
 // log-sum-exp merge of the pieces of one unit, 8 columns of one row per thread; pieces in worker order
@@ -269,6 +294,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     const uint32_t bar_base = base + kSmemBar;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + kSmemMisc);
     volatile int* misc = abort_flag + 1;
+    volatile int* pieces = misc + 1;  // of a cut unit: the first block that holds some, their number, the first one's slot
     auto full_bar = [&](int s) { return bar_base + s * 8; };
     auto empty_bar = [&](int s) { return bar_base + (kStages + s) * 8; };
     auto q_full_bar = [&](int s) { return bar_base + (2 * kStages + s) * 8; };
@@ -276,49 +302,33 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (kScores) pdl_launch_dependents();  // the weights kernel's blocks may take their places; they wait for this grid's end
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(full_bar(s), 1 + 2 * kQuarters);  // the tile copy and the eight scale copies
-            mbar_init(empty_bar(s), kWarpsPerGroup);
-        }
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(q_full_bar(s), 1);
-            mbar_init(q_empty_bar(s), kConsumerWarps);
-        }
-        *abort_flag = 0;
-        fence_mbar_init();
-    }
     // found once and kept in shared memory: what only the merge of a cut unit needs takes no registers in between
     volatile Share& share = *reinterpret_cast<volatile Share*>(gen_base + kSmemShare);
-    if (warp == kConsumerWarps) {
-        const Share found = find_share(p, lane);
-        if (lane == 0) *reinterpret_cast<Share*>(gen_base + kSmemShare) = found;
-    }
-    __syncthreads();
-    const long long lo = share.lo, hi = share.hi;
-    const int cost = share.cost;
-    if (lo >= hi) return;
     const int U = p.Hkv * p.n_gblk;
 
     if (warp >= kConsumerWarps) {
+        // The registers are given away, and the tensor maps fetched, while the consumers' first warps find the share and set up
+        // the barriers: giving them away afterwards put 2000 cycles between the share and the first copy.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+        if (warp == kConsumerWarps && lane == 0) {
+            tma_prefetch_desc(&tm_k);
+            tma_prefetch_desc(&tm_v);
+        }
+        named_bar_sync(2, kDecodeThreads);
+        const int lo = share.lo, hi = share.hi, cost = share.cost;
+        if (lo >= hi) return;
         // ------------------------------ producers ------------------------------
         // One warp per consumer group, each with the group's own three stages: a wait, two tile copies and the scale copies
         // take the issuing thread about as long as a block at full bandwidth has for two tiles, so one producer for all
         // groups was what bounded the kernel.  Lane 0 copies the tiles, lanes 0-7 one block scale each (a quarter's K or V
-        // scale); their arrivals are part of the stage's full barrier.  The first producer also brings the query rows.
+        // scale); their arrivals are part of the stage's full barrier.  The last producer also brings the query rows, its lanes
+        // in turn: on the way to the first tile they would be as long as the tile's own copies.
         const int grp = warp - kConsumerWarps;
         if (lane < 2 * kQuarters) {
-            if (lane == 0) {
-                tma_prefetch_desc(&tm_k);
-                tma_prefetch_desc(&tm_v);
-            }
             int b = share.b;
-            int n_cells = cost + tiles_of(clamp_len(__ldg(p.seq_lens + b), p.capacity));
-            const long long pos = lo - share.seq_lo;
-            int unit = static_cast<int>(div_nonneg(pos, n_cells));
-            int cell = static_cast<int>(pos - static_cast<long long>(unit) * n_cells);  // of the unit, next to look at
-            int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
+            int n_cells = cost + tiles_of(share.len);
+            int cell = lo - share.unit_lo;  // of the unit, next to look at
+            int kvh = share.unit / p.n_gblk, gblk = share.unit - kvh * p.n_gblk;
             int slot = grp, q_slot = 0;
             uint32_t phase = 0, q_phase = 0;
             int turn = 0;  // the group whose turn the next tile is
@@ -326,21 +336,21 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
             const float* scales = lane < kQuarters ? p.k_scale : p.v_scale;
             const int quarter = lane % kQuarters;
             const uint32_t scale_dst = base + kSmemScale + lane * 4;
-            long long left = hi - lo;  // cells of this block's range still ahead
+            int left = hi - lo;  // cells of this block's range still ahead
 #pragma unroll 1
             while (left > 0) {
-                const int here = static_cast<int>(left < n_cells - cell ? left : n_cells - cell);  // of this unit
+                const int here = left < n_cells - cell ? left : n_cells - cell;  // of this unit
                 int tile = cell - cost;
                 const int tile_end = tile + here;
                 if (tile < 0) tile = 0;
                 if (tile < tile_end) {
                     const int n_here = tile_end - tile;
-                    if (grp == 0 && lane == 0) {
+                    if (grp == kGroups - 1) {
                         const int rows = (p.G - gblk * kRows) < kRows ? (p.G - gblk * kRows) : kRows;
                         const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(kvh) * p.G + gblk * kRows;
                         mbar_wait_idle(q_empty_bar(q_slot), q_phase ^ 1u, abort_flag, SITE_KV8_Q_EMPTY, q_slot);
-                        mbar_arrive_expect_tx(q_full_bar(q_slot), rows * kD * 2);
-                        for (int r = 0; r < rows; ++r)
+                        if (lane == 0) mbar_arrive_expect_tx(q_full_bar(q_slot), rows * kD * 2);
+                        for (int r = lane; r < rows; r += 2 * kQuarters)
                             bulk_load(base + kSmemQ + q_slot * kQBytes + r * kQPitch, p.q + (head0 + r) * kD, kD * 2, q_full_bar(q_slot));
                     }
                     if ((q_slot ^= 1) == 0) q_phase ^= 1u;
@@ -390,7 +400,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     }
                 };
                 for (int st = grp; st < kStages; st += kGroups) drain(full_bar(st), st < slot ? phase : phase ^ 1u);
-                if (grp == 0)
+                if (grp == kGroups - 1)
                     for (int st = 0; st < 2; ++st) drain(q_full_bar(st), st < q_slot ? q_phase : q_phase ^ 1u);
             }
         }
@@ -398,6 +408,24 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     }
 
     // -------------------------------- consumers --------------------------------
+    if (warp == 0) {
+        const Share found = find_share(p, lane);
+        if (lane == 0) *reinterpret_cast<Share*>(gen_base + kSmemShare) = found;
+    } else if (threadIdx.x == 32) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full_bar(s), 1 + 2 * kQuarters);  // the tile copy and the eight scale copies
+            mbar_init(empty_bar(s), kWarpsPerGroup);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(q_full_bar(s), 1);
+            mbar_init(q_empty_bar(s), kConsumerWarps);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    named_bar_sync(2, kDecodeThreads);
+    const int lo = share.lo, hi = share.hi, cost = share.cost;
+    if (lo >= hi) return;
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
     const int g = lane >> 2, tig = lane & 3;
     const int grp = warp / kWarpsPerGroup, sub = warp % kWarpsPerGroup;
@@ -415,10 +443,10 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     const uint32_t v_off = v_row * 128u, v_swz = (v_row & 7u) ^ static_cast<uint32_t>(lane >> 4);
 
     int b = share.b;
-    int len = clamp_len(__ldg(p.seq_lens + b), p.capacity);
+    int len = share.len;
     int n_cells = cost + tiles_of(len);
-    int unit = static_cast<int>(div_nonneg(lo - share.seq_lo, n_cells));  // within the sequence
-    long long unit_lo = share.seq_lo + static_cast<long long>(unit) * n_cells;
+    int unit = share.unit;  // within the sequence
+    int unit_lo = share.unit_lo;
     bool first_unit = true;
     int turn = 0;    // the group whose turn the next tile is
     int slot = grp;  // the next stage of this warp's group
@@ -430,13 +458,22 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     while (unit_lo < hi) {
         const int n_t = n_cells - cost;
         // this block's tiles of the unit
-        int tile = lo > unit_lo + cost ? static_cast<int>(lo - unit_lo) - cost : 0;
-        const int tile_end = hi < unit_lo + n_cells ? static_cast<int>(hi - unit_lo) - cost : n_t;
+        int tile = lo > unit_lo + cost ? lo - unit_lo - cost : 0;
+        const int tile_end = hi < unit_lo + n_cells ? hi - unit_lo - cost : n_t;
         const bool whole = tile == 0 && tile_end == n_t;
         if (tile < tile_end) {
         const int kvh = unit / p.n_gblk, gblk = unit - kvh * p.n_gblk;
         const int rows = (p.G - gblk * kRows) < kRows ? (p.G - gblk * kRows) : kRows;
         const long long head0 = static_cast<long long>(b) * p.Hq + static_cast<long long>(kvh) * p.G + gblk * kRows;
+
+        if (!whole && threadIdx.x == 0) {
+            // the blocks that hold pieces of the unit, worked out while the first copies are on their way
+            const int T = share.T, W = share.W;
+            const int w_first = block_of_cell(unit_lo + cost, T, W);
+            pieces[0] = w_first;
+            pieces[1] = block_of_cell(unit_lo + n_cells - 1, T, W) - w_first + 1;
+            pieces[2] = cell_lo(w_first, T, W) >= unit_lo ? 0 : 1;  // the first one's slot for it
+        }
 
         // Q fragments: a lane's K codes of a token are dims 32 tig .. 32 tig + 31, and so are its dims of a query row; four dims
         // make a k-step
@@ -497,7 +534,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                 for (int u = 0; u < kParts; ++u) {
                     const uint32_t at = base + kSmemScale + slot * (2 * kQuarters * 4) + (sub * kParts + u) * 4;
                     ksc[u] = lds32(at);
-                    vsc[u] = lds32(at + kQuarters * 4);
+                    vsc[u] = fmaxf(lds32(at + kQuarters * 4), kMinVScale);
                 }
                 // ---- scores: 16 heads x 16 tokens a part; two accumulators per n-block make independent chains ----
                 float s[kParts][2][4];
@@ -690,7 +727,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     *reinterpret_cast<uint32_t*>(p.o + (head0 + row) * kD + rd * 32 + col0) =
                         pack_bf16x2(acc[rd][0] * inv, acc[rd][1] * inv);
                 if (col0 == 0) {
-                    const float l2 = lt == 0.f ? -INFINITY : ms - kPShift + log2f(lt);
+                    const float l2 = log2_of_sum(ms, lt);
                     if (p.lse) p.lse[head0 + row] = l2 * kLn2;
                     if (kScores) p.lse2[head0 + row] = l2;
                 }
@@ -705,32 +742,45 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
         if (!whole) {
             // this block's piece of the unit is in the workspace: count it in; the last one to arrive merges
-            const long long T = share.T, W = share.W;
-            const long long w_first = block_of_cell(unit_lo + cost, T, W);
-            const long long w_last = block_of_cell(unit_lo + n_cells - 1, T, W);
-            const int n_pieces = static_cast<int>(w_last - w_first) + 1;
-            unsigned* counter = p.counters + w_first;
-            named_bar_sync(1, kConsumerWarps * 32);
-            if (threadIdx.x == 0) {
-                __threadfence();
-                const bool last = atomicAdd(counter, 1u) == static_cast<unsigned>(n_pieces - 1);
-                __threadfence();
-                if (last) *counter = 0u;  // the counters are zero again when the kernel ends
-                misc[0] = last ? 1 : 0;
-            }
-            named_bar_sync(1, kConsumerWarps * 32);
-            if (misc[0] != 0) {
-                const int mrow = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
-                const int which_first = cell_lo(w_first, T, W) >= unit_lo ? 0 : 1;
+            const int w_first = pieces[0], n_pieces = pieces[1], which_first = pieces[2];
+            auto piece = [&](int i) { return p.slots + static_cast<long long>((w_first + i) * 2 + (i == 0 ? which_first : 0)) * kSlotFloats; };
+            // kFan neighbours first, their sum in the first one's slot, then those sums; few pieces go straight to the second step
+            const int mine = static_cast<int>(blockIdx.x) - w_first;
+            const bool flat = n_pieces <= kFlatPieces;
+            const int mrow = threadIdx.x >> 4, c8 = (threadIdx.x & 15) * 8;
+#pragma unroll 1
+            for (int step = flat ? 1 : 0; step < 2; ++step) {
+                const int at = step == 0 ? mine / kFan * kFan : 0;                    // first of the pieces to be merged
+                const int stride = step == 0 || flat ? 1 : kFan;
+                int n = step == 1 ? (n_pieces + stride - 1) / stride : n_pieces - at;  // their number
+                if (step == 0 && n > kFan) n = kFan;
+                if (step == 0 && n == 1) continue;
+                named_bar_sync(1, kConsumerWarps * 32);
+                if (threadIdx.x == 0) {
+                    unsigned* counter = p.counters + step * kMaxWorkers + w_first + at;
+                    const bool last = atomic_inc_acq_rel(counter) == static_cast<unsigned>(n - 1);
+                    if (last) *counter = 0u;  // the counters are zero again when the kernel ends
+                    misc[0] = last ? 1 : 0;
+                }
+                named_bar_sync(1, kConsumerWarps * 32);
+                if (misc[0] == 0) break;
+                float mg[8], mm = 0.f, ll = 0.f;
                 if (mrow < rows) {
-                    float mg[8], mm, ll;
-                    auto piece = [&](int i) {
-                        return p.slots + ((w_first + i) * 2 + (i == 0 ? which_first : 0)) * kSlotFloats + mrow * kPW;
-                    };
-                    if (n_pieces <= 4)
-                        merge_pieces<4>(n_pieces, c8, piece, mg, mm, ll);
+                    auto row_of = [&](int i) { return piece(at + i * stride) + mrow * kPW; };
+                    if (n <= 4)
+                        merge_pieces<4>(n, c8, row_of, mg, mm, ll);
                     else
-                        merge_pieces<8>(n_pieces, c8, piece, mg, mm, ll);
+                        merge_pieces<8>(n, c8, row_of, mg, mm, ll);
+                }
+                if (step == 0) {
+                    named_bar_sync(1, kConsumerWarps * 32);  // the first one's (m, l) have been read by all that need them
+                    if (mrow < rows) {
+                        float* dst = piece(at) + mrow * kPW;
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(dst + c8 + e) = make_float2(mg[e], mg[e + 1]);
+                        if (c8 == 0) *reinterpret_cast<float2*>(dst + kD) = make_float2(mm, ll);
+                    }
+                } else if (mrow < rows) {
                     const float inv = ll == 0.f ? 0.f : 1.f / ll;
                     uint4 pk;
                     pk.x = pack_bf16x2(mg[0] * inv, mg[1] * inv);
@@ -739,7 +789,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
                     pk.w = pack_bf16x2(mg[6] * inv, mg[7] * inv);
                     *reinterpret_cast<uint4*>(p.o + (head0 + mrow) * kD + c8) = pk;
                     if (c8 == 0) {
-                        const float l2 = ll == 0.f ? -INFINITY : mm - kPShift + log2f(ll);
+                        const float l2 = log2_of_sum(mm, ll);
                         if (p.lse) p.lse[head0 + mrow] = l2 * kLn2;
                         if (kScores) p.lse2[head0 + mrow] = l2;
                     }
@@ -792,7 +842,7 @@ __global__ void __launch_bounds__(kWeightThreads) decode_weights_kernel(const De
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
-// Workspace: arrival counters at the start (1024, as in the bf16 decode), partial slots, then -- with weights -- the
+// Workspace: arrival counters at the start (4 KB, as in the bf16 decode), partial slots, then -- with weights -- the
 // log2 normalisers and the scores of every (query head, token).
 struct DecodePlan {
     int W, n_gblk;
@@ -809,11 +859,11 @@ static int make_decode_plan(int B, int capacity, int Hq, int Hkv, int D, bool wi
     const long long units = static_cast<long long>(B) * Hkv * plan->n_gblk;
     if (units * kRows > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
     const long long most = units * ((capacity + kTok - 1) / kTok);  // tiles if every sequence filled the cache
+    if (most + units * kUnitCost > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;  // cells are counted in 32 bits
     long long W = num_workers > 0 ? num_workers : sm_count;
-    if (W > decode::kFixedCounters) W = decode::kFixedCounters;
+    if (W > kMaxWorkers) W = kMaxWorkers;
     if (W > most) W = most;
     if (W < 1) W = 1;
-    if (most / W + 1 > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;  // a block's tile count is a 32-bit loop index
     plan->W = static_cast<int>(W);
     plan->slot_offset = decode::kSlotOffsetBytes;
     plan->lse2_offset = plan->slot_offset + static_cast<size_t>(W) * 2 * kSlotFloats * sizeof(float);
@@ -912,7 +962,7 @@ static int decode_launch(const void* q, const void* k, const void* v, const floa
     CUtensorMap tm_k, tm_v;
     if ((rc = encode_cache_map(&tm_k, k, B, capacity, Hkv, kv_layout)) != CLLO_OK) return rc;
     if ((rc = encode_cache_map(&tm_v, v, B, capacity, Hkv, kv_layout)) != CLLO_OK) return rc;
-    if (!counters_zero && plan.W > 1) CLLO_CUDA_TRY(cudaMemsetAsync(ws, 0, plan.W * sizeof(unsigned), st));
+    if (!counters_zero && plan.W > 1) CLLO_CUDA_TRY(cudaMemsetAsync(ws, 0, 2 * kMaxWorkers * sizeof(unsigned), st));
     std::atomic<bool>* attr = di->kv8_decode_attr_set;
     if (format == CLLO_FMT_E4M3)
         rc = weights ? decode_launch_kernel<CLLO_FMT_E4M3, true>(tm_k, tm_v, p, plan.W, attr + 0, st)

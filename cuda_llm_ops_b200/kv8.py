@@ -45,7 +45,8 @@ class KV8Cache:
     """The tensors of an 8-bit KV cache.
 
     ``k``, ``v``: float8_e4m3fn or int8, [B,S,Hkv,D] (``KV_BSHD``) or [B,Hkv,S,D] (``KV_BHSD``), S = capacity in tokens;
-    ``k_scale``, ``v_scale``: fp32 [B,Hkv,ceil(S / block_tokens)].  A value is ``code * scale`` of its block.
+    ``k_scale``, ``v_scale``: fp32 [B,Hkv,ceil(S / block_tokens)].  A value is ``code * scale`` of its block; scales are not
+    negative, and 0 goes with codes that are 0.
     """
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "kv_layout", "block_tokens", "batch", "capacity", "num_kv_heads",

@@ -275,6 +275,52 @@ def test_decode_is_repeatable_and_independent_of_the_number_of_workers():
     assert_clean_status()
 
 
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("B,S,Hq,H,workers", [
+    (1, 12000, 16, 1, 0),     # one kv head over all blocks: merged in two steps
+    (1, 3100, 5, 1, 25),      # one more than what is merged in one step
+    (1, 3100, 5, 1, 24),
+    (1, 1600, 3, 1, 13),
+    (2, 40000, 20, 1, 512),   # more pieces than SMs; two blocks of query heads
+    (3, 4000, 4, 2, 148),
+])
+def test_decode_of_units_that_many_blocks_share(dtype, B, S, Hq, H, workers):
+    ops = _ops()
+    lens = [S - 5 * b for b in range(B)]
+    cache = _filled_cache(31, B, S, H, dtype, 1, 64, lens)
+    q = torch.randn(B, Hq, D, generator=_gen(32), device="cuda").to(torch.bfloat16)
+    first = None
+    for _ in range(3):  # the counters are left as they were found
+        lse = torch.empty(B, Hq, device="cuda")
+        out = ops.kv8_decode(q, cache, _ints(lens), lse=lse, num_workers=workers)
+        _check_decode(cache, q, _ints(lens), SCALE, out, lse)
+        first = out if first is None else first
+        assert torch.equal(out.view(torch.int16), first.view(torch.int16))
+    assert_clean_status()
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+def test_decode_of_blocks_that_nothing_was_written_to(dtype):
+    """A new cache is all zeros, its scales too: tokens of value 0, whose scores are 0."""
+    ops = _ops()
+    cache = ops.kv8_cache(2, 300, 2, dtype, 1, 32)
+    q = torch.randn(2, 8, D, generator=_gen(3), device="cuda").to(torch.bfloat16)
+    lens = _ints([300, 1])
+    lse = torch.empty(2, 8, device="cuda")
+    weights = torch.zeros(2, 2, 300, device="cuda")
+    out = ops.kv8_decode(q, cache, lens, lse=lse, weights=weights)
+    assert (out == 0).all()
+    _check_decode(cache, q, lens, SCALE, out, lse, added=(torch.zeros_like(weights), weights))
+    ops.kv8_append(cache, _rows(4, 2, 2, 130, D), _rows(5, 2, 2, 130, D), _ints([40, 0]))
+    lens = _ints([300, 210])
+    base = weights.clone()
+    out = ops.kv8_decode(q, cache, lens, lse=lse, weights=weights)
+    _check_decode(cache, q, lens, SCALE, out, lse, added=(base, weights))
+    kept, _, _, _ = ops.kv8_evict(cache, weights, lens, 200)
+    out = ops.kv8_decode(q, kept, lens.clamp(max=200), lse=lse)
+    _check_decode(kept, q, lens.clamp(max=200), SCALE, out, lse)
+
+
 def test_decode_in_graphs_that_share_nothing():
     """Two captured calls replayed on two streams at once, lengths changed in between; an eager call beside them."""
     ops = _ops()
