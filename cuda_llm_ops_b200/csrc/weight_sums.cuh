@@ -15,7 +15,9 @@
 //
 // Work decomposition.  A unit is (sequence, kv head, 256 keys): two key tiles that share every query tile.  Its steps are
 // the (head of the group, 128 queries) pairs that the mask lets it see; under a causal mask the first keys have the
-// most.  The steps of all units (plus kUnitCost cells each for what a unit costs by itself) form one index space that the
+// most.  Where no more than 64 (32) queries of a head can count -- a window, a short prompt -- a step takes the queries
+// of two (four) heads: a step costs much the same however many of its columns count (4 prompts of 8192 tokens, window 64,
+// groups of 4: 54 us with one head a step, 40 with two).  The steps of all units (plus kUnitCost cells each for what a unit costs by itself) form one index space that the
 // persistent blocks share evenly; the lengths live on the device, so every block works out its share for itself, in closed
 // form per sequence.  A unit cut between blocks leaves one fp32 partial per key and block; the last block to arrive adds
 // them up in block order.
@@ -51,7 +53,8 @@ constexpr int kSmemBar = kSmemLse + kLseStages * kQ * 4;
 constexpr int kNumBars = 2 * kKStages + 2 * kQStages + 2 * kLseStages + 4 * kTiles + 1;
 constexpr int kSmemHalf = kSmemBar + kNumBars * 8;  // the second warpgroup's sum of every key
 constexpr int kSmemMisc = kSmemHalf + kPair * 4;
-constexpr int kSmemBytes = kSmemMisc + 32 + 1024;
+constexpr int kSmemWalk = (kSmemMisc + 32 + 7) / 8 * 8;  // the block's first unit, found by one warp
+constexpr int kSmemBytes = kSmemWalk + 128 + 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kEpiThreads = kEpiWarps * 32;
 
@@ -67,10 +70,21 @@ struct Params {
     unsigned* counters;
     float scale_log2;
     int B, Sq, Skv, Hq, Hkv, G, q_start, window, causal, accumulate, n_pairs;
+    int head_shift;       // log2 of the columns that a head has in a query tile: 7, or 6 or 5 where that takes all its queries
+    int groups;           // heads of a kv head's group, or those pairs or fours of them
+
 };
 
-using decode::worker_lo;
-using decode::worker_of_tile;
+// a / b for non-negative values; most of them fit 32 bits, where a division costs a quarter
+__device__ __forceinline__ long long div_nonneg(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+// the cells [worker_lo(w), worker_lo(w + 1)) of block w, and the block that holds cell c
+__device__ __forceinline__ long long worker_lo(long long w, long long T, long long W) { return div_nonneg(w * T, W); }
+__device__ __forceinline__ long long worker_of_cell(long long c, long long T, long long W) {
+    return div_nonneg((c + 1) * W - 1, T);
+}
 
 // The part of a sequence's work that does not depend on the kv head: which queries count, and how many steps a pair of key
 // tiles takes per head.
@@ -94,7 +108,7 @@ struct Seq {
         if (e > np) e = np;
         if (e > p) e = p;
         if (e > p1) n += static_cast<long long>(m) * (e - p1) - (static_cast<long long>(e) * (e - 1) - static_cast<long long>(p1) * (p1 - 1));
-        return static_cast<long long>(kUnitCost) * p + prm.G * n;
+        return static_cast<long long>(kUnitCost) * p + prm.groups * n;
     }
 };
 
@@ -131,13 +145,13 @@ struct Walk {
     int b, kvh, p;
     Seq seq;
     // of the current unit
-    int n, steps;       // query tiles per head, steps in all
+    int n, steps;       // query tiles per head (or heads that share one), steps in all
     int s_lo, s_hi;     // this block's steps
     bool first;         // the block's first unit
 
     __device__ __forceinline__ void enter(const Params& prm) {
         n = seq.tiles(p);
-        steps = prm.G * n;
+        steps = prm.groups * n;
         const long long base = unit_lo + kUnitCost;
         s_lo = lo > base ? static_cast<int>(lo - base) : 0;
         s_hi = hi < base + steps ? static_cast<int>(hi - base) : steps;
@@ -165,13 +179,13 @@ struct Walk {
         const int own = prm.causal ? p * kPair - prm.q_start : 0;
         return (own > seq.i_lo ? own : seq.i_lo) + j * kQ;
     }
+    // heads whose queries the tiles of group g hold
+    __device__ __forceinline__ int heads(const Params& prm, int g, int head_shift) const {
+        const int most = kQ >> head_shift, left = prm.G - g * most;
+        return left < most ? left : most;
+    }
     // key tiles of the unit that hold keys: a second one without any is not loaded
     __device__ __forceinline__ int key_tiles() const { return p * kPair + kKeys < seq.len ? 2 : 1; }
-    // whether key tile t of the unit has anything to do with the query tile at row i0
-    __device__ __forceinline__ bool sees(const Params& prm, int t, int i0) const {
-        const int key0 = p * kPair + t * kKeys;
-        return key0 < seq.len && !(prm.causal && prm.q_start + i0 + kQ - 1 < key0);
-    }
 };
 
 __device__ __forceinline__ Walk start_walk(const Params& p, int lane) {
@@ -186,8 +200,9 @@ __device__ __forceinline__ Walk start_walk(const Params& p, int lane) {
     w.b = w.kvh = w.p = 0;
     w.first = true;
     if (blockIdx.x >= w.W) return w;
-    w.lo = worker_lo(blockIdx.x, w.T, w.W);
-    w.hi = worker_lo(blockIdx.x + 1, w.T, w.W);
+    const long long edge = worker_lo(blockIdx.x + (lane & 1), w.T, w.W);  // both ends at once
+    w.lo = __shfl_sync(0xffffffffu, edge, 0);
+    w.hi = __shfl_sync(0xffffffffu, edge, 1);
     long long seq_lo = 0;
     for (int i0 = 0; i0 < p.B; i0 += 32) {
         const int i = i0 + lane;
@@ -209,16 +224,16 @@ __device__ __forceinline__ Walk start_walk(const Params& p, int lane) {
         seq_lo = __shfl_sync(0xffffffffu, end, 31);
     }
     w.seq = describe(p, w.b);
-    w.kvh = static_cast<int>((w.lo - seq_lo) / w.seq.cells);
+    w.kvh = static_cast<int>(div_nonneg(w.lo - seq_lo, w.seq.cells));
     const long long head_lo = seq_lo + w.kvh * w.seq.cells;
     const long long off = w.lo - head_lo;
-    int a = 0, z = p.n_pairs;  // the last pair whose first cell is <= off
+    int a = 0, z = p.n_pairs;  // the last pair whose first cell is <= off lies in [a, z); 32 places are looked at at once
     while (z - a > 1) {
-        const int mid = a + (z - a) / 2;
-        if (w.seq.before(p, mid) <= off)
-            a = mid;
-        else
-            z = mid;
+        const int step = (z - a + 31) / 32, at = a + lane * step;
+        const unsigned below = __ballot_sync(0xffffffffu, at < z && w.seq.before(p, at) <= off);  // lane 0 among them
+        const int last = 31 - __clz(static_cast<int>(below));
+        z = a + (last + 1) * step < z ? a + (last + 1) * step : z;
+        a += last * step;
     }
     w.p = a;
     w.unit_lo = head_lo + w.seq.before(p, a);
@@ -226,9 +241,12 @@ __device__ __forceinline__ Walk start_walk(const Params& p, int lane) {
     return w;
 }
 
+// kShared: heads share a query tile
+template <bool kShared>
 __global__ void __launch_bounds__(kThreads, 1)
 weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const Params p) {
     using namespace prefill;
+    const int head_shift = kShared ? p.head_shift : 7;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
@@ -276,10 +294,16 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
     }
-    Walk w = start_walk(p, lane);
+    Walk* first_walk = reinterpret_cast<Walk*>(gen_base + sums::kSmemWalk);
+    static_assert(sizeof(Walk) <= 128, "the walk's place in shared memory");
+    if (warp == 1) {  // all 20 warps finding it at once were in one another's way: 6000 cycles instead of 3900
+        const Walk found = start_walk(p, lane);
+        if (lane == 0) *first_walk = found;
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    Walk w = *first_walk;
     const uint32_t tmem_base = *tmem_slot;
 
     if (warp == kEpiWarps) {
@@ -293,10 +317,13 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 int g = w.s_lo / w.n, j = w.s_lo - g * w.n;
                 for (int s = w.s_lo; s < w.s_hi; ++s) {
                     mbar_wait_idle(q_empty(qs), qp ^ 1u, abort_flag, SITE_SUMS_Q, qs);
-                    mbar_arrive_expect_tx(q_full(qs), sums::kTileBytes);
-                    for (int d = 0; d < 2; ++d)
-                        tma_load_4d(base + sums::kSmemQ + qs * sums::kTileBytes + d * kSlabBytes, &tm_q, q_full(qs), d * 64,
-                                    w.row0(p, j), w.kvh * p.G + g, w.b);
+                    const int heads = w.heads(p, g, head_shift), i0 = w.row0(p, j);
+                    const int head0 = w.kvh * p.G + g * (kQ >> head_shift);
+                    const uint32_t dst = base + sums::kSmemQ + qs * sums::kTileBytes;
+                    mbar_arrive_expect_tx(q_full(qs), heads * (sums::kTileBytes >> (7 - head_shift)));
+                    for (int u = 0; u < heads; ++u)
+                        for (int d = 0; d < 2; ++d)
+                            tma_load_4d(dst + d * kSlabBytes + (u << head_shift) * 128, &tm_q, q_full(qs), d * 64, i0, head0 + u, w.b);
                     if (++qs == kQStages) {
                         qs = 0;
                         qp ^= 1u;
@@ -344,39 +371,49 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         }
     } else if (warp == kEpiWarps + 1) {
         // -------------------------------- MMA issuer --------------------------------
-        // the whole warp runs the loop and the leader lane's predicate guards the MMAs (see tc_mma_ss_lo_if)
+        // The whole warp runs the loop and the leader lane's predicate guards the MMAs (see tc_mma_ss_lo_if).  What the operands
+        // and the control flow depend on goes through a broadcast: only then does the compiler know that it is the same in all
+        // lanes, and keeps it in uniform registers.
         const uint32_t leader = lane == 0 ? 1u : 0u;
         const uint32_t hi = smem_desc_hi(1024);
+        auto same = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+        const uint32_t acc0 = static_cast<uint32_t>(same(static_cast<int>(tmem_base)));
         int ks = 0, qs = 0, ds[sums::kTiles] = {0, 0};
         uint32_t kp = 0, qp = 0, dp[sums::kTiles] = {0, 0};
-        for (; !w.done(); w.next(p)) {
-            if (!w.active()) continue;
+        for (; same(!w.done()); w.next(p)) {
+            const int n_steps = same(w.s_hi - w.s_lo);
+            if (n_steps <= 0) continue;
             int k_stage[sums::kTiles] = {0, 0};
-            const int n_tiles = w.key_tiles();
+            const int n_tiles = same(w.key_tiles());
 #pragma unroll
             for (int t = 0; t < sums::kTiles; ++t) {
                 if (t >= n_tiles) continue;
-                if (lane == 0) mbar_wait_idle(k_full(ks), kp, abort_flag, SITE_SUMS_K, ks);
+                mbar_wait_idle(k_full(ks), kp, abort_flag, SITE_SUMS_K, ks);
                 k_stage[t] = ks;
                 if (++ks == kKStages) {
                     ks = 0;
                     kp ^= 1u;
                 }
             }
-            __syncwarp();
-            int j = w.s_lo % w.n;
-            for (int s = w.s_lo; s < w.s_hi; ++s) {
-                if (lane == 0) mbar_wait_idle(q_full(qs), qp, abort_flag, SITE_SUMS_Q, qs);
-                const int i0 = w.row0(p, j);
+            // tile j of the unit's n is seen by key tile t from j_sees on (as the exponentials have it)
+            const int n = same(w.n), r0 = w.row0(p, 0), key0 = w.p * kPair;
+            int j = same(w.s_lo % w.n), j_sees[sums::kTiles];
+#pragma unroll
+            for (int t = 0; t < sums::kTiles; ++t) {
+                const int ahead = p.causal ? key0 + t * kKeys - p.q_start - r0 : 0;
+                j_sees[t] = same(t >= n_tiles ? 0x7fffffff : (ahead > 0 ? ahead / kQ : 0));
+            }
+            for (int left = n_steps; left > 0; --left) {
+                mbar_wait_idle(q_full(qs), qp, abort_flag, SITE_SUMS_Q, qs);
+                const uint32_t bq = smem_desc_lo(base + sums::kSmemQ + qs * sums::kTileBytes, 16);
 #pragma unroll
                 for (int t = 0; t < sums::kTiles; ++t) {
-                    if (!w.sees(p, t, i0)) continue;
-                    if (lane == 0) mbar_wait_idle(d_empty(t, ds[t]), dp[t] ^ 1u, abort_flag, SITE_SUMS_D, t);
+                    if (j < j_sees[t]) continue;
+                    mbar_wait_idle(d_empty(t, ds[t]), dp[t] ^ 1u, abort_flag, SITE_SUMS_D, t);
                     __syncwarp();
                     tc_fence_after();
                     const uint32_t a = smem_desc_lo(base + sums::kSmemK + k_stage[t] * sums::kTileBytes, 16);
-                    const uint32_t bq = smem_desc_lo(base + sums::kSmemQ + qs * sums::kTileBytes, 16);
-                    const uint32_t d = tmem_base + (t * 2 + ds[t]) * kQ;
+                    const uint32_t d = acc0 + (t * 2 + ds[t]) * kQ;
                     tc_mma_ss_lo_if<false>(leader, d, a, bq, hi, kIdescQK);
 #pragma unroll
                     for (int k = 1; k < 8; ++k) {
@@ -391,7 +428,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                     qs = 0;
                     qp ^= 1u;
                 }
-                if (++j == w.n) j = 0;
+                if (++j == n) j = 0;
             }
             for (int t = 0; t < n_tiles; ++t) tc_commit_if(leader, k_empty(k_stage[t]));
         }
@@ -428,12 +465,14 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             int g = w.s_lo / w.n, j = w.s_lo - g * w.n;
             for (int s = w.s_lo; s < w.s_hi; ++s) {
                 const int i0 = w.row0(p, j), slot = put % kLseStages;
-                const float* src = p.lse + (static_cast<long long>(w.b) * p.Hq + w.kvh * p.G + g) * p.Sq;
+                const int heads = w.heads(p, g, head_shift);
+                const float* src = p.lse + (static_cast<long long>(w.b) * p.Hq + w.kvh * p.G + g * (kQ >> head_shift)) * p.Sq;
                 mbar_wait_idle(lse_empty(slot), (static_cast<uint32_t>(put / kLseStages) & 1u) ^ 1u, abort_flag, SITE_SUMS_LSE, slot);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = i0 + e * 32 + lane;
-                    kv8::cp_async_4(smem_u32(lse_buf + slot * kQ + e * 32 + lane), src + (i < w.seq.i_hi ? i : i0));
+                    const int c = e * 32 + lane, u = c >> head_shift, i = i0 + (c & ((1 << head_shift) - 1));
+                    kv8::cp_async_4(smem_u32(lse_buf + slot * kQ + c),
+                                    src + static_cast<long long>(u < heads ? u : 0) * p.Sq + (i < w.seq.i_hi ? i : i0));
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (++put > kLseAhead) {
@@ -476,7 +515,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             // the first column of tile 0 that this key sees; without a causal mask every one, for all keys of a warp alike
             const int own = p.causal ? ahead + static_cast<int>(threadIdx.x & (kKeys - 1)) : lane - 31;
             const float scale = p.scale_log2;
-            int j = w.s_lo % w.n;
+            int j = w.s_lo % w.n, g = w.s_lo / w.n;
 #pragma unroll 1
             for (int left = w.s_hi - w.s_lo; left > 0; --left) {
                 mbar_wait_idle(lse_full(ls), lp, abort_flag, SITE_SUMS_LSE, ls);
@@ -502,7 +541,8 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                             sum[3] += fast_exp2(fmaf(x[e + 3], scale, l4.w));
                         }
                     };
-                    if (lo_last <= 0 && hi >= kQ) {
+                    const int cols = 1 << head_shift, end = w.heads(p, g, head_shift) << head_shift;  // of a head, of all heads
+                    if (lo_last <= 0 && hi >= cols && end == kQ) {
 #pragma unroll
                         for (int c = 0; c < kQ; c += 32) {
                             float x[32];
@@ -511,12 +551,13 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                         }
                     } else {
 #pragma unroll 1
-                        for (int c = 0; c < kQ; c += 32) {
+                        for (int at = 0; at < end; at += 32) {
+                            const int c = at & (cols - 1);  // within the head
                             if (c >= hi || lo_first >= c + 32) continue;  // nothing for any key of the warp
                             float x[32];
-                            tmem_ld32_wait(acc + c, x);
+                            tmem_ld32_wait(acc + at, x);
                             if (lo_last <= c && hi >= c + 32) {
-                                add_chunk(x, nl + c);
+                                add_chunk(x, nl + at);
                                 continue;
                             }
                             // bit e: the chunk's column e counts for this key.  What does not count may be anything, NaN too
@@ -524,7 +565,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                                                   (hi >= c + 32 ? 0xffffffffu : (1u << (hi - c)) - 1u);
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
-                                const float y = fmaf(x[e], scale, nl[c + e]);
+                                const float y = fmaf(x[e], scale, nl[at + e]);
                                 sum[e & 3] += fast_exp2(seen >> e & 1u ? y : -INFINITY);
                             }
                         }
@@ -540,7 +581,10 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                     ls = 0;
                     lp ^= 1u;
                 }
-                if (++j == w.n) j = 0;
+                if (++j == w.n) {
+                    j = 0;
+                    ++g;
+                }
             }
             if (key >= w.seq.len) total = 0.f;  // whatever lies behind the sequence
             // the two warpgroups' sums of a key meet; the barrier also keeps the next unit's value out until this one has been read
@@ -554,8 +598,8 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             }
             // this block's part of the unit goes to the workspace; the last block to arrive adds the parts up
             if (turn == 0) p.slots[(static_cast<long long>(blockIdx.x) * 2 + (w.first ? 0 : 1)) * kPair + key_in_pair] = total;
-            const long long w_first = worker_of_tile(w.unit_lo + kUnitCost, w.T, w.W);
-            const long long w_last = worker_of_tile(w.unit_lo + kUnitCost + w.steps - 1, w.T, w.W);
+            const long long w_first = worker_of_cell(w.unit_lo + kUnitCost, w.T, w.W);
+            const long long w_last = worker_of_cell(w.unit_lo + kUnitCost + w.steps - 1, w.T, w.W);
             const int n_pieces = static_cast<int>(w_last - w_first) + 1;
             named_bar_sync(1, kEpiThreads);
             if (threadIdx.x == 0) {
@@ -588,12 +632,12 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
-static int encode_map(CUtensorMap* map, const void* basep, int B, int H, int S) {
+static int encode_map(CUtensorMap* map, const void* basep, int B, int H, int S, uint32_t rows) {
     const uint64_t row = static_cast<uint64_t>(kD) * 2;
     const uint64_t dims[4] = {static_cast<uint64_t>(kD), static_cast<uint64_t>(S), static_cast<uint64_t>(H),
                               static_cast<uint64_t>(B)};
     const uint64_t strides[3] = {row, row * S, row * S * H};
-    const uint32_t box[4] = {64, 128, 1, 1};
+    const uint32_t box[4] = {64, rows, 1, 1};
     return encode_bf16_4d(map, basep, dims, strides, box);
 }
 
@@ -640,16 +684,23 @@ static int launch(const void* q, const void* k, const float* lse, const int* seq
     p.causal = causal ? 1 : 0;
     p.accumulate = flags & CLLO_SUMS_ACCUMULATE ? 1 : 0;
     p.n_pairs = (Skv + kPair - 1) / kPair;
+    const int most_rows = window > 0 && window < Sq ? window : Sq;  // queries of a head that count at most
+    p.head_shift = most_rows <= 32 ? 5 : most_rows <= 64 ? 6 : 7;
+    p.groups = (p.G + (kQ >> p.head_shift) - 1) / (kQ >> p.head_shift);
     CUtensorMap tm_q, tm_k;
-    if ((rc = encode_map(&tm_q, q, B, Hq, Sq)) != CLLO_OK) return rc;
-    if ((rc = encode_map(&tm_k, k, B, Hkv, Skv)) != CLLO_OK) return rc;
+    if ((rc = encode_map(&tm_q, q, B, Hq, Sq, 1u << p.head_shift)) != CLLO_OK) return rc;
+    if ((rc = encode_map(&tm_k, k, B, Hkv, Skv, kKeys)) != CLLO_OK) return rc;
     if (!di->sums_attr_set) {
-        CLLO_CUDA_TRY(cudaFuncSetAttribute(weight_sums_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        CLLO_CUDA_TRY(cudaFuncSetAttribute(weight_sums_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        CLLO_CUDA_TRY(cudaFuncSetAttribute(weight_sums_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
         di->sums_attr_set = true;
     }
     const int blocks = blocks_for(di->sm_count);
     if (!(flags & CLLO_WS_COUNTERS_ZERO)) CLLO_CUDA_TRY(cudaMemsetAsync(workspace, 0, blocks * sizeof(unsigned), st));
-    weight_sums_kernel<<<blocks, kThreads, kSmemBytes, st>>>(tm_q, tm_k, p);
+    if (p.head_shift < 7)
+        weight_sums_kernel<true><<<blocks, kThreads, kSmemBytes, st>>>(tm_q, tm_k, p);
+    else
+        weight_sums_kernel<false><<<blocks, kThreads, kSmemBytes, st>>>(tm_q, tm_k, p);
     CLLO_CUDA_TRY(cudaGetLastError());
     return CLLO_OK;
 }

@@ -16,6 +16,7 @@ graph and follows the lengths at replay.  None of the calls changes a length; ``
 """
 import contextlib
 import ctypes
+import functools
 import math
 import threading
 
@@ -97,7 +98,7 @@ def kv8_cache(batch, capacity, num_kv_heads, dtype=torch.float8_e4m3fn, kv_layou
 
 
 def _check_lens(name, t, batch, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != batch \
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or t.numel() != batch \
             or t.device != device or not t.is_contiguous():
         raise ValueError("%s must be a contiguous int32 tensor [batch] on the cache's device" % name)
 
@@ -115,6 +116,7 @@ def _require_cuda(cache):
 _Strides = ctypes.c_longlong * 3
 
 
+@functools.lru_cache(maxsize=1024)
 def _row_strides(s, kv_layout):
     """{batch, token, head} of a [B,T,H,D] or [B,H,T,D] tensor's strides."""
     return _Strides(s[0], s[1], s[2]) if kv_layout == KV_BSHD else _Strides(s[0], s[2], s[1])
@@ -328,8 +330,8 @@ def kv8_evict(cache, weights, seq_lens, budget, sink=0, recent=0, out=None, out_
     else:
         _check_fp32("out_weights", out_weights, (B, H, out.capacity), device)
     with _on(device):
-        new_lens = torch.empty(B, dtype=torch.int32, device=device)
-        indices = torch.empty((B, H, budget), dtype=torch.int32, device=device)
+        new_lens = torch.empty_like(seq_lens)
+        indices = seq_lens.new_empty((B, H, budget))
         rc = _lib.load().cllo_kv8_evict(
             cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
             weights.data_ptr(), seq_lens.data_ptr(), out.k.data_ptr(), out.v.data_ptr(), out.k_scale.data_ptr(),

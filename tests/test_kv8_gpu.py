@@ -422,6 +422,18 @@ def test_weight_sums(B, Sq, Skv, Hq, H, causal, q_start, lens, window):
     assert_clean_status()
 
 
+@pytest.mark.parametrize("window", [1, 31, 32, 33, 64, 65, 128, 129])
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 8])
+def test_weight_sums_of_windows_whose_heads_share_a_tile(window, group):
+    test_weight_sums(3, 700, 700, 2 * group, 2, True, 0, [700, 513, 20], window)
+
+
+@pytest.mark.parametrize("Sq,Skv,q_start,lens", [(20, 600, 575, [595, 300]), (64, 64, 0, [64, 7]), (33, 900, 200, [233, 210])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_weight_sums_of_few_queries(causal, Sq, Skv, q_start, lens):
+    test_weight_sums(2, Sq, Skv, 7, 1, causal, q_start if causal else 0, lens, None)
+
+
 def test_weight_sums_of_the_forward_add_up_to_its_rows():
     """With the forward's own lse the sums of a causal prompt add up to the number of (head, query) rows."""
     ops = _ops()
