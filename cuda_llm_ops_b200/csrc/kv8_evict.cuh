@@ -52,8 +52,11 @@ __device__ __forceinline__ uint32_t cluster_size() {
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 // a word of another block's shared memory, at the address it has in this block's
 __device__ __forceinline__ int cluster_load(const int* p, uint32_t rank) {
@@ -74,15 +77,16 @@ __device__ __forceinline__ void cluster_load2(const int* p, uint32_t rank, int& 
 // once and stay in shared memory as integers; a pass counts the digits of the keys that share the prefix found so far
 // (equal digits of a warp are added together first: weights cluster in few exponents, and ties share every digit), the
 // blocks add up each other's counts over distributed shared memory, and every block finds the same digit.  Bound by the
-// latency of its passes: 4 cluster barriers, 8 block barriers.
+// latency of its passes: 5 cluster barriers, 8 block barriers.
 __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictParams p) {
-    extern __shared__ uint32_t keys[];
-    __shared__ __align__(8) int hist[2][kBins];
+    extern __shared__ __align__(16) uint32_t keys[];
+    __shared__ __align__(8) int hist[3][kBins];  // one per pass
     __shared__ int warp_sum[kSelectThreads / 32];
     __shared__ int s_digit, s_need;
     __shared__ int s_counts[2];  // this block's tokens that stay whatever the others hold, and those at the threshold
     pdl_launch_dependents();  // the moving blocks may take their places; they wait for this grid's end
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < 3 * kBins; i += kSelectThreads) hist[0][i] = 0;
     const int C = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
     const int row = blockIdx.x / C;
     const int h = row % p.Hkv, b = row / p.Hkv;
@@ -101,7 +105,10 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
     const float* w = p.weights + static_cast<long long>(row) * p.capacity + t0;
     const int lo = p.sink - t0, hi = len - p.recent - t0;  // candidates [lo, hi) in the chunk's own terms
     const int n_smem = n < kKeysInSmem ? n : kKeysInSmem;
-    for (int i0 = tid; i0 < n_smem; i0 += kSelectThreads * kSelectUnroll) {
+    // The key of a token that is no candidate is 0, which no weight has: order_key is at least that of -infinity.
+    auto candidate_key = [&](int i, float x) { return i >= lo && i < hi ? order_key(x) : 0u; };
+    const int n_pad = (n_smem + 3) & ~3;
+    for (int i0 = tid; i0 < n_pad; i0 += kSelectThreads * kSelectUnroll) {
         float x[kSelectUnroll];
 #pragma unroll
         for (int u = 0; u < kSelectUnroll; ++u) {
@@ -111,38 +118,44 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
 #pragma unroll
         for (int u = 0; u < kSelectUnroll; ++u) {
             const int i = i0 + u * kSelectThreads;
-            if (i < n_smem) keys[i] = order_key(x[u]);
+            if (i < n_pad) keys[i] = i < n_smem ? candidate_key(i, x[u]) : 0u;
         }
     }
-    auto key_at = [&](int i) { return i < n_smem ? keys[i] : order_key(__ldg(w + i)); };
+    auto key_at = [&](int i) { return i < n_smem ? keys[i] : candidate_key(i, __ldg(w + i)); };
+    __syncthreads();
 
     const bool any = p.budget > p.sink + p.recent;
     uint32_t prefix = 0u, mask = 0u;
     int need = p.budget - p.sink - p.recent;  // how many of the keys that share the prefix are kept
     if (any) {
-        int buf = 0;
 #pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
             const uint32_t digits = pass == 2 ? 0x3ffu : 0x7ffu;
-            for (int i = tid; i < kBins; i += kSelectThreads) hist[buf][i] = 0;
-            __syncthreads();  // also: the keys are in place
-            const int steps = (n + kSelectThreads - 1) / kSelectThreads;
-#pragma unroll 4
-            for (int k = 0; k < steps; ++k) {
-                const int i = k * kSelectThreads + tid;
-                const uint32_t key = i < n && i >= lo && i < hi ? key_at(i) : 0u;
-                const bool in = i < n && i >= lo && i < hi && (key & mask) == prefix;
+            int* counts = hist[pass];
+            auto count = [&](uint32_t key) {  // by all lanes of a warp together
+                const bool in = (key & mask) == prefix;
                 const unsigned active = __ballot_sync(0xffffffffu, in);
-                if (active == 0u) continue;
+                if (active == 0u) return;
                 const int first = __ffs(active) - 1;
                 const int d = static_cast<int>((key >> shift) & digits), d0 = __shfl_sync(0xffffffffu, d, first);
                 if (__all_sync(0xffffffffu, !in || d == d0)) {
-                    if (lane == first) atomicAdd(&hist[buf][d0], __popc(active));  // ties, or one exponent for all
+                    if (lane == first) atomicAdd(&counts[d0], __popc(active));  // ties, or one exponent for all
                 } else if (in) {
-                    atomicAdd(&hist[buf][d], 1);
+                    atomicAdd(&counts[d], 1);
                 }
+            };
+            const int quads = n_pad / 4;
+#pragma unroll 2
+            for (int q0 = 0; q0 < quads; q0 += kSelectThreads) {
+                const uint4 k4 = q0 + tid < quads ? reinterpret_cast<const uint4*>(keys)[q0 + tid] : make_uint4(0u, 0u, 0u, 0u);
+                count(k4.x);
+                count(k4.y);
+                count(k4.z);
+                count(k4.w);
             }
+#pragma unroll 1
+            for (int i0 = n_smem; i0 < n; i0 += kSelectThreads) count(i0 + tid < n ? key_at(i0 + tid) : 0u);
             cluster_sync();
             // sum over the cluster, then the largest digit at which the count from the top reaches `need`: two bins a thread,
             // highest first
@@ -150,7 +163,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
 #pragma unroll
             for (int r = 0; r < kMaxCluster; ++r) {
                 part[r][0] = part[r][1] = 0;
-                if (r < C) cluster_load2(&hist[buf][kBins - 2 - 2 * tid], r, part[r][1], part[r][0]);
+                if (r < C) cluster_load2(&counts[kBins - 2 - 2 * tid], r, part[r][1], part[r][0]);
             }
 #pragma unroll
             for (int r = 0; r < kMaxCluster; ++r) {
@@ -181,7 +194,6 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
             prefix |= static_cast<uint32_t>(s_digit) << shift;
             mask |= digits << shift;
             need = s_need;
-            buf ^= 1;  // the others may still be reading this pass's counts
         }
     }
 
@@ -190,7 +202,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
         above = equal = false;
         if (i >= n) return;
         if (i < lo || i >= hi) {
-            above = true;
+            above = true;  // sink or recent
         } else if (any) {
             const uint32_t key = key_at(i);
             above = key > prefix;
@@ -201,15 +213,20 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
     const int per_warp = ((n + kSelectThreads / 32 - 1) / (kSelectThreads / 32) + 31) / 32 * 32;
     const int w_lo = warp * per_warp, w_hi = w_lo + per_warp < n ? w_lo + per_warp : n;
     int n_above = 0, n_equal = 0;
+    unsigned kept_above = 0u, kept_equal = 0u;  // lane k: the warp's answers of its k-th step
 #pragma unroll 4
     for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
         bool above, equal;
         classify(i0 + lane, above, equal);
-        n_above += __popc(__ballot_sync(0xffffffffu, above));
-        n_equal += __popc(__ballot_sync(0xffffffffu, equal));
+        const unsigned ba = __ballot_sync(0xffffffffu, above), be = __ballot_sync(0xffffffffu, equal);
+        n_above += __popc(ba);
+        n_equal += __popc(be);
+        if (i0 - w_lo == lane * 32) {
+            kept_above = ba;
+            kept_equal = be;
+        }
     }
-    int* totals = hist[0];  // two ints per warp; the last counts to be read were hist[0] of the third pass
-    cluster_sync();
+    int* totals = hist[0];  // two ints per warp; the others read the first pass's counts before they came to the second's barrier
     if (lane == 0) {
         totals[2 * warp] = n_above;
         totals[2 * warp + 1] = n_equal;
@@ -242,19 +259,28 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
         a_before += a;
         e_before += e;
     }
+    cluster_arrive();  // this block has read what it reads of the others
     const unsigned below = (1u << lane) - 1u;
 #pragma unroll 2
     for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
-        bool above, equal;
-        classify(i0 + lane, above, equal);
-        const unsigned ba = __ballot_sync(0xffffffffu, above), be = __ballot_sync(0xffffffffu, equal);
+        unsigned ba, be;
+        if (const int k = (i0 - w_lo) / 32; k < 32) {
+            ba = __shfl_sync(0xffffffffu, kept_above, k);
+            be = __shfl_sync(0xffffffffu, kept_equal, k);
+        } else {
+            bool above, equal;
+            classify(i0 + lane, above, equal);
+            ba = __ballot_sync(0xffffffffu, above);
+            be = __ballot_sync(0xffffffffu, equal);
+        }
+        const bool above = ba >> lane & 1u, equal = be >> lane & 1u;
         const int a = a_before + __popc(ba & below), e = e_before + __popc(be & below);
         // of the tokens at the threshold the first `need` stay
         if (above || (equal && e < need)) idx[a + (e < need ? e : need)] = t0 + i0 + lane;
         a_before += __popc(ba);
         e_before += __popc(be);
     }
-    cluster_sync();  // no block leaves while another may still read its counts
+    cluster_wait();  // no block leaves while another may still read its counts
 }
 
 // four lanes per row, 32 bytes of K and of V per lane
