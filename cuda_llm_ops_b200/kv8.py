@@ -28,6 +28,7 @@ from .flash_gqa import HEAD_DIM, KV_BHSD, KV_BSHD, _counted_workspaces, _require
 _FORMATS = {torch.float8_e4m3fn: _lib.FMT_E4M3, torch.int8: _lib.FMT_INT8}
 BLOCK_TOKENS = (16, 32, 64, 128)
 _MAX_POSITIONS = 1 << 30
+_FP32, _INT32 = torch.float32, torch.int32
 
 # A decoding step's calls take a few microseconds on the GPU: the device switch and the stream look-up of torch.cuda cost
 # as much again per call, so the switch is skipped where the device is current and the stream comes from the raw getter.
@@ -54,28 +55,28 @@ class KV8Cache:
                  "format")
 
     def __init__(self, k, v, k_scale, v_scale, kv_layout=KV_BHSD, block_tokens=64):
-        fmt = _FORMATS.get(k.dtype)
-        if fmt is None or v.dtype != k.dtype:
+        dtype, shape, device = k.dtype, k.shape, k.device
+        fmt = _FORMATS.get(dtype)
+        if fmt is None or v.dtype is not dtype:
             raise ValueError("k and v must both be float8_e4m3fn or both int8")
-        if kv_layout != KV_BSHD and kv_layout != KV_BHSD:
-            raise ValueError("unknown kv_layout")
         if block_tokens not in BLOCK_TOKENS:
             raise ValueError("block_tokens must be one of %s" % (BLOCK_TOKENS,))
-        if k.dim() != 4 or v.shape != k.shape or k.shape[3] != HEAD_DIM:
+        if len(shape) != 4 or v.shape != shape or shape[3] != HEAD_DIM:
             raise ValueError("expected k and v of identical 4-D shape with head_dim %d" % HEAD_DIM)
         if kv_layout == KV_BSHD:
-            batch, capacity, heads, _ = k.shape
+            batch, capacity, heads, _ = shape
+        elif kv_layout == KV_BHSD:
+            batch, heads, capacity, _ = shape
         else:
-            batch, heads, capacity, _ = k.shape
-        if batch < 1 or capacity < 1 or heads < 1:
+            raise ValueError("unknown kv_layout")
+        if not (batch and capacity and heads):
             raise ValueError("a cache holds at least one sequence, one token and one kv head")
         scales = (batch, heads, -(-capacity // block_tokens))
-        if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.shape != scales \
+        if k_scale.dtype is not _FP32 or v_scale.dtype is not _FP32 or k_scale.shape != scales \
                 or v_scale.shape != scales:
             raise ValueError("k_scale and v_scale must be fp32 [batch, num_kv_heads, ceil(capacity / block_tokens)]")
         if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("the cache's tensors must be contiguous")
-        device = k.device
         if v.device != device or k_scale.device != device or v_scale.device != device:
             raise ValueError("the cache's tensors must be on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
@@ -98,13 +99,13 @@ def kv8_cache(batch, capacity, num_kv_heads, dtype=torch.float8_e4m3fn, kv_layou
 
 
 def _check_lens(name, t, batch, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or t.numel() != batch \
-            or t.device != device or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not _INT32 or t.shape != (batch,) or t.device != device \
+            or not t.is_contiguous():
         raise ValueError("%s must be a contiguous int32 tensor [batch] on the cache's device" % name)
 
 
 def _check_fp32(name, t, shape, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != shape or t.device != device or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not _FP32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError("%s must be a contiguous fp32 tensor of shape %s on the same device" % (name, list(shape)))
 
 
@@ -118,7 +119,9 @@ _Strides = ctypes.c_longlong * 3
 
 @functools.lru_cache(maxsize=1024)
 def _row_strides(s, kv_layout):
-    """{batch, token, head} of a [B,T,H,D] or [B,H,T,D] tensor's strides."""
+    """{batch, token, head} of a [B,T,H,D] or [B,H,T,D] tensor's strides; None if its rows are not contiguous and aligned."""
+    if s[3] != 1 or (s[0] | s[1] | s[2]) % 8:
+        return None
     return _Strides(s[0], s[1], s[2]) if kv_layout == KV_BSHD else _Strides(s[0], s[2], s[1])
 
 
@@ -130,24 +133,24 @@ def kv8_append(cache, k_new, v_new, seq_lens, new_lens=None):
     [B] (default: T for all): how many of the T rows are real.  Rows beyond the capacity are not stored.  A block that was
     partly filled keeps its scale unless the new rows need a larger one; then its old rows are re-rounded.
     """
-    for name, t in (("k_new", k_new), ("v_new", v_new)):
-        _require_cuda_bf16(name, t)
+    _require_cuda_bf16("k_new", k_new)
+    _require_cuda_bf16("v_new", v_new)
     _require_cuda(cache)
-    device = cache.k.device
-    if k_new.dim() != 4 or v_new.shape != k_new.shape:
+    device, layout, shape = cache.k.device, cache.kv_layout, k_new.shape
+    if len(shape) != 4 or v_new.shape != shape:
         raise ValueError("k_new and v_new must be of identical 4-D shape")
-    if cache.kv_layout == KV_BSHD:
-        B, T, H, D = k_new.shape
+    if layout == KV_BSHD:
+        B, T, H, D = shape
     else:
-        B, H, T, D = k_new.shape
+        B, H, T, D = shape
     if B != cache.batch or H != cache.num_kv_heads or D != HEAD_DIM:
         raise ValueError("k_new and v_new must match the cache's batch, kv heads and head_dim")
     if k_new.device != device or v_new.device != device:
         raise ValueError("k_new and v_new must be on the cache's device")
-    k_strides, v_strides = k_new.stride(), v_new.stride()
-    for name, t, s in (("k_new", k_new, k_strides), ("v_new", v_new, v_strides)):
-        if s[3] != 1 or (s[0] | s[1] | s[2]) % 8 or t.data_ptr() % 16:
-            raise ValueError("%s must have contiguous, 16-byte aligned rows" % name)
+    k_at, k_strides = k_new.data_ptr(), _row_strides(k_new.stride(), layout)
+    v_at, v_strides = v_new.data_ptr(), _row_strides(v_new.stride(), layout)
+    if k_strides is None or v_strides is None or k_at % 16 or v_at % 16:
+        raise ValueError("k_new and v_new must have contiguous, 16-byte aligned rows")
     _check_lens("seq_lens", seq_lens, B, device)
     if new_lens is not None:
         _check_lens("new_lens", new_lens, B, device)
@@ -155,10 +158,9 @@ def kv8_append(cache, k_new, v_new, seq_lens, new_lens=None):
         return
     with _on(device):
         rc = _lib.load().cllo_kv8_append_bf16(
-            k_new.data_ptr(), _row_strides(k_strides, cache.kv_layout), v_new.data_ptr(),
-            _row_strides(v_strides, cache.kv_layout), seq_lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
+            k_at, k_strides, v_at, v_strides, seq_lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(),
             cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), B, T,
-            cache.capacity, H, D, cache.kv_layout, cache.block_tokens, cache.format, _stream_ptr(device))
+            cache.capacity, H, D, layout, cache.block_tokens, cache.format, _stream_ptr(device))
     _lib.check(rc, "cllo_kv8_append_bf16")
 
 
@@ -196,11 +198,12 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
     _require_cuda_bf16("q", q)
     _require_cuda(cache)
     device = cache.k.device
-    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.shape[0] != cache.batch:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != HEAD_DIM or shape[0] != cache.batch:
         raise ValueError("expected q [B,Hq,%d] with the cache's batch" % HEAD_DIM)
     if not q.is_contiguous() or q.device != device:
         raise ValueError("q must be contiguous and on the cache's device")
-    B, Hq, D = q.shape
+    B, Hq, D = shape
     H = cache.num_kv_heads
     if Hq == 0 or Hq % H != 0:
         raise ValueError("Query heads must be divisible by KV heads")
@@ -211,7 +214,7 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
         scale = 1.0 / math.sqrt(D)
     if out is None:
         out = torch.empty_like(q)
-    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous() or out.device != device:
+    elif out.dtype != torch.bfloat16 or out.shape != shape or not out.is_contiguous() or out.device != device:
         raise ValueError("Output tensor must be contiguous bf16 of q's shape")
     if lse is not None:
         _check_fp32("lse", lse, (B, Hq), device)
@@ -220,14 +223,15 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
     lib = _lib.load()
     with _on(device):
         nbytes = _decode_workspace_bytes(device, B, cache.capacity, Hq, H, weights is not None, num_workers)
-        flag = 0
         if workspace is None:
             workspace, flag = _workspace("decode", device, nbytes)
+        else:
+            nbytes, flag = workspace.numel() * workspace.element_size(), 0
         rc = lib.cllo_kv8_decode_bf16(
             q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
             seq_lens.data_ptr(), scale, out.data_ptr(), None if lse is None else lse.data_ptr(),
-            None if weights is None else weights.data_ptr(), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), B, cache.capacity, Hq, H, D, cache.kv_layout | flag,
+            None if weights is None else weights.data_ptr(), workspace.data_ptr(), nbytes, B, cache.capacity, Hq, H, D,
+            cache.kv_layout | flag,
             cache.block_tokens, cache.format, num_workers, _stream_ptr(device))
     _lib.check(rc, "cllo_kv8_decode_bf16")
     return out
@@ -248,6 +252,11 @@ def _decode_workspace_bytes(device, B, capacity, Hq, Hkv, with_weights, num_work
     return n
 
 
+@functools.lru_cache(maxsize=64)
+def _sums_workspace_bytes(device_index):  # asked with that device current
+    return int(_lib.load().cllo_attn_weight_sums_workspace_bytes())
+
+
 def attention_weight_sums(q, k, lse, scale=None, causal=True, q_start=0, seq_lens=None, window=None, out=None,
                           accumulate=False, workspace=None):
     """How much weight a prompt's queries gave to every key: fp32 [B,Hkv,Skv].
@@ -258,13 +267,15 @@ def attention_weight_sums(q, k, lse, scale=None, causal=True, q_start=0, seq_len
     under a causal mask, query rows behind them do not count.  ``window``: only the last ``window`` query positions
     of each sequence count (default: all).  ``accumulate=True`` adds to ``out``.
     """
-    for name, t in (("q", q), ("k", k)):
-        _require_cuda_bf16(name, t)
-    if q.dim() != 4 or k.dim() != 4 or k.shape[0] != q.shape[0] or q.shape[3] != HEAD_DIM or k.shape[3] != HEAD_DIM:
+    _require_cuda_bf16("q", q)
+    _require_cuda_bf16("k", k)
+    q_shape, k_shape = q.shape, k.shape
+    if len(q_shape) != 4 or len(k_shape) != 4 or k_shape[0] != q_shape[0] or q_shape[3] != HEAD_DIM \
+            or k_shape[3] != HEAD_DIM:
         raise ValueError("expected q [B,Hq,Sq,%d] and k [B,Hkv,Skv,%d]" % (HEAD_DIM, HEAD_DIM))
-    B, Hq, Sq, D = q.shape
-    H, Skv = k.shape[1], k.shape[2]
-    if min(B, Hq, Sq, H, Skv) < 1:
+    B, Hq, Sq, D = q_shape
+    _, H, Skv, _ = k_shape
+    if not (B and Hq and Sq and H and Skv):
         raise ValueError("q and k must not be empty")
     if Hq % H != 0:
         raise ValueError("Query heads must be divisible by KV heads")
@@ -292,12 +303,15 @@ def attention_weight_sums(q, k, lse, scale=None, causal=True, q_start=0, seq_len
     with _on(device):
         flags = _lib.SUMS_ACCUMULATE if accumulate else 0
         if workspace is None:
-            workspace, zero = _workspace("sums", device, int(lib.cllo_attn_weight_sums_workspace_bytes()))
+            nbytes = _sums_workspace_bytes(device.index)
+            workspace, zero = _workspace("sums", device, nbytes)
             flags |= zero
+        else:
+            nbytes = workspace.numel() * workspace.element_size()
         rc = lib.cllo_attn_weight_sums_bf16(
             q.data_ptr(), k.data_ptr(), lse.data_ptr(), None if seq_lens is None else seq_lens.data_ptr(), scale,
             1 if causal else 0, q_start, min(window or 0, _MAX_POSITIONS), flags, out.data_ptr(), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), B, Sq, Skv, Hq, H, D, _stream_ptr(device))
+            nbytes, B, Sq, Skv, Hq, H, D, _stream_ptr(device))
     _lib.check(rc, "cllo_attn_weight_sums_bf16")
     return out
 
