@@ -1,13 +1,15 @@
 // Append to the 8-bit KV cache: bf16 K/V rows -> codes and block scales.
 //
-// One thread block handles one (batch, kv head, cache block, K or V).  Of the cache block's rows some may be old (the
-// sequence ended inside it), some are new, the rest lie behind the sequence and are left alone:
+// One thread block handles consecutive cache blocks of one (batch, kv head, K or V).  Of a cache block's rows some may be
+// old (the sequence ended inside it), some are new, the rest lie behind the sequence and are left alone:
 //     scale' = max(scale of the old rows, 2^e(amax of the new rows)),   code = rne(x / scale'),
 // and the old rows are re-rounded to scale' only if it grew.  The scale is that of format kv8_format.cuh: powers of two,
 // so x / scale' is a product and exact.
 //
 // Bound by memory: 2 B read and 1 B written per value.  The new rows are loaded once, 16 bytes per lane (half a warp per
-// row), and wait in registers for the block's amax.
+// row), and wait in registers for the block's amax, while the next cache block's rows are already on their way: 4 prompts of
+// 16384 tokens, 8 kv heads, 68 us, 5.9 TB/s (0.90 of a copy).  One token each for 60 sequences: 5 us, the latency of
+// lengths, rows and two barriers.
 #pragma once
 
 #include "host_util.cuh"
@@ -29,10 +31,6 @@ struct AppendParams {
     const int* new_lens;  // nullable
     int T, capacity, Hkv, n_blocks, blocks_touched, per_cta;
 };
-
-// a block of 128 tokens is two registers' worth of rows too many to hold twice
-template <int kBlock>
-constexpr bool kPrefetch = true;
 
 template <int kFmt, int kBlock>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
@@ -76,7 +74,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
         for (int i = 0; i < kPasses; ++i) x[i] = next[i];
         const bool has_old = row0 < held;
         const float old_scale = has_old ? scales[blk] : 0.f;
-        if (kPrefetch<kBlock> && blk + 1 < blk_end && row0 + kBlock < end) fetch(blk + 1);
+        if (blk + 1 < blk_end && row0 + kBlock < end) fetch(blk + 1);
         // the largest magnitude of the new rows, as bf16 bits; infinities and NaN, which do not take part, lie above all numbers
         uint32_t top = 0u;
 #pragma unroll
@@ -179,7 +177,8 @@ static int append_launch(const void* k_new, const long long* k_strides, const vo
     // T tokens starting anywhere inside a block reach this many blocks at most
     const int touched = (T - 1 + block - 1) / block + 1;
     p.blocks_touched = touched < p.n_blocks ? touched : p.n_blocks;
-    // cache blocks per thread block: several where there are enough to fill the GPU all the same
+    // Cache blocks per thread block: several, one loading while the one before it is turned into codes, where there are enough
+    // to fill the GPU all the same (4 prompts of 16384 tokens: 68.4 us with up to 8, 72.9 with one each; smaller calls get one).
     const long long per_cta = static_cast<long long>(B) * Hkv * p.blocks_touched * 2 / (static_cast<long long>(di->sm_count) * 16);
     p.per_cta = static_cast<int>(per_cta < 1 ? 1 : (per_cta > 8 ? 8 : per_cta));
     const long long blocks = static_cast<long long>(B) * Hkv * ((p.blocks_touched + p.per_cta - 1) / p.per_cta);

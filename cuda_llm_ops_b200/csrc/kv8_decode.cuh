@@ -5,6 +5,11 @@
 // over the seq_lens[b] tokens that the cache holds of sequence b; with `weights`, the probabilities of the step are
 // added to weights[b, kv head, t], summed over the query heads of the group in a fixed order.
 //
+// Measured: 60 x 4096 tokens, 128/8 heads, e4m3, tokens before heads: 97 us, 5.2 TB/s (0.80 of a copy), bound by the memory
+// system (the same copies without arithmetic: 96 us); 1,048,576 tokens, 64/8 heads, int8: 332 us, 0.99 of a copy; 17 sequences
+// of 0 to 16384 tokens, 40/8 heads, with weights: 57 us, 4.2 TB/s, bound by issue and by what short units cost; one sequence
+// of 1024 tokens: 14 us, a chain of latencies.
+//
 // Work decomposition, as in the bf16 decode kernel (gqa_decode.cuh): a unit is one (sequence, kv head, block of <= 16
 // query heads), cut into tiles of 64 tokens (at least one, so that an empty sequence writes its zeros); the tiles of all
 // units form one index space that W persistent blocks share evenly.  The lengths live on the device, so every block adds
@@ -307,8 +312,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     const int U = p.Hkv * p.n_gblk;
 
     if (warp >= kConsumerWarps) {
-        // The registers are given away, and the tensor maps fetched, while the consumers' first warps find the share and set up
-        // the barriers: giving them away afterwards put 2000 cycles between the share and the first copy.
+        // The registers are given away, and the tensor maps fetched, while the consumers' first warps set up the barriers and find
+        // the share (2700 cycles from the launch, 1300 of them the latency of the lengths).
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
         if (warp == kConsumerWarps && lane == 0) {
             tma_prefetch_desc(&tm_k);
@@ -318,7 +323,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         const int lo = share.lo, hi = share.hi, cost = share.cost;
         if (lo >= hi) return;
         // ------------------------------ producers ------------------------------
-        // One warp per consumer group, each with the group's own three stages: a wait, two tile copies and the scale copies
+        // One warp per consumer group, each with the group's own two stages: a wait, two tile copies and the scale copies
         // take the issuing thread about as long as a block at full bandwidth has for two tiles, so one producer for all
         // groups was what bounded the kernel.  Lane 0 copies the tiles, lanes 0-7 one block scale each (a quarter's K or V
         // scale); their arrivals are part of the stage's full barrier.  The last producer also brings the query rows, its lanes
@@ -810,7 +815,9 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     }
 }
 
-// weights[b, h, t] += sum over the group's heads, in order, of 2^(score - lse2); one thread per token
+// weights[b, h, t] += sum over the group's heads, in order, of 2^(score - lse2); one thread per token.  A kernel of its own since
+// a probability needs the normaliser of the whole sequence; the scores are 4 B per query head and token, mostly still in L2
+// (17 sequences of 0 to 16384 tokens, 40 heads: 8 us of the 57).
 constexpr int kWeightThreads = 256, kWeightTok = 1024;
 __global__ void __launch_bounds__(kWeightThreads) decode_weights_kernel(const DecodeParams p, float* weights, int n_chunks) {
     pdl_wait_prior_grid();  // scores and normalisers; by every block, so that this grid never ends before the decode's

@@ -77,7 +77,7 @@ __device__ __forceinline__ void cluster_load2(const int* p, uint32_t rank, int& 
 // once and stay in shared memory as integers; a pass counts the digits of the keys that share the prefix found so far
 // (equal digits of a warp are added together first: weights cluster in few exponents, and ties share every digit), the
 // blocks add up each other's counts over distributed shared memory, and every block finds the same digit.  Bound by the
-// latency of its passes: 5 cluster barriers, 8 block barriers.
+// latency of its passes, 5 cluster barriers and 8 block barriers: 32 rows of 32768 tokens 18 us, 264 of up to 2304 15 us.
 __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictParams p) {
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ __align__(8) int hist[3][kBins];  // one per pass
@@ -288,7 +288,8 @@ __host__ __device__ constexpr int gather_threads(int block) { return block * 4; 
 
 // One thread block per block of the second cache, one row per four lanes: all loads in flight before the first is looked at;
 // values -> amax -> new scale -> codes.  Bound by the latency of its gathers (position, then 128-byte rows) and by issue: what
-// a row costs besides its values (addresses, scales) is as much as the values cost, so a lane takes 32 bytes of each.
+// a row costs besides its values (addresses, scales) is as much as the values cost, so a lane takes 32 bytes of each (33 x 1152
+// to 2304 int8 tokens: 46 us, 5.1 TB/s; with 16 bytes of each of two rows per lane 60).
 template <int kFmt, int kBlock>
 __global__ void __launch_bounds__(gather_threads(kBlock)) gather_kernel(const EvictParams p) {
     constexpr int kThreads = gather_threads(kBlock);
@@ -448,7 +449,8 @@ static int evict_launch(const void* k, const void* v, const float* k_scale, cons
     p.block_shift = block_shift_of(block);
     const long long blocks = static_cast<long long>(rows) * p.n_blocks_to;
     if (blocks > 0x7fffffffLL) return CLLO_E_UNSUPPORTED;
-    // blocks per row: enough to fill the GPU, chunks of at least 2048 tokens
+    // blocks per row: enough to fill the GPU, chunks of at least 2048 tokens (both kernels of 32 rows of 32768 tokens: 31 us with
+    // four, 52 with one; 8 rows of 131072: 34 us with eight, 42 with as few as hold the keys)
     int cluster = 1;
     while (cluster < kMaxCluster && rows * cluster * 2 <= static_cast<size_t>(di->sm_count) && capacity / (cluster * 2) >= 2048) cluster *= 2;
     // rows longer than what one block holds in shared memory are shared out even on a full GPU
