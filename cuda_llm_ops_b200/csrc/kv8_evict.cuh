@@ -77,11 +77,11 @@ __device__ __forceinline__ void cluster_load2(const int* p, uint32_t rank, int& 
 // once and stay in shared memory as integers; a pass counts the digits of the keys that share the prefix found so far
 // (equal digits of a warp are added together first: weights cluster in few exponents, and ties share every digit), the
 // blocks add up each other's counts over distributed shared memory, and every block finds the same digit.  Bound by the
-// latency of its passes, 5 cluster barriers and 8 block barriers: 32 rows of 32768 tokens 18 us, 264 of up to 2304 15 us.
+// latency of its passes, 5 cluster barriers and 9 block barriers: 32 rows of 32768 tokens 18 us, 264 of up to 2304 15 us.
 __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictParams p) {
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ __align__(8) int hist[3][kBins];  // one per pass
-    __shared__ int warp_sum[kSelectThreads / 32];
+    __shared__ int group_sum[3][32];             // of kBins / 32 bins each
     __shared__ int s_digit, s_need;
     __shared__ int s_counts[2];  // this block's tokens that stay whatever the others hold, and those at the threshold
     pdl_launch_dependents();  // the moving blocks may take their places; they wait for this grid's end
@@ -90,6 +90,11 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
     const int C = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
     const int row = blockIdx.x / C;
     const int h = row % p.Hkv, b = row / p.Hkv;
+    {  // the row's weights set out for L2 while the length is on its way
+        const int part = (p.capacity + C - 1) / C, end = part * (rank + 1) < p.capacity ? part * (rank + 1) : p.capacity;
+        const float* all = p.weights + static_cast<long long>(row) * p.capacity;
+        for (int i = part * rank + tid * 32; i < end; i += kSelectThreads * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(all + i));
+    }
     const int len = clamp_len(p.seq_lens[b], p.capacity);
     int* idx = p.indices + static_cast<long long>(row) * p.budget;
     const int kept = len < p.budget ? len : p.budget;
@@ -156,39 +161,54 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
             }
 #pragma unroll 1
             for (int i0 = n_smem; i0 < n; i0 += kSelectThreads) count(i0 + tid < n ? key_at(i0 + tid) : 0u);
-            cluster_sync();
-            // sum over the cluster, then the largest digit at which the count from the top reaches `need`: two bins a thread,
-            // highest first
-            int part[kMaxCluster][2], c[2] = {0, 0};
-#pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) {
-                part[r][0] = part[r][1] = 0;
-                if (r < C) cluster_load2(&counts[kBins - 2 - 2 * tid], r, part[r][1], part[r][0]);
-            }
-#pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) {
-                c[0] += part[r][0];
-                c[1] += part[r][1];
-            }
-            int v = c[0] + c[1];
-            const int mine = v;
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += u;
-            }
-            if (lane == 31) warp_sum[warp] = v;
+            // The largest digit at which the count from the top reaches `need`, over the whole cluster: first its group of 64
+            // bins by the groups' sums, then the bin; few words cross between the blocks (all 2048 bins of every other block: 1000
+            // cycles more a pass).
             __syncthreads();
-            int others = lane < warp ? warp_sum[lane] : 0;
+            {
+                const int2 x = *reinterpret_cast<const int2*>(&counts[64 * warp + 2 * lane]);
+                const int sum = __reduce_add_sync(0xffffffffu, x.x + x.y);
+                if (lane == 0) group_sum[pass][warp] = sum;
+            }
+            cluster_sync();
+            if (warp == 0) {
+                auto from_top = [&](int v) {  // inclusive sum over the lanes
 #pragma unroll
-            for (int o = 16; o; o >>= 1) others += __shfl_xor_sync(0xffffffffu, others, o);
-            int before = others + v - mine;  // keys in higher bins
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int u = __shfl_up_sync(0xffffffffu, v, o);
+                        if (lane >= o) v += u;
+                    }
+                    return v;
+                };
+                int part[kMaxCluster][2], c[2] = {0, 0};
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (before < need && need <= before + c[u]) {
-                    s_digit = kBins - 1 - (2 * tid + u);
-                    s_need = need - before;
+                for (int r = 0; r < kMaxCluster; ++r) part[r][0] = r < C ? cluster_load(&group_sum[pass][31 - lane], r) : 0;
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) c[0] += part[r][0];
+                int v = from_top(c[0]);
+                const int at = __ffs(__ballot_sync(0xffffffffu, v - c[0] < need && need <= v)) - 1;
+                int before = __shfl_sync(0xffffffffu, v - c[0], at);  // keys in higher groups
+                const int top = 64 * (31 - at) + 63 - 2 * lane;       // this lane's higher bin of the group
+                c[0] = c[1] = 0;
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) {
+                    part[r][0] = part[r][1] = 0;
+                    if (r < C) cluster_load2(&counts[top - 1], r, part[r][1], part[r][0]);
                 }
-                before += c[u];
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) {
+                    c[0] += part[r][0];
+                    c[1] += part[r][1];
+                }
+                before += from_top(c[0] + c[1]) - c[0] - c[1];  // keys in higher bins
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (before < need && need <= before + c[u]) {
+                        s_digit = top - u;
+                        s_need = need - before;
+                    }
+                    before += c[u];
+                }
             }
             __syncthreads();
             prefix |= static_cast<uint32_t>(s_digit) << shift;
