@@ -36,7 +36,12 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kSelectThreads = 1024;
+// Threads of a selecting block: 1024, or 512 where its chunk of a row is small (8 rows of 4096 tokens in two blocks each, with
+// the moving kernel: 12.7 us with 1024, 11.7 with 512) and where there are more rows than SMs, so that two blocks share one (512
+// rows of 2048: 66 and 47 us; 160 rows of 2304: 35 and 27).  Else 1024 (144 rows of 2752: 23.6 and 24.2 us, of 8192 44 and 47).
+constexpr int kSelectThreads = 1024, kSelectThreadsHalf = 512;
+constexpr int kSmallChunk = 2048;
+constexpr int kHalfMaxTokens = 16384;                          // what two blocks hold in shared memory beside each other
 constexpr int kDigitBits = 11, kBins = 1 << kDigitBits;      // three passes: 11, 11 and 10 bits
 constexpr int kMaxCluster = 8;
 constexpr int kKeysInSmem = 48 * 1024;                         // of a block's chunk; what is longer is read again in each pass
@@ -77,8 +82,10 @@ __device__ __forceinline__ void cluster_load2(const int* p, uint32_t rank, int& 
 // once and stay in shared memory as integers; a pass counts the digits of the keys that share the prefix found so far
 // (equal digits of a warp are added together first: weights cluster in few exponents, and ties share every digit), the
 // blocks add up each other's counts over distributed shared memory, and every block finds the same digit.  Bound by the
-// latency of its passes, 5 cluster barriers and 9 block barriers: 32 rows of 32768 tokens 18 us, 264 of up to 2304 15 us.
-__global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictParams p) {
+// latency of its passes, 5 cluster barriers and 9 block barriers: 32 rows of 32768 tokens 16 us, 264 of up to 2304 14 us.
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads, kSelectThreads / kThreads) select_kernel(const EvictParams p) {
+    constexpr int kWarps = kThreads / 32;
     extern __shared__ __align__(16) uint32_t keys[];
     __shared__ __align__(8) int hist[3][kBins];  // one per pass
     __shared__ int group_sum[3][32];             // of kBins / 32 bins each
@@ -86,22 +93,22 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
     __shared__ int s_counts[2];  // this block's tokens that stay whatever the others hold, and those at the threshold
     pdl_launch_dependents();  // the moving blocks may take their places; they wait for this grid's end
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    for (int i = tid; i < 3 * kBins; i += kSelectThreads) hist[0][i] = 0;
+    for (int i = tid; i < 3 * kBins; i += kThreads) hist[0][i] = 0;
     const int C = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
     const int row = blockIdx.x / C;
     const int h = row % p.Hkv, b = row / p.Hkv;
     {  // the row's weights set out for L2 while the length is on its way
         const int part = (p.capacity + C - 1) / C, end = part * (rank + 1) < p.capacity ? part * (rank + 1) : p.capacity;
         const float* all = p.weights + static_cast<long long>(row) * p.capacity;
-        for (int i = part * rank + tid * 32; i < end; i += kSelectThreads * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(all + i));
+        for (int i = part * rank + tid * 32; i < end; i += kThreads * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(all + i));
     }
     const int len = clamp_len(p.seq_lens[b], p.capacity);
     int* idx = p.indices + static_cast<long long>(row) * p.budget;
     const int kept = len < p.budget ? len : p.budget;
     if (h == 0 && tid == 0 && rank == 0) p.new_lens[b] = kept;
-    for (int j = kept + rank * kSelectThreads + tid; j < p.budget; j += C * kSelectThreads) idx[j] = -1;
+    for (int j = kept + rank * kThreads + tid; j < p.budget; j += C * kThreads) idx[j] = -1;
     if (len <= p.budget) {  // the whole cluster alike
-        for (int j = rank * kSelectThreads + tid; j < len; j += C * kSelectThreads) idx[j] = j;
+        for (int j = rank * kThreads + tid; j < len; j += C * kThreads) idx[j] = j;
         return;
     }
     const int chunk = (len + C - 1) / C;
@@ -113,16 +120,16 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
     // The key of a token that is no candidate is 0, which no weight has: order_key is at least that of -infinity.
     auto candidate_key = [&](int i, float x) { return i >= lo && i < hi ? order_key(x) : 0u; };
     const int n_pad = (n_smem + 3) & ~3;
-    for (int i0 = tid; i0 < n_pad; i0 += kSelectThreads * kSelectUnroll) {
+    for (int i0 = tid; i0 < n_pad; i0 += kThreads * kSelectUnroll) {
         float x[kSelectUnroll];
 #pragma unroll
         for (int u = 0; u < kSelectUnroll; ++u) {
-            const int i = i0 + u * kSelectThreads;
+            const int i = i0 + u * kThreads;
             x[u] = i < n_smem ? __ldg(w + i) : 0.f;
         }
 #pragma unroll
         for (int u = 0; u < kSelectUnroll; ++u) {
-            const int i = i0 + u * kSelectThreads;
+            const int i = i0 + u * kThreads;
             if (i < n_pad) keys[i] = i < n_smem ? candidate_key(i, x[u]) : 0u;
         }
     }
@@ -152,7 +159,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
             };
             const int quads = n_pad / 4;
 #pragma unroll 2
-            for (int q0 = 0; q0 < quads; q0 += kSelectThreads) {
+            for (int q0 = 0; q0 < quads; q0 += kThreads) {
                 const uint4 k4 = q0 + tid < quads ? reinterpret_cast<const uint4*>(keys)[q0 + tid] : make_uint4(0u, 0u, 0u, 0u);
                 count(k4.x);
                 count(k4.y);
@@ -160,15 +167,16 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
                 count(k4.w);
             }
 #pragma unroll 1
-            for (int i0 = n_smem; i0 < n; i0 += kSelectThreads) count(i0 + tid < n ? key_at(i0 + tid) : 0u);
+            for (int i0 = n_smem; i0 < n; i0 += kThreads) count(i0 + tid < n ? key_at(i0 + tid) : 0u);
             // The largest digit at which the count from the top reaches `need`, over the whole cluster: first its group of 64
             // bins by the groups' sums, then the bin; few words cross between the blocks (all 2048 bins of every other block: 1000
             // cycles more a pass).
             __syncthreads();
-            {
-                const int2 x = *reinterpret_cast<const int2*>(&counts[64 * warp + 2 * lane]);
+#pragma unroll
+            for (int g = warp; g < 32; g += kWarps) {
+                const int2 x = *reinterpret_cast<const int2*>(&counts[64 * g + 2 * lane]);
                 const int sum = __reduce_add_sync(0xffffffffu, x.x + x.y);
-                if (lane == 0) group_sum[pass][warp] = sum;
+                if (lane == 0) group_sum[pass][g] = sum;
             }
             cluster_sync();
             if (warp == 0) {
@@ -230,7 +238,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
         }
     };
     // a warp owns a contiguous stretch of the chunk, so that only the warps' totals have to meet
-    const int per_warp = ((n + kSelectThreads / 32 - 1) / (kSelectThreads / 32) + 31) / 32 * 32;
+    const int per_warp = ((n + kWarps - 1) / (kWarps) + 31) / 32 * 32;
     const int w_lo = warp * per_warp, w_hi = w_lo + per_warp < n ? w_lo + per_warp : n;
     int n_above = 0, n_equal = 0;
     unsigned kept_above = 0u, kept_equal = 0u;  // lane k: the warp's answers of its k-th step
@@ -253,7 +261,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) select_kernel(const EvictPa
     }
     __syncthreads();
     if (warp == 0) {
-        int a = totals[2 * lane], e = totals[2 * lane + 1];
+        int a = lane < kWarps ? totals[2 * lane] : 0, e = lane < kWarps ? totals[2 * lane + 1] : 0;
         for (int o = 16; o; o >>= 1) {
             a += __shfl_xor_sync(0xffffffffu, a, o);
             e += __shfl_xor_sync(0xffffffffu, e, o);
@@ -479,12 +487,15 @@ static int evict_launch(const void* k, const void* v, const float* k_scale, cons
     const int smem = (chunk < kKeysInSmem ? chunk : kKeysInSmem) * 4;
     if (rows * cluster > 0x7fffffffULL) return CLLO_E_UNSUPPORTED;
     if (!di->kv8_select_attr_set) {
-        CLLO_CUDA_TRY(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeysInSmem * 4));
+        CLLO_CUDA_TRY(cudaFuncSetAttribute(select_kernel<kSelectThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeysInSmem * 4));
+        CLLO_CUDA_TRY(cudaFuncSetAttribute(select_kernel<kSelectThreadsHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           kHalfMaxTokens * 4));
         di->kv8_select_attr_set = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster));
-    cfg.blockDim = dim3(kSelectThreads);
+    const bool half = chunk <= kSmallChunk || (rows > static_cast<size_t>(di->sm_count) && chunk <= kHalfMaxTokens);
+    cfg.blockDim = dim3(half ? kSelectThreadsHalf : kSelectThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr = {};
@@ -493,7 +504,7 @@ static int evict_launch(const void* k, const void* v, const float* k_scale, cons
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    CLLO_CUDA_TRY(cudaLaunchKernelEx(&cfg, select_kernel, p));
+    CLLO_CUDA_TRY(cudaLaunchKernelEx(&cfg, half ? select_kernel<kSelectThreadsHalf> : select_kernel<kSelectThreads>, p));
     const unsigned grid = static_cast<unsigned>(blocks);
     CLLO_CUDA_TRY((format == CLLO_FMT_E4M3 ? gather_dispatch<CLLO_FMT_E4M3> : gather_dispatch<CLLO_FMT_INT8>)(p, block, grid, st));
     return CLLO_OK;

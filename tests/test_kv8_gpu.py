@@ -528,6 +528,17 @@ def test_evict(dtype, B, S, H, block, layout, lens, budget, sink, recent):
     assert_clean_status()
 
 
+@pytest.mark.parametrize("B,S,H,budget", [
+    (40, 2300, 4, 700),      # more rows than SMs, chunks beyond 2048 tokens
+    (1, 2048, 3, 100),       # a chunk of 2048 tokens
+    (1, 2049, 3, 2000),      # and of one more
+    (3, 9000, 8, 1500),      # several blocks a row
+])
+def test_evict_in_blocks_of_either_size(B, S, H, budget):
+    lens = [S - 3 * b for b in range(B)]
+    test_evict(torch.int8, B, S, H, 32, 0, lens, budget, 4, 64)
+
+
 def test_evict_of_special_weights():
     """All equal, negative, zeros of both signs, infinities, NaN."""
     ops = _ops()
