@@ -307,7 +307,7 @@ int cllo_rope_bf16(const void* input, void* output, int B, int S, int hidden, fl
  *   scales  [B,Hkv,ceil(capacity / block_tokens)] fp32;  block_tokens = 16, 32, 64 or 128
  * The library writes power-of-two scales: the smallest 2^e, -60 <= e <= 60, with amax <= qmax * 2^e over the block's
  * finite values (qmax = 448 or 127); infinities and what is beyond 2^60 * qmax saturate, a NaN is kept by e4m3 and becomes
- * 0 as an integer.  The attention reads any positive scales within [2^-60, 2^60].
+ * 0 as an integer.  The attention reads any positive scales within [2^-60, 2^60], and 0 with codes that are 0.
  * seq_lens [B] int32 are lengths on the device, so a captured graph follows them; a length outside [0, capacity] is held
  * to that range.  capacity <= 2^30.  D = 128.
  */
