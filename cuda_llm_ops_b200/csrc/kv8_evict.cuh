@@ -46,6 +46,8 @@ constexpr int kDigitBits = 11, kBins = 1 << kDigitBits;      // three passes: 11
 constexpr int kMaxCluster = 8;
 constexpr int kKeysInSmem = 48 * 1024;                         // of a block's chunk; what is longer is read again in each pass
 constexpr int kSelectUnroll = 8;
+// Keys that a chunk of n tokens takes in shared memory: whole groups of four, since they are counted four at a time.
+__host__ __device__ constexpr int keys_in_smem(int n) { return ((n < kKeysInSmem ? n : kKeysInSmem) + 3) & ~3; }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, kSelectThreads / kThreads) select_ke
     const int n_smem = n < kKeysInSmem ? n : kKeysInSmem;
     // The key of a token that is no candidate is 0, which no weight has: order_key is at least that of -infinity.
     auto candidate_key = [&](int i, float x) { return i >= lo && i < hi ? order_key(x) : 0u; };
-    const int n_pad = (n_smem + 3) & ~3;
+    const int n_pad = keys_in_smem(n);
     for (int i0 = tid; i0 < n_pad; i0 += kThreads * kSelectUnroll) {
         float x[kSelectUnroll];
 #pragma unroll
@@ -484,7 +486,7 @@ static int evict_launch(const void* k, const void* v, const float* k_scale, cons
     // rows longer than what one block holds in shared memory are shared out even on a full GPU
     while (cluster < kMaxCluster && capacity / cluster > kKeysInSmem) cluster *= 2;
     const int chunk = (capacity + cluster - 1) / cluster;
-    const int smem = (chunk < kKeysInSmem ? chunk : kKeysInSmem) * 4;
+    const int smem = keys_in_smem(chunk) * 4;
     if (rows * cluster > 0x7fffffffULL) return CLLO_E_UNSUPPORTED;
     if (!di->kv8_select_attr_set) {
         CLLO_CUDA_TRY(cudaFuncSetAttribute(select_kernel<kSelectThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeysInSmem * 4));

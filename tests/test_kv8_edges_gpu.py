@@ -1,0 +1,76 @@
+"""The 8-bit KV cache operators at sizes, values and calls that are easy to get wrong."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import kv8_ref as ref
+from gpu_util import assert_clean_status
+from test_kv8_gpu import _check_evict, _filled_cache, _gen, _garbage_cache, _ints, _ops
+
+pytestmark = pytest.mark.gpu
+D = 128
+E4M3 = torch.float8_e4m3fn
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# eviction: chunks of a row that are no multiple of four tokens
+# ------------------------------------------------------------------------------------------------------------------
+class _KernelNodeParams(ctypes.Structure):  # CUDA_KERNEL_NODE_PARAMS of the driver interface
+    _fields_ = [("func", ctypes.c_void_p)] + [(n, ctypes.c_uint) for n in ("gx", "gy", "gz", "bx", "by", "bz", "smem")] + \
+               [("params", ctypes.c_void_p), ("extra", ctypes.c_void_p), ("kern", ctypes.c_void_p), ("ctx", ctypes.c_void_p)]
+
+
+def _captured_kernels(call):
+    """(grid, block, dynamic shared memory) of every kernel that `call` launches; it is captured and never run."""
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    cuda = ctypes.CDLL("libcuda.so.1")
+    raw = ctypes.c_void_p(graph.raw_cuda_graph())
+    n = ctypes.c_size_t(0)
+    assert cuda.cuGraphGetNodes(raw, None, ctypes.byref(n)) == 0
+    nodes = (ctypes.c_void_p * n.value)()
+    assert cuda.cuGraphGetNodes(raw, nodes, ctypes.byref(n)) == 0
+    found = []
+    for node in nodes:
+        kind = ctypes.c_int(-1)
+        assert cuda.cuGraphNodeGetType(ctypes.c_void_p(node), ctypes.byref(kind)) == 0
+        if kind.value == 0:
+            p = _KernelNodeParams()
+            assert cuda.cuGraphKernelNodeGetParams_v2(ctypes.c_void_p(node), ctypes.byref(p)) == 0
+            found.append((p.gx, p.bx, p.smem))
+    return found
+
+
+@pytest.mark.parametrize("B,S,H", [(1, 1, 1), (1, 30, 1), (1, 2049, 3), (1, 2050, 1), (3, 4099, 50), (1, 4999, 40), (2, 20483, 2)])
+def test_evict_has_shared_memory_for_every_key_that_it_writes(B, S, H):
+    """The keys of a chunk are written and read in groups of four: the last group belongs to what the launch asks for."""
+    ops = _ops()
+    cache = ops.kv8_cache(B, S, H)
+    weights, lens = torch.zeros(B, H, S, device="cuda"), _ints([S] * B)
+    out = ops.kv8_cache(B, 1, H)
+    select = [k for k in _captured_kernels(lambda: ops.kv8_evict(cache, weights, lens, 1, out=out)) if k[2]]
+    assert len(select) == 1
+    grid, _, smem = select[0]
+    chunk = -(-S // (grid // (B * H)))
+    assert smem >= 4 * (-(-chunk // 4) * 4), (chunk, smem)
+
+
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+@pytest.mark.parametrize("B,S,H,budget", [
+    (1, 29, 1, 9), (2, 2049, 3, 1000), (1, 2050, 1, 77), (1, 2051, 2, 2050), (3, 4099, 50, 65), (2, 20483, 2, 3000),
+    (1, 8 * 48 * 1024 + 3, 1, 513),  # chunks of one more than what shared memory holds
+])
+def test_evict_of_rows_of_any_length(dtype, B, S, H, budget):
+    ops = _ops()
+    lens = [S - 2 * b for b in range(B)]
+    cache = _filled_cache(300, B, S, H, dtype, 1, 64, lens)
+    weights = torch.rand(B, H, S, generator=_gen(301), device="cuda")
+    weights[:, :, -5:] += 1  # the tail of the last group among the kept
+    out = _garbage_cache(302, B, budget, H, dtype, 1, 64)
+    before = [t.view(torch.uint8).clone() for t in (out.k, out.v)]
+    result = ops.kv8_evict(cache, weights, _ints(lens), budget, sink=1, recent=2, out=out)
+    _check_evict(cache, weights, lens, budget, 1, 2, result, before)
+    assert_clean_status()
