@@ -441,13 +441,23 @@ static int evict_launch(const void* k, const void* v, const float* k_scale, cons
     const size_t rows = static_cast<size_t>(B) * Hkv;
     const size_t n = rows * capacity * kD, n_to = rows * capacity_to * kD;
     const size_t n_scale = rows * ((capacity + block - 1) / block) * 4, n_scale_to = rows * ((capacity_to + block - 1) / block) * 4;
-    // rows move while others are still being read: the caches (and the weights) may not share memory
-    if (ranges_overlap(k, n, k_to, n_to) || ranges_overlap(k, n, v_to, n_to) || ranges_overlap(v, n, k_to, n_to) ||
-        ranges_overlap(v, n, v_to, n_to) ||
-        ranges_overlap(k_scale, n_scale, k_scale_to, n_scale_to) || ranges_overlap(k_scale, n_scale, v_scale_to, n_scale_to) ||
-        ranges_overlap(v_scale, n_scale, k_scale_to, n_scale_to) || ranges_overlap(v_scale, n_scale, v_scale_to, n_scale_to) ||
-        (weights_to && ranges_overlap(weights, rows * capacity * 4, weights_to, rows * capacity_to * 4)))
-        return CLLO_E_BAD_ARG;
+    // Blocks read while others write: no tensor written to may share memory with one that is read, or with another one written to.
+    struct Range {
+        const void* at;
+        size_t bytes;
+    };
+    const Range written[] = {{k_to, n_to}, {v_to, n_to}, {k_scale_to, n_scale_to}, {v_scale_to, n_scale_to},
+                             {new_lens, static_cast<size_t>(B) * 4}, {indices, rows * budget * 4},
+                             {weights_to, weights_to ? rows * capacity_to * 4 : 0}};
+    const Range read[] = {{k, n}, {v, n}, {k_scale, n_scale}, {v_scale, n_scale}, {weights, rows * capacity * 4},
+                          {seq_lens, static_cast<size_t>(B) * 4}};
+    for (const Range* w = written; w != written + 7; ++w) {
+        if (w->bytes == 0) continue;
+        for (const Range& r : read)
+            if (ranges_overlap(w->at, w->bytes, r.at, r.bytes)) return CLLO_E_BAD_ARG;
+        for (const Range* o = written; o != w; ++o)
+            if (ranges_overlap(w->at, w->bytes, o->at, o->bytes)) return CLLO_E_BAD_ARG;
+    }
     DeviceInfo* di = nullptr;
     int rc = current_device_info(&di);
     if (rc != CLLO_OK) return rc;

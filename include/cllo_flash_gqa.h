@@ -366,7 +366,7 @@ int cllo_attn_weight_sums_bf16(const void* q, const void* k, const float* lse, c
  * size and format; capacity_to >= min(budget, capacity)), whose block scales are computed anew; weights_to (nullable,
  * [B,Hkv,capacity_to]) receives the kept weights, indices [B,Hkv,budget] the kept positions (-1 behind them) and
  * new_lens [B] = min(seq_lens, budget).  Rows behind new_lens are left as they were.  No tensor written to may overlap one
- * that is read (CLLO_E_BAD_ARG).
+ * that is read -- new_lens may not be seq_lens -- or another one written to (CLLO_E_BAD_ARG).
  */
 int cllo_kv8_evict(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                    const float* weights, const int* seq_lens, void* k_to, void* v_to, float* k_scale_to,

@@ -1,0 +1,41 @@
+"""The 8-bit KV cache operators at calls that are easy to get wrong, as far as they are answered without a GPU."""
+import itertools
+
+import pytest
+import torch
+
+# cllo_kv8_evict with B = 1, one kv head, 64 tokens cut to 32, blocks of 16: what is read, what is written, and their bytes
+READ = dict(k=64 * 128, v=64 * 128, k_scale=16, v_scale=16, weights=256, seq_lens=4)
+WRITTEN = dict(k_to=32 * 128, v_to=32 * 128, k_scale_to=8, v_scale_to=8, weights_to=128, new_lens=4, indices=128)
+
+
+def _evict(lib, **at):
+    """The status of the call with every tensor in a place of its own, except where `at` says."""
+    place = {n: (i + 1) << 24 for i, n in enumerate([*READ, *WRITTEN])}
+    place.update(at)
+    return lib.cllo_kv8_evict(*(place[n] for n in (*READ, "k_to", "v_to", "k_scale_to", "v_scale_to", "weights_to", "new_lens",
+                                                   "indices")), 1, 64, 32, 1, 128, 32, 0, 0, 1, 16, 0, None)
+
+
+def test_evict_refuses_tensors_that_share_memory(built_library):
+    """Lengths updated in place among them: blocks read the old lengths while another writes the new ones."""
+    from cuda_llm_ops_b200 import _lib
+    lib = _lib.load()
+    if torch.cuda.is_available():
+        pytest.skip("the calls that are not refused would launch on these addresses")
+    assert _evict(lib) not in (_lib.OK, _lib.E_BAD_ARG)  # no device
+    sizes = {**READ, **WRITTEN}
+    place = {n: (i + 1) << 24 for i, n in enumerate(sizes)}
+    pairs = list(itertools.product(WRITTEN, READ)) + list(itertools.permutations(WRITTEN, 2))
+    for w, other in pairs:
+        step = 16 if w in ("k_to", "v_to") else 4
+        for at in (place[other], place[other] + sizes[other] - sizes[other] % 16 - (step if sizes[other] % 16 == 0 else 0),
+                   place[other] - sizes[w] + step):
+            if step == 16:
+                at -= at % 16
+            if at < place[other] + sizes[other] and place[other] < at + sizes[w]:
+                assert _evict(lib, **{w: at}) == _lib.E_BAD_ARG, (w, other, at - place[other])
+        if step == 4 or sizes[other] % 16 == 0:  # next to each other is fine
+            assert _evict(lib, **{w: place[other] + sizes[other]}) not in (_lib.OK, _lib.E_BAD_ARG), (w, other)
+    assert _evict(lib, seq_lens=1 << 20, new_lens=1 << 20) == _lib.E_BAD_ARG
+    assert _evict(lib, weights_to=None) not in (_lib.OK, _lib.E_BAD_ARG)
