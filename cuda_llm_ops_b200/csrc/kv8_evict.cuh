@@ -437,6 +437,10 @@ static int evict_launch(const void* k, const void* v, const float* k_scale, cons
     if (!valid_format(format) || !valid_block(block)) return CLLO_E_BAD_ARG;
     if (D != kD) return CLLO_E_UNSUPPORTED;
     if (!aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(k_to, 16) || !aligned_to(v_to, 16)) return CLLO_E_BAD_ARG;
+    if (!aligned_to(k_scale, 4) || !aligned_to(v_scale, 4) || !aligned_to(weights, 4) || !aligned_to(seq_lens, 4) ||
+        !aligned_to(k_scale_to, 4) || !aligned_to(v_scale_to, 4) || !aligned_to(weights_to, 4) || !aligned_to(new_lens, 4) ||
+        !aligned_to(indices, 4))
+        return CLLO_E_BAD_ARG;
     if (capacity > kMaxCapacity || capacity_to > kMaxCapacity) return CLLO_E_UNSUPPORTED;
     const size_t rows = static_cast<size_t>(B) * Hkv;
     const size_t n = rows * capacity * kD, n_to = rows * capacity_to * kD;

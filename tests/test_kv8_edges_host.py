@@ -39,3 +39,13 @@ def test_evict_refuses_tensors_that_share_memory(built_library):
             assert _evict(lib, **{w: place[other] + sizes[other]}) not in (_lib.OK, _lib.E_BAD_ARG), (w, other)
     assert _evict(lib, seq_lens=1 << 20, new_lens=1 << 20) == _lib.E_BAD_ARG
     assert _evict(lib, weights_to=None) not in (_lib.OK, _lib.E_BAD_ARG)
+
+
+def test_evict_refuses_misaligned_tensors(built_library):
+    """Rows move 16 bytes at a time, everything else is read and written as 32-bit words."""
+    from cuda_llm_ops_b200 import _lib
+    lib = _lib.load()
+    place = {n: (i + 1) << 24 for i, n in enumerate([*READ, *WRITTEN])}
+    for name, at in place.items():
+        for off in (8, 4) if name in ("k", "v", "k_to", "v_to") else (1, 2, 3):
+            assert _evict(lib, **{name: at + off}) == _lib.E_BAD_ARG, (name, off)
