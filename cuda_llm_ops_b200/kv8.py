@@ -109,6 +109,11 @@ def _check_fp32(name, t, shape, device):
         raise ValueError("%s must be a contiguous fp32 tensor of shape %s on the same device" % (name, list(shape)))
 
 
+def _check_workspace(t, device):
+    if not isinstance(t, torch.Tensor) or t.device != device or not t.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on the device of the call")
+
+
 def _require_cuda(cache):
     if not cache.k.is_cuda:
         raise RuntimeError("the cache must be on a CUDA device: this library has no CPU path")
@@ -226,6 +231,7 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
         if workspace is None:
             workspace, flag = _workspace("decode", device, nbytes)
         else:
+            _check_workspace(workspace, device)
             nbytes, flag = workspace.numel() * workspace.element_size(), 0
         rc = lib.cllo_kv8_decode_bf16(
             q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
@@ -307,6 +313,7 @@ def attention_weight_sums(q, k, lse, scale=None, causal=True, q_start=0, seq_len
             workspace, zero = _workspace("sums", device, nbytes)
             flags |= zero
         else:
+            _check_workspace(workspace, device)
             nbytes = workspace.numel() * workspace.element_size()
         rc = lib.cllo_attn_weight_sums_bf16(
             q.data_ptr(), k.data_ptr(), lse.data_ptr(), None if seq_lens is None else seq_lens.data_ptr(), scale,

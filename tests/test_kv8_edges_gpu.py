@@ -74,3 +74,20 @@ def test_evict_of_rows_of_any_length(dtype, B, S, H, budget):
     result = ops.kv8_evict(cache, weights, _ints(lens), budget, sink=1, recent=2, out=out)
     _check_evict(cache, weights, lens, budget, 1, 2, result, before)
     assert_clean_status()
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# workspaces
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("make", [lambda n: torch.zeros(n, dtype=torch.uint8),
+                                  lambda n: torch.zeros(2 * n, dtype=torch.uint8, device="cuda")[::2],
+                                  lambda n: torch.zeros(n // 1024, 1024, dtype=torch.uint8, device="cuda").t()])
+def test_workspaces_that_a_kernel_could_not_write_are_refused(make):
+    ops = _ops()
+    ws = make(1 << 24)
+    cache = ops.kv8_cache(1, 64, 1)
+    q = torch.zeros(1, 2, D, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="workspace"):
+        ops.kv8_decode(q, cache, _ints([64]), workspace=ws)
+    with pytest.raises(ValueError, match="workspace"):
+        ops.attention_weight_sums(q[:, :, None], q[:, :1, None], torch.zeros(1, 2, 1, device="cuda"), workspace=ws)

@@ -49,3 +49,16 @@ def test_evict_refuses_misaligned_tensors(built_library):
     for name, at in place.items():
         for off in (8, 4) if name in ("k", "v", "k_to", "v_to") else (1, 2, 3):
             assert _evict(lib, **{name: at + off}) == _lib.E_BAD_ARG, (name, off)
+
+
+def test_workspaces_that_a_kernel_could_not_write(built_library):
+    """One of another device, or with gaps between its elements, is refused before its address is taken."""
+    from cuda_llm_ops_b200 import kv8
+    cpu, cuda = torch.device("cpu"), torch.device("cuda", 0)
+    kv8._check_workspace(torch.zeros(4096, dtype=torch.uint8), cpu)
+    kv8._check_workspace(torch.zeros(4, 1024), cpu)
+    for t, device in ((torch.zeros(4096, dtype=torch.uint8), cuda), (torch.zeros(4096, dtype=torch.uint8, device="meta"), cpu),
+                      (torch.zeros(4096, dtype=torch.uint8)[::2], cpu), (torch.zeros(64, 64).t(), cpu), (bytearray(4096), cpu),
+                      (4096, cpu)):
+        with pytest.raises(ValueError, match="workspace"):
+            kv8._check_workspace(t, device)
