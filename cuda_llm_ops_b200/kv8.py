@@ -177,8 +177,8 @@ _counted_workspaces.append(_workspaces)
 def _workspace(kind, device, nbytes):
     """(scratch, flag): scratch whose arrival counters are zero, and the flag that vouches for it.
 
-    Eager calls of one kind share one tensor per (device, stream): calls on one stream do not overlap, and the kernel leaves the
-    counters zero.  A call that is being captured gets a tensor of its own from the graph's pool, and the call clears the
+    Eager calls of one kind share one tensor per (device, stream): launches on one stream do not overlap, and the kernel leaves
+    the counters zero.  A call that is being captured gets a tensor of its own from the graph's pool, and the call clears the
     counters at every replay: two graphs may be replayed at the same time.
     """
     if torch._C._cuda_isCurrentStreamCapturing():
@@ -191,6 +191,15 @@ def _workspace(kind, device, nbytes):
             if ws is None or ws.numel() < nbytes:
                 ws = _workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
     return ws, _lib.WS_COUNTERS_ZERO
+
+
+# A decode with weights is two launches, the second of which reads what the first left in the scratch.  No other host thread's
+# call on that scratch, with weights or without, may come between them: one thread at a time makes its launches.
+_launch_locks = [threading.Lock() for _ in range(61)]
+
+
+def _launch_lock(workspace):
+    return _launch_locks[(workspace.data_ptr() >> 8) % len(_launch_locks)]
 
 
 def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None, num_workers=0, workspace=None):
@@ -233,12 +242,12 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
         else:
             _check_workspace(workspace, device)
             nbytes, flag = workspace.numel() * workspace.element_size(), 0
-        rc = lib.cllo_kv8_decode_bf16(
-            q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-            seq_lens.data_ptr(), scale, out.data_ptr(), None if lse is None else lse.data_ptr(),
-            None if weights is None else weights.data_ptr(), workspace.data_ptr(), nbytes, B, cache.capacity, Hq, H, D,
-            cache.kv_layout | flag,
-            cache.block_tokens, cache.format, num_workers, _stream_ptr(device))
+        with _launch_lock(workspace):
+            rc = lib.cllo_kv8_decode_bf16(
+                q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+                seq_lens.data_ptr(), scale, out.data_ptr(), None if lse is None else lse.data_ptr(),
+                None if weights is None else weights.data_ptr(), workspace.data_ptr(), nbytes, B, cache.capacity, Hq, H, D,
+                cache.kv_layout | flag, cache.block_tokens, cache.format, num_workers, _stream_ptr(device))
     _lib.check(rc, "cllo_kv8_decode_bf16")
     return out
 

@@ -332,7 +332,8 @@ int cllo_kv8_append_bf16(const void* k_new, const long long k_strides[3], const 
  * weights (nullable, fp32 [B,Hkv,capacity]): the step's probabilities, summed over the query heads of each group, are
  * ADDED to weights[b,h,0..len).
  * workspace: cllo_kv8_decode_workspace_bytes(...) bytes, 256-byte aligned, contents arbitrary; calls that may overlap on
- * the GPU need one each.  kv_layout may carry CLLO_WS_COUNTERS_ZERO as in cllo_gqa_decode_bf16.  num_workers: 0 = chosen
+ * the GPU need one each.  With weights the call is two launches, the second reading what the first left in the workspace: where
+ * host threads share one, on one stream too, no call on it may begin before another thread's has returned.  kv_layout may carry CLLO_WS_COUNTERS_ZERO as in cllo_gqa_decode_bf16.  num_workers: 0 = chosen
  * by the library.
  */
 size_t cllo_kv8_decode_workspace_bytes(int B, int capacity, int Hq, int Hkv, int D, int with_weights, int num_workers);

@@ -1,6 +1,8 @@
 """The 8-bit KV cache operators at sizes, values and calls that are easy to get wrong."""
 import ctypes
 import math
+import threading
+import time
 
 import pytest
 import torch
@@ -91,3 +93,87 @@ def test_workspaces_that_a_kernel_could_not_write_are_refused(make):
         ops.kv8_decode(q, cache, _ints([64]), workspace=ws)
     with pytest.raises(ValueError, match="workspace"):
         ops.attention_weight_sums(q[:, :, None], q[:, :1, None], torch.zeros(1, 2, 1, device="cuda"), workspace=ws)
+
+
+def test_decode_with_weights_goes_through_its_launches_one_thread_at_a_time(monkeypatch):
+    """A call with weights is two launches that hand scores over in the stream's scratch: no other thread's call, with
+    weights or without, may come between them.  The library's function is replaced by one that notes who else is inside."""
+    ops = _ops()
+    from cuda_llm_ops_b200 import _lib
+    inside, met, entered, note = {}, [], [], threading.Lock()
+
+    class Library:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def cllo_kv8_decode_bf16(self, *args):
+            workspace = args[10]
+            with note:
+                met.append(inside.get(workspace, 0))
+                inside[workspace] = inside.get(workspace, 0) + 1
+                entered.append(workspace)
+            time.sleep(0.05)  # where the real one is between its launches
+            with note:
+                inside[workspace] -= 1
+            return _lib.OK
+
+    cache = ops.kv8_cache(2, 300, 2)
+    q = torch.zeros(2, 8, D, dtype=torch.bfloat16, device="cuda")
+    weights = [torch.zeros(2, 2, 300, device="cuda"), None, torch.zeros(2, 2, 300, device="cuda")]
+    lens = _ints([300, 7])
+    own = torch.zeros(1 << 23, dtype=torch.uint8, device="cuda")
+    real = _lib.load()
+    monkeypatch.setattr(_lib, "_lib", Library())
+    for workspace in (None, own):  # the stream's scratch, and one that the threads share
+        threads = [threading.Thread(target=ops.kv8_decode, args=(q, cache, lens), kwargs=dict(weights=w, workspace=workspace))
+                   for w in weights]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    assert len(entered) == 6 and len(set(entered)) == 2
+    assert met == [0] * 6
+
+
+def test_decode_with_weights_from_two_host_threads_on_one_stream():
+    """Both threads' weights are those of the same calls made one after the other, bit for bit."""
+    ops = _ops()
+    calls, lens = 500, [[900, 40], [33, 700, 512]]
+    busy = torch.zeros(8192, 8192, dtype=torch.bfloat16, device="cuda")
+    caches = [_filled_cache(400 + 10 * i, len(n), 1024, 2, E4M3, 1, 64, n) for i, n in enumerate(lens)]
+    qs = [torch.randn(len(n), 8, D, generator=_gen(430 + i), device="cuda").to(torch.bfloat16) for i, n in enumerate(lens)]
+    dev = [_ints(n) for n in lens]
+
+    def work(i, weights, outs):
+        for _ in range(calls):
+            outs.append(ops.kv8_decode(qs[i], caches[i], dev[i], weights=weights))
+
+    def run(together):
+        weights = [torch.zeros(len(n), 2, 1024, device="cuda") for n in lens]
+        outs = [[], []]
+        torch.cuda.synchronize()
+        for _ in range(30):  # the stream's queue runs full, so that the threads meet inside their launches
+            torch.mm(busy, busy)
+        start = threading.Barrier(2 if together else 1)
+
+        def thread(i):
+            start.wait()
+            work(i, weights[i], outs[i])
+        threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+            if not together:
+                t.join()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert all(len(o) == calls for o in outs)
+        return weights, outs
+
+    want, want_out = run(False)
+    for _ in range(3):
+        got, got_out = run(True)
+        for i in range(2):
+            assert torch.equal(got[i], want[i]), "thread %d: weights off by %g" % (i, (got[i] - want[i]).abs().max())
+            assert all(torch.equal(o.view(torch.int16), want_out[i][0].view(torch.int16)) for o in got_out[i])
+    assert_clean_status()
