@@ -53,7 +53,8 @@ constexpr int kKStages = 3, kQStages = 3, kLseStages = 16, kLseAhead = 8;
 constexpr int kSmemK = 0;
 constexpr int kSmemQ = kKStages * kTileBytes;
 constexpr int kSmemLse = kSmemQ + kQStages * kTileBytes;
-constexpr int kSmemBar = kSmemLse + kLseStages * kQ * 4;
+constexpr int kSmemDead = kSmemLse + kLseStages * kQ * 4;  // one bit per column: its row's lse is -inf, it adds nothing
+constexpr int kSmemBar = kSmemDead + kLseStages * (kQ / 8);
 constexpr int kNumBars = 2 * kKStages + 2 * kQStages + 2 * kLseStages + 4 * kTiles + 1;
 constexpr int kSmemHalf = kSmemBar + kNumBars * 8;  // the second warpgroup's sum of every key
 constexpr int kSmemMisc = kSmemHalf + kPair * 4;
@@ -255,6 +256,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
     float* lse_buf = reinterpret_cast<float*>(gen_base + sums::kSmemLse);
+    uint32_t* dead_buf = reinterpret_cast<uint32_t*>(gen_base + sums::kSmemDead);
     const uint32_t bar0 = base + sums::kSmemBar;
     auto k_full = [&](int s) { return bar0 + 8 * s; };
     auto k_empty = [&](int s) { return bar0 + 8 * (kKStages + s); };
@@ -451,16 +453,20 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     } else if (warp == kEpiWarps + 2) {
         // -------------------------------- lse loader --------------------------------
         // Copies the steps' lse values (four per lane) eight steps ahead, and turns each lane's own four into
-        // -lse * log2(e) once they have landed; -inf (no contribution) for rows that saw no key.  Values behind the last
-        // counted row are never looked at.
+        // -lse * log2(e) once they have landed.  A row with lse = -inf saw no key and adds nothing, whatever its query holds: its
+        // column's bit has the exponentials leave it out.  Values behind the last counted row are never looked at.
         int put = 0, got = 0;  // steps issued, steps handed over
         auto hand_over = [&]() {
             const int slot = got % kLseStages;
+            unsigned dead = 0u;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float* x = lse_buf + slot * kQ + e * 32 + lane;
-                *x = *x == -INFINITY ? -INFINITY : -*x * sums::kLog2e;
+                const unsigned word = __ballot_sync(0xffffffffu, *x == -INFINITY);
+                if (lane == e) dead = word;
+                *x = -*x * sums::kLog2e;
             }
+            if (lane < 4) dead_buf[slot * 4 + lane] = dead;
             mbar_arrive(lse_full(slot));
             ++got;
         };
@@ -531,6 +537,8 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                     __syncwarp();
                     tc_fence_after();
                     const float* nl = lse_buf + ls * kQ;
+                    const uint4 dead4 = *reinterpret_cast<const uint4*>(dead_buf + ls * 4);
+                    const bool dead = (dead4.x | dead4.y | dead4.z | dead4.w) != 0u;  // for all threads alike
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
                     // columns that count: from the warp's keys' own first ones up to i_hi
                     const int lo = own - j * kQ, hi = rows - j * kQ;
@@ -546,7 +554,7 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                         }
                     };
                     const int cols = 1 << head_shift, end = w.heads(p, g, head_shift) << head_shift;  // of a head, of all heads
-                    if (lo_last <= 0 && hi >= cols && end == kQ) {
+                    if (lo_last <= 0 && hi >= cols && end == kQ && !dead) {
 #pragma unroll
                         for (int c = 0; c < kQ; c += 32) {
                             float x[32];
@@ -560,13 +568,14 @@ weight_sums_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                             if (c >= hi || lo_first >= c + 32) continue;  // nothing for any key of the warp
                             float x[32];
                             tmem_ld32_wait(acc + at, x);
-                            if (lo_last <= c && hi >= c + 32) {
+                            if (lo_last <= c && hi >= c + 32 && !dead) {
                                 add_chunk(x, nl + at);
                                 continue;
                             }
                             // bit e: the chunk's column e counts for this key.  What does not count may be anything, NaN too
                             const uint32_t seen = (lo <= c ? 0xffffffffu : lo < c + 32 ? 0xffffffffu << (lo - c) : 0u) &
-                                                  (hi >= c + 32 ? 0xffffffffu : (1u << (hi - c)) - 1u);
+                                                  (hi >= c + 32 ? 0xffffffffu : (1u << (hi - c)) - 1u) &
+                                                  ~dead_buf[ls * 4 + at / 32];
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
                                 const float y = fmaf(x[e], scale, nl[at + e]);

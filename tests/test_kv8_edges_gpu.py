@@ -9,7 +9,7 @@ import torch
 
 import kv8_ref as ref
 from gpu_util import assert_clean_status
-from test_kv8_gpu import _check_evict, _filled_cache, _gen, _garbage_cache, _ints, _ops
+from test_kv8_gpu import SCALE, _check_evict, _check_sums, _filled_cache, _gen, _garbage_cache, _ints, _ops
 
 pytestmark = pytest.mark.gpu
 D = 128
@@ -176,4 +176,28 @@ def test_decode_with_weights_from_two_host_threads_on_one_stream():
         for i in range(2):
             assert torch.equal(got[i], want[i]), "thread %d: weights off by %g" % (i, (got[i] - want[i]).abs().max())
             assert all(torch.equal(o.view(torch.int16), want_out[i][0].view(torch.int16)) for o in got_out[i])
+    assert_clean_status()
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# weight sums: rows that saw nothing
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("causal,window,group", [(False, None, 2), (True, None, 2), (True, 64, 4), (True, 20, 3), (False, 100, 1)])
+def test_weight_sums_of_rows_without_keys_whose_queries_are_not_finite(causal, window, group):
+    """lse = -inf says that a row saw no key (padding, a mask that left nothing): it adds nothing, whatever its query holds."""
+    ops = _ops()
+    B, H, S = 2, 2, 400
+    q = torch.randn(B, group * H, S, D, generator=_gen(1), device="cuda").to(torch.bfloat16)
+    k = torch.randn(B, H, S, D, generator=_gen(2), device="cuda").to(torch.bfloat16)
+    s = SCALE * q.float().view(B, H, -1, S, D) @ k.float()[:, :, None].transpose(-1, -2)
+    if causal:
+        s = s.masked_fill(torch.ones(S, S, dtype=torch.bool, device="cuda").triu(1), -math.inf)
+    lse = s.logsumexp(-1).view(B, group * H, S)
+    clean = q.clone()
+    for row, value in ((5, math.nan), (127, math.inf), (128, -math.inf), (255, math.nan), (383, math.nan), (390, math.inf), (399, math.nan)):
+        q[0, :, row], lse[0, :, row], clean[0, :, row] = value, -math.inf, 0
+    q[1, 0, 390, 3], lse[1, 0, 390], clean[1, 0, 390] = math.nan, -math.inf, 0  # of one head, in one place
+    q[1, -1], lse[1, -1], clean[1, -1] = math.nan, -math.inf, 0                 # a whole head
+    got = ops.attention_weight_sums(q, k, lse, causal=causal, window=window)
+    _check_sums(got, clean, k, lse, SCALE, causal, window=window)
     assert_clean_status()
