@@ -441,7 +441,7 @@ static int evict_launch(const void* k, const void* v, const float* k_scale, cons
         !aligned_to(k_scale_to, 4) || !aligned_to(v_scale_to, 4) || !aligned_to(weights_to, 4) || !aligned_to(new_lens, 4) ||
         !aligned_to(indices, 4))
         return CLLO_E_BAD_ARG;
-    if (capacity > kMaxCapacity || capacity_to > kMaxCapacity) return CLLO_E_UNSUPPORTED;
+    if (capacity > kMaxCapacity || capacity_to > kMaxCapacity || budget > kMaxCapacity) return CLLO_E_UNSUPPORTED;
     const size_t rows = static_cast<size_t>(B) * Hkv;
     const size_t n = rows * capacity * kD, n_to = rows * capacity_to * kD;
     const size_t n_scale = rows * ((capacity + block - 1) / block) * 4, n_scale_to = rows * ((capacity_to + block - 1) / block) * 4;

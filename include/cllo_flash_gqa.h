@@ -362,8 +362,8 @@ int cllo_attn_weight_sums_bf16(const void* q, const void* k, const float* lse, c
 
 /*
  * Eviction by accumulated weight.  Per (batch, kv head) the cache's first `sink` and last `recent` tokens stay, and of the
- * others the budget - sink - recent with the largest weights[b,h,t] (of equal weights the earliest; NaN counts as
- * largest); a sequence within the budget stays whole.  What stays moves, in order, to the second cache (same layout, block
+ * others the budget - sink - recent (budget <= 2^30) with the largest weights[b,h,t] (of equal weights the earliest; NaN
+ * counts as largest); a sequence within the budget stays whole.  What stays moves, in order, to the second cache (same layout, block
  * size and format; capacity_to >= min(budget, capacity)), whose block scales are computed anew; weights_to (nullable,
  * [B,Hkv,capacity_to]) receives the kept weights, indices [B,Hkv,budget] the kept positions (-1 behind them) and
  * new_lens [B] = min(seq_lens, budget).  Rows behind new_lens are left as they were.  No tensor written to may overlap one

@@ -62,3 +62,17 @@ def test_workspaces_that_a_kernel_could_not_write(built_library):
                       (4096, cpu)):
         with pytest.raises(ValueError, match="workspace"):
             kv8._check_workspace(t, device)
+
+
+def test_evict_refuses_budgets_beyond_what_its_counts_hold(built_library):
+    """Positions are counted in 32 bits, in steps of several thousand: a budget near 2^31 would carry them past it."""
+    from cuda_llm_ops_b200 import _lib
+    lib = _lib.load()
+    place = [(i + 1) << 40 for i in range(len(READ) + len(WRITTEN))]
+
+    def evict(budget):
+        return lib.cllo_kv8_evict(*place, 1, 64, 64, 1, 128, budget, 0, 0, 1, 16, 0, None)
+    for budget in ((1 << 30) + 1, (1 << 31) - 8192, (1 << 31) - 1):
+        assert evict(budget) == _lib.E_UNSUPPORTED, budget
+    if not torch.cuda.is_available():
+        assert evict(1 << 30) not in (_lib.OK, _lib.E_UNSUPPORTED, _lib.E_BAD_ARG)  # no device
