@@ -340,6 +340,10 @@ def kv8_evict(cache, weights, seq_lens, budget, sink=0, recent=0, out=None, out_
     new cache of ``budget`` tokens; it must not share memory with ``cache``), the kept weights to ``out_weights``
     (fp32 [B,Hkv,capacity of out]; default: new, zero behind the kept ones).  ``indices`` int32 [B,Hkv,budget] are the
     kept positions, -1 behind them; the returned lengths are ``min(seq_lens, budget)``.
+
+    A sequence that was cut fills the default ``out``, and ``kv8_append`` stores nothing beyond a cache's capacity: where tokens
+    are to follow, pass an ``out`` with room for them.  Of a given ``out`` and ``out_weights`` what lies behind the kept tokens is
+    left as it was: zero ``out_weights`` before the call where ``kv8_decode`` is to add to it afterwards.
     """
     _require_cuda(cache)
     device = cache.k.device

@@ -9,7 +9,8 @@ import torch
 
 import kv8_ref as ref
 from gpu_util import assert_clean_status
-from test_kv8_gpu import SCALE, _check_evict, _check_sums, _filled_cache, _gen, _garbage_cache, _ints, _ops
+from test_kv8_gpu import (SCALE, _bits, _check_decode, _check_evict, _check_sums, _filled_cache, _garbage_cache, _gen, _ints,
+                          _ops)
 
 pytestmark = pytest.mark.gpu
 D = 128
@@ -201,3 +202,50 @@ def test_weight_sums_of_rows_without_keys_whose_queries_are_not_finite(causal, w
     got = ops.attention_weight_sums(q, k, lse, causal=causal, window=window)
     _check_sums(got, clean, k, lse, SCALE, causal, window=window)
     assert_clean_status()
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# eviction and what follows it
+# ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+def test_two_caches_and_two_weight_tensors_in_turn(dtype):
+    """Evictions between two caches, the second weight tensor zeroed before each: a token that is appended afterwards starts with
+    no weight, whatever its place held before, and is attended to."""
+    ops = _ops()
+    B, H, Hq, cap, budget = 2, 2, 8, 160, 100
+    lens = [160, 90]
+    caches = [_filled_cache(500, B, cap, H, dtype, 1, 32, lens), _garbage_cache(501, B, cap, H, dtype, 1, 32)]
+    weights = [torch.rand(B, H, cap, generator=_gen(502), device="cuda"), torch.full((B, H, cap), 3.0, device="cuda")]
+    dev = _ints(lens)
+    for turn in range(3):
+        held, before = dev.tolist(), [t.view(torch.uint8).clone() for t in (caches[1].k, caches[1].v)]
+        weights[1].zero_()
+        result = ops.kv8_evict(caches[0], weights[0], dev, budget, sink=2, recent=20, out=caches[1], out_weights=weights[1])
+        _check_evict(caches[0], weights[0], held, budget, 2, 20, result, before)
+        caches.reverse()
+        weights.reverse()
+        dev = result[2].clone()
+        for step in range(3):
+            new = [torch.randn(B, H, 1, D, generator=_gen(510 + 9 * turn + 3 * step + i), device="cuda").to(torch.bfloat16)
+                   for i in range(2)]
+            ops.kv8_append(caches[0], *new, dev)
+            dev = dev + 1
+            q = torch.randn(B, Hq, D, generator=_gen(512 + 9 * turn + 3 * step), device="cuda").to(torch.bfloat16)
+            base = weights[0].clone()
+            at = dev.long() - 1
+            assert (base[torch.arange(B, device="cuda"), :, at] == 0).all(), "the new token brings weight along"
+            out = ops.kv8_decode(q, caches[0], dev, weights=weights[0])
+            _check_decode(caches[0], q, dev, SCALE, out, added=(base, weights[0]))
+    assert_clean_status()
+
+
+def test_the_cache_that_eviction_makes_has_no_room_and_one_with_room_takes_the_next_token():
+    ops = _ops()
+    cache = _filled_cache(520, 1, 100, 2, torch.int8, 1, 32, [100])
+    weights = torch.rand(1, 2, 100, generator=_gen(521), device="cuda")
+    row = torch.randn(1, 2, 1, D, generator=_gen(522), device="cuda").to(torch.bfloat16)
+    for out, stored in ((None, False), (ops.kv8_cache(1, 64, 2, torch.int8, 1, 32), True)):
+        kept, _, lens, _ = ops.kv8_evict(cache, weights, _ints([100]), 50, out=out)
+        before = _bits(kept)
+        ops.kv8_append(kept, row, row, lens)
+        assert all(torch.equal(a, b) for a, b in zip(before, _bits(kept))) != stored
