@@ -8,8 +8,10 @@
 //
 // Bound by memory: 2 B read and 1 B written per value.  The new rows are loaded once, 16 bytes per lane (half a warp per
 // row), and wait in registers for the block's amax, while the next cache block's rows are already on their way: 4 prompts of
-// 16384 tokens, 8 kv heads, 68 us, 5.9 TB/s (0.90 of a copy).  One token each for 60 sequences: 5 us, the latency of
-// lengths, rows and two barriers.
+// 16384 tokens, 8 kv heads, e4m3: 74 us per call, 5.5 TB/s (0.83 of a copy); 69 us in a graph.  int8 81 us in a graph, 0.75: a
+// code takes a conversion, two bounds and its place in the word, where e4m3 has one instruction for two; lengths that
+// differ cost nothing (16 sequences of 0 to 8192 tokens 85 us, of 4096 each 85).  One token each for 60 sequences: 5 us in a graph,
+// the latency of lengths, rows and two barriers; 11 per call, the host.
 #pragma once
 
 #include "host_util.cuh"
@@ -178,7 +180,8 @@ static int append_launch(const void* k_new, const long long* k_strides, const vo
     const int touched = (T - 1 + block - 1) / block + 1;
     p.blocks_touched = touched < p.n_blocks ? touched : p.n_blocks;
     // Cache blocks per thread block: several, one loading while the one before it is turned into codes, where there are enough
-    // to fill the GPU all the same (4 prompts of 16384 tokens: 68.4 us with up to 8, 72.9 with one each; smaller calls get one).
+    // to fill the GPU all the same (4 prompts of 16384 tokens, in a graph: 68.4 us with up to 8, 72.9 with one each; smaller calls get
+    // one).
     const long long per_cta = static_cast<long long>(B) * Hkv * p.blocks_touched * 2 / (static_cast<long long>(di->sm_count) * 16);
     p.per_cta = static_cast<int>(per_cta < 1 ? 1 : (per_cta > 8 ? 8 : per_cta));
     const long long blocks = static_cast<long long>(B) * Hkv * ((p.blocks_touched + p.per_cta - 1) / p.per_cta);

@@ -5,10 +5,12 @@
 // over the seq_lens[b] tokens that the cache holds of sequence b; with `weights`, the probabilities of the step are
 // added to weights[b, kv head, t], summed over the query heads of the group in a fixed order.
 //
-// Measured: 60 x 4096 tokens, 128/8 heads, e4m3, tokens before heads: 97 us, 5.2 TB/s (0.80 of a copy), bound by the memory
-// system (the same copies without arithmetic: 96 us); 1,048,576 tokens, 64/8 heads, int8: 332 us, 0.99 of a copy; 17 sequences
-// of 0 to 16384 tokens, 40/8 heads, with weights: 57 us, 4.2 TB/s, bound by issue and by what short units cost; one sequence
-// of 1024 tokens: 14 us, a chain of latencies.
+// Measured, per call, calls back to back: 60 x 4096 tokens, 128/8 heads, e4m3, tokens before heads: 103 us, 4.9 TB/s (0.75 of a
+// copy; 99 us in a graph), bound by the memory system (the same copies without arithmetic, in a graph: 97 us; heads before
+// tokens 91 and 83); 1,048,576 tokens, 64/8 heads, int8: 414 us, 0.79 of a copy, under the power cap (ten calls in a row 333 us);
+// 17 sequences of 0 to 16384 tokens, 40/8 heads, with weights: 58 us, 4.1 TB/s, bound by issue and by what short units cost;
+// one sequence of 1024 tokens: 15 us (13 in a graph), a chain of latencies.  Groups above 16 heads are several units, each of which
+// copies and converts the cache for itself: 16 x 16384 tokens, 8 kv heads, e4m3: 91 us with groups of 16, 163 with 20 or 32.
 //
 // Work decomposition, as in the bf16 decode kernel (gqa_decode.cuh): a unit is one (sequence, kv head, block of <= 16
 // query heads), cut into tiles of 64 tokens (at least one, so that an empty sequence writes its zeros); the tiles of all
@@ -29,7 +31,9 @@
 //   * the V codes become f16 for m16n8k16, and the V scale goes into the exponent: with lv = log2 vscale,
 //     p'_t = 2^(s_t + lv_t - m + 11), m = max(s_t + lv_t), so that O = sum p' v8 needs no scaling and
 //     l = sum p'_t / vscale_t.  p' is rounded to f16 for the product (half a step: 2^-11 relative, 2^-25 absolute below f16's
-//     normal range), l is summed in fp32 before rounding.  The reference m may lag behind the true maximum by 2^4 (kLazy),
+//     normal range), l is summed in fp32 before rounding; three more bits than the bf16 that the output is rounded to, whose
+//     rounding is all that shows against 64 bits (1.7e-3 rms, as with fp32 probabilities; some outputs land a bf16 step
+//     from where fp32 probabilities put them, 5e-4 rms).  The reference m may lag behind the true maximum by 2^4 (kLazy),
 //     so the largest p' lies in [2^11, 2^15] and the absolute part is at most 2^-36 of it.
 //
 // Layout without transposes.  K: a lane reads 32 consecutive bytes of its token's row as the B operand; the k index may be
@@ -82,13 +86,16 @@ constexpr int kSmemShare = kSmemMisc + 32;
 constexpr int kDecodeSmemBytes = kSmemShare + 64 + 1024;
 static_assert(kDecodeSmemBytes <= 227 * 1024, "shared memory of a block");
 // What a unit costs beyond its tiles (its query rows, the merge of the eight states, the output), in tiles.  The shares of
-// the blocks are cut in these units, so that a block that gets many short sequences is not the last one to finish: 17
-// sequences of 0 to 16384 tokens, 8 kv heads: 81 us at 0, 61 at 4, 55 at 6, 49 at 12, 53 at 16; no effect on full batches.
+// the blocks are cut in these units, so that a block that gets many short sequences is not the last one to finish: 17 sequences
+// of 0 to 16384 tokens, 8 kv heads, groups of 5: 57.5 us at 0, 48.9 at 4, 47.1 at 8, 46.9 at 10, 46.8 at 12, 46.9 at 14, 47.1 at 16
+// (groups of 4, 8 and 16 likewise, 8 to 14 within 2 %); 64 of 0 to 2048, 4 kv heads, groups of 8: 37.7, 31.1, 26.9, 26.9, 26.9, 27.1,
+// 28.5; 33 of 0 to 8192, 2 kv heads, groups of 16: 26.9, 24.8, 23.7, then 22.8.  No effect on full batches.
 // Held to the tiles that a block gets on average: where there are fewer than that, spreading the tiles comes first.
 constexpr int kUnitCost = 10;
 // A unit that many blocks share (one long sequence, few kv heads) is merged in two steps, kFan pieces each: one block that
-// reads 148 pieces of 16 rows takes longer than the attention (16384 tokens of one kv head, 148 blocks: 41 us in one
-// step, 22.5 in two).  Up to kFlatPieces one step is as fast: the second costs another round of arrivals.
+// reads 148 pieces of 16 rows takes longer than the attention (16384 tokens of one kv head, 148 blocks: 41.7 us in one
+// step, 22.3 in two; with 4, 8, 16 or 24 pieces each 24.5, 21.7, 22.5, 20.6; two kv heads, 74 blocks each: 24.7 in one step, 18.4 in
+// two of any of these).  Up to kFlatPieces one step is as fast (24 pieces 16.3 us either way).
 constexpr int kFlatPieces = 24, kFan = 12;
 constexpr int kMaxWorkers = 512;  // two sets of arrival counters in the first 4 KB of the workspace
 static_assert(2 * kMaxWorkers <= decode::kFixedCounters, "the counters' place in the workspace");
@@ -817,7 +824,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
 // weights[b, h, t] += sum over the group's heads, in order, of 2^(score - lse2); one thread per token.  A kernel of its own since
 // a probability needs the normaliser of the whole sequence; the scores are 4 B per query head and token, mostly still in L2
-// (17 sequences of 0 to 16384 tokens, 40 heads: 8 us of the 57).
+// (17 sequences of 0 to 16384 tokens, 40 heads: 47 us without weights, 59 with).
 constexpr int kWeightThreads = 256, kWeightTok = 1024;
 __global__ void __launch_bounds__(kWeightThreads) decode_weights_kernel(const DecodeParams p, float* weights, int n_chunks) {
     pdl_wait_prior_grid();  // scores and normalisers; by every block, so that this grid never ends before the decode's

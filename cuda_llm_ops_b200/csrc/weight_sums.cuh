@@ -22,9 +22,13 @@
 // block works out its share for itself, in closed form per sequence.  A unit cut between blocks leaves one fp32 partial per
 // key and block; the last block to arrive adds them up in block order.
 //
-// Measured: all queries of 8192 tokens, 32/4 heads: 308 us alone, 331 in a row under the power cap, 830 TFLOP/s; bound by the
-// exponentials (1.07 G of them are 240 us at the special-function units' rate, 0.83 busy).  The last 64 queries of 4 prompts of
-// 4307 to 8030 tokens, 32/8 heads: 31 us; bound by what a unit of two steps costs besides them.
+// Measured, per call, calls back to back: all queries of 8192 tokens, 32/4 heads: 339 us under the power cap, 820 TFLOP/s (305 us
+// in short runs); bound by the exponentials (1.07 G of them are 240 us at the special-function units' rate, 0.83 busy).  The last 64
+// queries of 4 prompts of 4307 to 8030 tokens, 32/8 heads: 31 us; bound by what a unit of two steps costs besides them.
+//
+// Rounding: scores, terms and sums are fp32, the exponential is the hardware's approximation (2^-22 relative); a key's terms go into
+// four running sums per step, these into one over the unit's steps, and those of a cut unit are added in block order.  Over all
+// queries of 8192 tokens, groups of 8: 8.9e-8 rms from 64 bits (an fp32 product, exponential and sum: 4.9e-8).
 //
 // Warps: 0-15 the exponentials, one key per thread -- warpgroups 0 and 2 key tile 0, 1 and 3 key tile 1, taking its
 // steps in turn: four warps per scheduler, so that one's tensor-memory load hides behind the others' exponentials -- 16 Q
@@ -46,6 +50,10 @@ constexpr int kQ = 128;                                          // queries per 
 constexpr int kTurns = 2;                                        // warpgroups per key tile: they take its steps in turn
 constexpr int kEpiWarps = kTiles * kTurns * 4;
 constexpr int kThreads = (kEpiWarps + 4) * 32;
+// What a unit costs by itself, in steps.  At least one: a unit that no query sees has a cell, whose holder clears its sums.  With 1, 2,
+// 3 and 4: all queries of 8192 tokens 305, 305, 305 and 306 us; a window of 64 of 4 prompts of 4096 to 8192 tokens (groups of 4)
+// 37.3, 35.5, 35.3, 35.3; of 16 of 1024 to 2048 (groups of 8) 33.9, 33.5, 35.1, 35.2; all queries of 8 of 512 to 1024 44.3, 46.7,
+// 47.3, 47.6.
 constexpr int kUnitCost = 2;
 constexpr int kSlabBytes = 128 * 128;         // [128 rows][64 dims] bf16, one swizzled slab
 constexpr int kTileBytes = 2 * kSlabBytes;

@@ -208,6 +208,10 @@ def kv8_decode(q, cache, seq_lens, scale=None, out=None, lse=None, weights=None,
     ``q`` [B,Hq,D] bf16, ``seq_lens`` int32 [B] tokens per sequence (0 gives zeros), ``lse`` (fp32 [B,Hq], optional) is
     filled with the log-sum-exp of the scores.  ``weights`` (fp32 [B,Hkv,capacity], optional): the step's probabilities,
     summed over the query heads of each group, are added to it -- what ``kv8_evict`` goes by.
+
+    Eager calls keep their scratch per (device, stream) for the life of the process; with ``weights`` it holds 4 bytes per query
+    head and token of the capacity.  ``workspace`` (contiguous, on the cache's device, of
+    ``cllo_kv8_decode_workspace_bytes`` bytes) takes its place; calls that may overlap on the GPU need one each.
     """
     _require_cuda_bf16("q", q)
     _require_cuda(cache)
@@ -280,7 +284,8 @@ def attention_weight_sums(q, k, lse, scale=None, causal=True, q_start=0, seq_len
     with q [B,Hq,Sq,D], k [B,Hkv,Skv,D] bf16 and the forward's ``lse`` [B,Hq,Sq] fp32; ``causal`` keeps
     t <= q_start + i.  ``seq_lens`` (int32 [B], optional): real lengths of a padded batch -- keys behind them get 0 and,
     under a causal mask, query rows behind them do not count.  ``window``: only the last ``window`` query positions
-    of each sequence count (default: all).  ``accumulate=True`` adds to ``out``.
+    of each sequence count (default: all); without lengths or without a causal mask these are the last rows of ``q``.  Rows with
+    ``lse`` = -inf add nothing.  ``accumulate=True`` adds to ``out``.  ``q`` and ``k`` are copied where they are not contiguous.
     """
     _require_cuda_bf16("q", q)
     _require_cuda_bf16("k", k)

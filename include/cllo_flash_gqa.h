@@ -333,8 +333,11 @@ int cllo_kv8_append_bf16(const void* k_new, const long long k_strides[3], const 
  * ADDED to weights[b,h,0..len).
  * workspace: cllo_kv8_decode_workspace_bytes(...) bytes, 256-byte aligned, contents arbitrary; calls that may overlap on
  * the GPU need one each.  With weights the call is two launches, the second reading what the first left in the workspace: where
- * host threads share one, on one stream too, no call on it may begin before another thread's has returned.  kv_layout may carry CLLO_WS_COUNTERS_ZERO as in cllo_gqa_decode_bf16.  num_workers: 0 = chosen
- * by the library.
+ * host threads share one, on one stream too, no call on it may begin before another thread's has returned.  With weights it holds
+ * 4 bytes per query head and token of the capacity, whatever the lengths.
+ * kv_layout may carry CLLO_WS_COUNTERS_ZERO as in cllo_gqa_decode_bf16.  num_workers: 0 = chosen by the library.
+ * Scores have to stay within fp32's range: beyond it outputs may be NaN.  The probabilities enter the product with V as f16
+ * (2^-11 relative), scores, normalisers, weights and accumulators are fp32.
  */
 size_t cllo_kv8_decode_workspace_bytes(int B, int capacity, int Hq, int Hkv, int D, int with_weights, int num_workers);
 int cllo_kv8_decode_bf16(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
