@@ -679,7 +679,8 @@ def device_status():
     rc = _lib.load().cllo_device_status(detail)
     if rc != 0:
         # a kernel gave up half-way: the cached workspaces may hold counts of pieces that never got merged
-        with _workspaces_lock:
+        # (inference mode: a scratch that a call made under it can be written to under it only)
+        with _workspaces_lock, torch.inference_mode():
             for cached in _counted_workspaces:
                 for ws in list(cached.values()):
                     ws.zero_()

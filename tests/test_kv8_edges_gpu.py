@@ -249,3 +249,42 @@ def test_the_cache_that_eviction_makes_has_no_room_and_one_with_room_takes_the_n
         before = _bits(kept)
         ops.kv8_append(kept, row, row, lens)
         assert all(torch.equal(a, b) for a, b in zip(before, _bits(kept))) != stored
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# after a kernel that gave up
+# ------------------------------------------------------------------------------------------------------------------
+class _GaveUp:
+    """The library, whose next status says that a kernel gave up half-way (none did)."""
+
+    def __init__(self, real):
+        self.real = real
+
+    def __getattr__(self, name):
+        return getattr(self.real, name)
+
+    def cllo_device_status(self, detail):
+        return -6
+
+
+def test_status_after_calls_in_inference_mode(monkeypatch):
+    """Scratch that a call made in inference mode is cleared like any other."""
+    ops = _ops()
+    from cuda_llm_ops_b200 import _lib, kv8
+    cache = _filled_cache(600, 1, 300, 2, E4M3, 1, 64, [300])
+    q = torch.randn(1, 8, D, generator=_gen(601), device="cuda").to(torch.bfloat16)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.inference_mode(), torch.cuda.stream(stream):
+        want = ops.kv8_decode(q, cache, _ints([300]))
+    torch.cuda.synchronize()
+    scratch = kv8._workspaces[("decode", 0, stream.cuda_stream)]
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "_lib", _GaveUp(_lib.load()))
+        assert ops.device_status()[0] == -6
+    torch.cuda.synchronize()
+    assert (scratch == 0).all()
+    with torch.cuda.stream(stream):
+        again = ops.kv8_decode(q, cache, _ints([300]))
+    torch.cuda.synchronize()
+    assert torch.equal(again.view(torch.int16), want.view(torch.int16))
