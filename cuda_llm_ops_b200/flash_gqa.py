@@ -673,15 +673,19 @@ def LaunchRopeBf16Kernel(input, output, batchSize, seqLen, hiddenDim, base=10000
 
 
 def device_status():
-    """Synchronise and return (status, detail) from ``cllo_device_status``."""
+    """Synchronise and return (status, detail) of the current device from ``cllo_device_status``."""
     import ctypes
     detail = (ctypes.c_int * 4)()
     rc = _lib.load().cllo_device_status(detail)
     if rc != 0:
-        # a kernel gave up half-way: the cached workspaces may hold counts of pieces that never got merged
+        # a kernel gave up half-way: this device's cached workspaces may hold counts of pieces that never got merged
         # (inference mode: a scratch that a call made under it can be written to under it only)
         with _workspaces_lock, torch.inference_mode():
-            for cached in _counted_workspaces:
-                for ws in list(cached.values()):
+            kept = [ws for cached in _counted_workspaces for ws in list(cached.values())]
+            here = torch.cuda.current_device() if kept else None
+            for ws in kept:
+                if ws.is_cuda and ws.device.index == here:
                     ws.zero_()
+            if kept:
+                torch.cuda.synchronize()  # some are another stream's, whose next call must find them cleared
     return rc, list(detail)

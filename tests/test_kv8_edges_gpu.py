@@ -288,3 +288,33 @@ def test_status_after_calls_in_inference_mode(monkeypatch):
         again = ops.kv8_decode(q, cache, _ints([300]))
     torch.cuda.synchronize()
     assert torch.equal(again.view(torch.int16), want.view(torch.int16))
+
+
+def test_status_clears_every_streams_scratch_before_it_returns(monkeypatch):
+    """Scratch is kept per stream: a call on another stream, made right after the status, finds no counts of lost pieces."""
+    ops = _ops()
+    from cuda_llm_ops_b200 import _lib, kv8
+    cache = _filled_cache(610, 1, 300, 2, E4M3, 1, 64, [300])
+    q = torch.randn(1, 8, D, generator=_gen(611), device="cuda").to(torch.bfloat16)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        ops.kv8_decode(q, cache, _ints([300]))
+    torch.cuda.synchronize()
+    scratch = kv8._workspaces[("decode", 0, stream.cuda_stream)]
+    scratch[:4096].fill_(1)
+    elsewhere = torch.ones(4096, dtype=torch.uint8)  # of a device that was not asked about
+    busy = torch.zeros(8192, 8192, dtype=torch.bfloat16, device="cuda")
+    torch.mm(busy, busy)
+    torch.cuda.synchronize()
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "_lib", _GaveUp(_lib.load()))
+        m.setitem(kv8._workspaces, ("decode", 99, 0), elsewhere)
+        for _ in range(30):
+            torch.mm(busy, busy)
+        assert ops.device_status()[0] == -6
+    with torch.cuda.stream(stream):
+        found = scratch[:4096].clone()
+    torch.cuda.synchronize()
+    assert (found == 0).all()
+    assert (elsewhere == 1).all()
