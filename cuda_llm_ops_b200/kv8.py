@@ -94,7 +94,8 @@ def kv8_cache(batch, capacity, num_kv_heads, dtype=torch.float8_e4m3fn, kv_layou
     if block_tokens not in BLOCK_TOKENS:
         raise ValueError("block_tokens must be one of %s" % (BLOCK_TOKENS,))
     k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for _ in range(2))
-    ks, vs = (torch.zeros((batch, num_kv_heads, -(-capacity // block_tokens)), device=device) for _ in range(2))
+    scales = (batch, num_kv_heads, -(-capacity // block_tokens))
+    ks, vs = (torch.zeros(scales, dtype=torch.float32, device=device) for _ in range(2))
     return KV8Cache(k, v, ks, vs, kv_layout, block_tokens)
 
 

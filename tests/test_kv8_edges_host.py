@@ -76,3 +76,16 @@ def test_evict_refuses_budgets_beyond_what_its_counts_hold(built_library):
         assert evict(budget) == _lib.E_UNSUPPORTED, budget
     if not torch.cuda.is_available():
         assert evict(1 << 30) not in (_lib.OK, _lib.E_UNSUPPORTED, _lib.E_BAD_ARG)  # no device
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_caches_under_another_default_dtype(default):
+    """Serving programs set torch's default dtype to their model's; the scales are fp32 all the same."""
+    import cuda_llm_ops_b200 as ops
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        cache = ops.kv8_cache(2, 100, 3, device="cpu")
+    finally:
+        torch.set_default_dtype(before)
+    assert cache.k_scale.dtype is torch.float32 and cache.v_scale.dtype is torch.float32
