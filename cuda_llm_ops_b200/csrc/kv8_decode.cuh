@@ -34,7 +34,8 @@
 //     normal range), l is summed in fp32 before rounding; three more bits than the bf16 that the output is rounded to, whose
 //     rounding is all that shows against 64 bits (1.7e-3 rms, as with fp32 probabilities; some outputs land a bf16 step
 //     from where fp32 probabilities put them, 5e-4 rms).  The reference m may lag behind the true maximum by 2^4 (kLazy),
-//     so the largest p' lies in [2^11, 2^15] and the absolute part is at most 2^-36 of it.
+//     so the largest p' lies in [2^11, 2^15] and the absolute part is at most 2^-36 of it.  Below 2^-126 a p' is 0: with V
+//     scales 2^120 apart that takes a probability below 2^-16 of the other token's.
 //
 // Layout without transposes.  K: a lane reads 32 consecutive bytes of its token's row as the B operand; the k index may be
 // permuted freely as long as Q uses the same permutation.  V: the transposing 8-bit load hands a lane four tokens of one

@@ -336,7 +336,8 @@ int cllo_kv8_append_bf16(const void* k_new, const long long k_strides[3], const 
  * host threads share one, on one stream too, no call on it may begin before another thread's has returned.  With weights it holds
  * 4 bytes per query head and token of the capacity, whatever the lengths.
  * kv_layout may carry CLLO_WS_COUNTERS_ZERO as in cllo_gqa_decode_bf16.  num_workers: 0 = chosen by the library.
- * Scores have to stay within fp32's range: beyond it outputs may be NaN.  The probabilities enter the product with V as f16
+ * Scores have to stay within fp32's range: beyond it outputs may be NaN.  A token whose probability times V scale is more than
+ * 2^136 below the sequence's largest counts for nothing, in the normaliser too.  The probabilities enter the product with V as f16
  * (2^-11 relative), scores, normalisers, weights and accumulators are fp32.
  */
 size_t cllo_kv8_decode_workspace_bytes(int B, int capacity, int Hq, int Hkv, int D, int with_weights, int num_workers);
